@@ -650,7 +650,7 @@ def _dev_synth_lib():
         tools = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tools")
         so, src = os.path.join(tools, "libsynth_fill_hip.so"), os.path.join(tools, "synth_fill_hip.hip")
         if not os.path.exists(so) or os.path.getmtime(so) < os.path.getmtime(src):
-            subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-o", so, src],
+            subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared", "-fPIC", "-o", so, src],
                            check=True, capture_output=True)
         lib = ctypes.CDLL(so)
         lib.synth_fill_hip.restype = None

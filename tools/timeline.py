@@ -20,7 +20,7 @@ SO = os.path.join(ROOT, "tools", f"libcalm_hip_tl{'_' + TAG if TAG else ''}{'' i
 src = os.path.join(ROOT, "calm_amd", "csrc", "infer_hip.hip")
 deps = [os.path.join(ROOT, "calm_amd", "csrc", f) for f in os.listdir(os.path.join(ROOT, "calm_amd", "csrc"))]
 if not os.path.exists(SO) or os.path.getmtime(SO) < max(os.path.getmtime(d) for d in deps):
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-DCALM_TIMELINE", *DEFS, *(["-mllvm", "-amdgpu-kernarg-preload-count=14"] if PRELOAD else []),
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-fPIC", "-DCALM_TIMELINE", *DEFS, *(["-mllvm", "-amdgpu-kernarg-preload-count=14"] if PRELOAD else []),
                     "-shared", "-o", SO, src], check=True)
 if "--build-only" in sys.argv:
     sys.exit(0)
