@@ -13,7 +13,9 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <atomic>
 #include <map>
+#include <mutex>
 #include <string>
 #include <tuple>
 #include <type_traits>
@@ -22,6 +24,8 @@
 #include "../../include/calm_hip.h"
 #include "kernels.hip.h"
 #include "prefill.hip.h"
+#include "paged.hip.h"
+#include "beam.hip.h"
 
 using namespace calm;
 
@@ -2589,6 +2593,10 @@ extern "C" double perf_stage_hip(struct Transformer* t, int stage, int iters, ui
 	}
 	return (double)ms * 1e3 / ((double)iters * c->n_layers);
 }
+
+// ---------------------------------------------------------------- paged cache, beam selection ----
+
+#include "paged_api.hip.h"
 
 #ifdef CALM_TIMELINE
 // tools/timeline.py only (a separate build with -DCALM_TIMELINE): arm / read the per-wave stamps of kernels.hip.h

@@ -1,0 +1,1401 @@
+// paged.hip.h -- a cache of several sequences in pages of 8-bit codes, and the kernels that fill, read, share and move them.
+//
+// Layout (struct KvPool, include/calm_hip.h).  A page holds KV_PAGE = 64 tokens of one sequence for every layer and kv head:
+//   K codes  [page][kv head][token 64][dim]                              int8, a token's dims contiguous
+//   V codes  [page][kv head][quad 4][dim][block 4][token 4]               int8: quad g of a dim holds tokens 4 g .. 4 g + 3 of each of
+//                                                                         the page's four blocks -- the 16 bytes one lane feeds to the
+//                                                                         V operand of two (four) matrix instructions
+//   scales   [page][kv head][block 4] for K and for V                     fp32 powers of two: a block is KV_BLOCK = 16 tokens of one head
+// value = code * scale, codes in [-127, 127].  Powers of two make every step exact but the one rounding to a code: the division, the
+// value read back, and the products of codes on the matrix cores (an int8 is exact in binary16).  Next to a free scale max / 127 they cost
+// at most one bit of the eight (half a bit on average over a block's maximum); in return a block whose scale grows (a later token of the
+// block is larger) is re-rounded by a shift, and results do not depend on how a division rounds.
+// A block that met an infinity or a NaN has the scale NaN: every row that sees one of its tokens is NaN, no other row is.
+#pragma once
+
+namespace calm {
+
+constexpr int KV_PAGE = 64, KV_BLOCK = 16;
+
+// bits of KvPool::status, raised by the kernels and cleared by the host
+enum { KV_BAD_PAGE = 1, KV_NO_PAGE = 2, KV_BAD_BATCH = 4, KV_BAD_PARENT = 8 };
+enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
+
+typedef _Float16 kv_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 kv_f16x8 __attribute__((ext_vector_type(8)));
+typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
+typedef float kv_f32x16 __attribute__((ext_vector_type(16)));
+
+// one layer of a pool
+struct KvLayer {
+	signed char *k, *v;
+	float *ks, *vs;
+	unsigned* status;
+	int n_pages, n_kv_heads;
+};
+// the rows of a call: sequence s owns rows [cu[s], cu[s + 1]) of the packed row arrays, its last ones; lens[s] counts them in
+struct KvRows {
+	const int *cu, *lens, *table;
+	int n_seqs, max_pages, n_rows, max_rows;
+};
+
+__device__ __forceinline__ void kv_flag(unsigned* status, unsigned bit) {
+	atomicOr(status, bit);
+}
+
+// ---- types ----------------------------------------------------------------------------------------------------------------------------
+
+// the two values of a word of a 16-bit type
+template <int DT>
+__device__ __forceinline__ void kv_two(unsigned w, float& a, float& b) {
+	if constexpr (DT == KV_F16) {
+		const kv_f16x2 h = __builtin_bit_cast(kv_f16x2, w);
+		a = (float)h[0], b = (float)h[1];
+	} else {
+		a = __builtin_bit_cast(float, w << 16), b = __builtin_bit_cast(float, w & 0xffff0000u);
+	}
+}
+template <int DT>
+__device__ __forceinline__ void kv_load4(const void* base, size_t at, float (&v)[4]) {
+	if constexpr (DT == KV_F32) {
+		const kv_f32x4 w = *(const kv_f32x4*)((const float*)base + at);
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			v[i] = w[i];
+		}
+	} else {
+		const u32x2 w = *(const u32x2*)((const unsigned short*)base + at);
+#pragma unroll
+		for (int i = 0; i < 2; ++i) {
+			const unsigned two = w[i]; // (a bit_cast of the vector's element itself reads element 0)
+			kv_two<DT>(two, v[2 * i], v[2 * i + 1]);
+		}
+	}
+}
+template <int DT>
+__device__ __forceinline__ unsigned short kv_half(float x) { // to nearest even: half a step of the type
+	if constexpr (DT == KV_F16) {
+		return __builtin_bit_cast(unsigned short, (_Float16)x);
+	} else {
+		return __builtin_bit_cast(unsigned short, (__bf16)x);
+	}
+}
+template <int DT>
+__device__ __forceinline__ void kv_store4(void* base, size_t at, const float (&v)[4]) {
+	if constexpr (DT == KV_F32) {
+		*(kv_f32x4*)((float*)base + at) = (kv_f32x4){v[0], v[1], v[2], v[3]};
+	} else {
+		const u32x2 w = {kv_half<DT>(v[0]) | ((unsigned)kv_half<DT>(v[1]) << 16), kv_half<DT>(v[2]) | ((unsigned)kv_half<DT>(v[3]) << 16)};
+		*(u32x2*)((unsigned short*)base + at) = w;
+	}
+}
+
+// eight codes as binary16, exactly: a code's byte with its sign bit turned over is code + 128, under the exponent byte 0x64 it reads
+// 1024 + (code + 128); five instructions for four codes
+__device__ __forceinline__ kv_f16x8 kv_codes8(unsigned w0, unsigned w1) {
+	const kv_f16x2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
+	u32x4 r;
+	w0 ^= 0x80808080u, w1 ^= 0x80808080u;
+	r[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u);
+	r[1] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u);
+	r[2] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u);
+	r[3] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u);
+#pragma unroll
+	for (int i = 0; i < 4; ++i) {
+		const unsigned two = r[i];
+		r[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(kv_f16x2, two) + off);
+	}
+	return __builtin_bit_cast(kv_f16x8, r);
+}
+
+// 2^e for -126 <= e <= 127
+__device__ __forceinline__ float kv_exp2i(int e) {
+	return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
+}
+// least e >= -126 with a <= 127 * 2^e, from the bits of a >= 0 (finite)
+__device__ __forceinline__ int kv_scale_exp(unsigned a) {
+	const int e = (int)(a >> 23) - 127 - 6 + ((a & 0x7fffffu) > 0x7e0000u ? 1 : 0); // 127 / 64 = 1.984375 = 1 + 0x7e0000 / 2^23
+	return e < -126 ? -126 : e;
+}
+
+// ---- append ---------------------------------------------------------------------------------------------------------------------------
+
+struct KvAppendArgs {
+	KvLayer p;
+	KvRows r;
+	const void *k, *v;
+	long k_row, k_head, v_row, v_head; // strides in elements
+};
+
+// item number `target` of a list that gives sequence s count(s) items: its sequence, and which of the sequence's it is; false behind the
+// end.  64 sequences at a time: counts across the lanes, their running sum, one ballot.
+template <class F>
+__device__ __forceinline__ bool kv_find(int n_seqs, int target, F count, int& seq, int& item) {
+	const int lane = lane_id();
+	for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+		const int mine = s0 + lane < n_seqs ? count(s0 + lane) : 0;
+		int sum = mine;
+#pragma unroll
+		for (int o = 1; o < 64; o <<= 1) {
+			const int up = __shfl_up(sum, o);
+			sum += lane >= o ? up : 0;
+		}
+		const unsigned long long b = __ballot(sum > target);
+		if (b) {
+			const int l = __builtin_ctzll(b);
+			seq = s0 + l;
+			item = target - __builtin_amdgcn_readlane(sum - mine, l);
+			return true;
+		}
+		target -= __builtin_amdgcn_readlane(sum, 63);
+	}
+	return false;
+}
+
+// the rows of sequence s that count: inside the packed arrays, at positions >= 0
+__device__ __forceinline__ void kv_rows_of(const KvRows& r, int s, int& row0, int& n, int& len) {
+	row0 = r.cu[s], n = r.cu[s + 1] - row0, len = r.lens[s];
+	if (row0 < 0 || n < 0 || row0 + n > r.n_rows) {
+		n = 0;
+	}
+	len = len < 0 ? 0 : len;
+}
+
+// One workgroup quantises what a call adds to one page and kv head, wave w the page's block w: rows in, the largest magnitude of the
+// block's new values, the scale, codes out.  Bytes bound it (a token's rows once in, a quarter or half of them out); a lane takes four
+// tokens x four dims, so K goes out as a dword per token and V as a dword per dim without crossing lanes.
+// grid = (pages touched at most, kv heads)
+template <int D, int DT>
+__global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
+	constexpr int NI = (D + 63) / 64; // items (quad of tokens, four dims) per lane: 4 x D / 4 over 64 lanes
+	const int lane = lane_id(), blk = wave_id(), h = blockIdx.y;
+	int s, at;
+	const KvRows& r = a.r;
+	const auto pages = [&](int i) {
+		int row0, n, len;
+		kv_rows_of(r, i, row0, n, len);
+		n = n < len ? n : len;
+		return n > 0 ? (len - 1) / KV_PAGE - (len - n) / KV_PAGE + 1 : 0;
+	};
+	if (!kv_find(r.n_seqs, (int)blockIdx.x, pages, s, at)) {
+		return;
+	}
+	int row0, n, len;
+	kv_rows_of(r, s, row0, n, len);
+	if (n > len) { // rows before position 0
+		row0 += n - len, n = len;
+	}
+	const int before = len - n;
+	const int pg = before / KV_PAGE + at;
+	const int pid = pg < r.max_pages ? r.table[(size_t)s * r.max_pages + pg] : -1;
+	if (pid < 0 || pid >= a.p.n_pages) {
+		if (threadIdx.x == 0 && h == 0) {
+			kv_flag(a.p.status, KV_BAD_PAGE);
+		}
+		return;
+	}
+	const int b0 = pg * KV_PAGE + blk * KV_BLOCK; // first position of the block
+	const int lo = before > b0 ? before - b0 : 0, hi = len - b0 < KV_BLOCK ? len - b0 : KV_BLOCK; // its new tokens
+	if (lo >= hi) {
+		return;
+	}
+	const size_t page = (size_t)pid * a.p.n_kv_heads + h;
+	signed char* const kp = a.p.k + page * (KV_PAGE * D) + blk * KV_BLOCK * D;
+	unsigned* const vp = (unsigned*)(a.p.v + page * (KV_PAGE * D)) + blk; // + (quad * D + dim) * 4
+#pragma unroll
+	for (int kv = 0; kv < 2; ++kv) {
+		const void* const src = kv ? a.v : a.k;
+		const size_t src0 = (size_t)(row0 + b0 + lo - before) * (size_t)(kv ? a.v_row : a.k_row) + (size_t)h * (size_t)(kv ? a.v_head : a.k_head);
+		float x[NI][4][4]; // [item][token][dim]
+		unsigned top = 0;
+#pragma unroll
+		for (int i = 0; i < NI; ++i) {
+			const int it = lane + 64 * i, g = it / (D / 4), d = it % (D / 4) * 4;
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				x[i][t][0] = x[i][t][1] = x[i][t][2] = x[i][t][3] = 0.f;
+				if (it < D && 4 * g + t >= lo && 4 * g + t < hi) {
+					kv_load4<DT>(src, src0 + (size_t)(4 * g + t - lo) * (size_t)(kv ? a.v_row : a.k_row) + d, x[i][t]);
+				}
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					const unsigned m = __builtin_bit_cast(unsigned, x[i][t][e]) & 0x7fffffffu;
+					top = top > m ? top : m;
+				}
+			}
+		}
+#pragma unroll
+		for (int o = 32; o > 0; o >>= 1) {
+			const unsigned m = __shfl_xor(top, o);
+			top = top > m ? top : m;
+		}
+		float* const sp = (kv ? a.p.vs : a.p.ks) + page * 4 + blk;
+		const unsigned was = lo > 0 ? __builtin_bit_cast(unsigned, *sp) & 0x7fffffffu : 0;
+		const bool poison = top >= 0x7f800000u || was >= 0x7f800000u;
+		int e = top >= 0x7f800000u ? -126 : kv_scale_exp(top);
+		const int e_was = was >= 0x00800000u && was < 0x7f800000u ? (int)(was >> 23) - 127 : -126;
+		e = e > e_was ? e : e_was; // (no old tokens: e_was is the least there is)
+		// 2^-e; e <= 122
+		const float inv = kv_exp2i(-e);
+		const bool shift = lo > 0 && e > e_was;
+		const float shrink = shift ? kv_exp2i(e_was - e < -126 ? -126 : e_was - e) : 1.f;
+#pragma unroll
+		for (int i = 0; i < NI; ++i) {
+			const int it = lane + 64 * i, g = it / (D / 4), d = it % (D / 4) * 4;
+			if (it >= D || 4 * g >= hi || (4 * g + 3 < lo && !shift)) {
+				continue; // nothing of this quad changes
+			}
+			unsigned out[4]; // K: a token's four dims; V: a dim's four tokens
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				out[j] = 0;
+				if (kv ? 4 * g < lo : 4 * g + j < lo) { // old tokens among them
+					out[j] = kv ? vp[(size_t)(g * D + d + j) * 4] : *(const unsigned*)(kp + (4 * g + j) * D + d);
+				}
+			}
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				const bool fresh = 4 * g + t >= lo;
+#pragma unroll
+				for (int c = 0; c < 4; ++c) {
+					unsigned& w = out[kv ? c : t];
+					const int sh = 8 * (kv ? t : c);
+					if (fresh) {
+						const float y = poison ? 0.f : x[i][t][c] * inv; // exact but where it underflows, to zero
+						w = (w & ~(0xffu << sh)) | (((unsigned)(int)__builtin_rintf(y) & 0xffu) << sh);
+					} else if (shift) {
+						const int old = (int)(signed char)(w >> sh);
+						w = (w & ~(0xffu << sh)) | (((unsigned)(int)__builtin_rintf((float)old * shrink) & 0xffu) << sh);
+					}
+				}
+			}
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				if (kv) {
+					vp[(size_t)(g * D + d + j) * 4] = out[j];
+				} else if (4 * g + j < hi && (4 * g + j >= lo || shift)) {
+					*(unsigned*)(kp + (4 * g + j) * D + d) = out[j];
+				}
+			}
+		}
+		if (lane == 0) {
+			*(unsigned*)sp = poison ? 0x7fc00000u : __builtin_bit_cast(unsigned, kv_exp2i(e));
+		}
+	}
+}
+
+// ---- read back ------------------------------------------------------------------------------------------------------------------------
+
+struct KvReadArgs {
+	KvLayer p;
+	const int *table, *lens, *start;
+	void *k, *v; // [seq][count][kv head][D]
+	int n_seqs, max_pages, count;
+};
+
+// values of positions start[s] .. start[s] + count - 1 of every sequence, zeros outside [0, lens[s]); a wave per (sequence, cache block, kv head)
+// grid = (blocks, kv heads, seqs)
+template <int D, int DT>
+__global__ __launch_bounds__(64) void k_kv_read(KvReadArgs a) {
+	const int lane = lane_id(), h = blockIdx.y, s = blockIdx.z, H = a.p.n_kv_heads;
+	const int start = a.start[s];
+	int len = a.lens[s];
+	len = len < 0 ? 0 : len;
+	const long b0 = ((long)(start >> 4) + blockIdx.x) * KV_BLOCK; // first position of the block (floor: start may be negative)
+	const long first = b0 > start ? b0 : start, last = b0 + KV_BLOCK < (long)start + a.count ? b0 + KV_BLOCK : (long)start + a.count;
+	if (first >= last) {
+		return;
+	}
+	int pid = -1;
+	if (b0 >= 0 && b0 < len) {
+		pid = b0 / KV_PAGE < a.max_pages ? a.table[(size_t)s * a.max_pages + b0 / KV_PAGE] : -1;
+		if (pid < 0 || pid >= a.p.n_pages) {
+			if (lane == 0 && h == 0) {
+				kv_flag(a.p.status, KV_BAD_PAGE);
+			}
+			pid = -2;
+		}
+	}
+	const int blk = (int)((b0 >> 4) & 3);
+	const size_t page = (size_t)(pid < 0 ? 0 : pid) * H + h;
+	const float nan = __builtin_nanf("");
+	const float ks = pid >= 0 ? a.p.ks[page * 4 + blk] : nan, vs = pid >= 0 ? a.p.vs[page * 4 + blk] : nan;
+#pragma unroll
+	for (int kv = 0; kv < 2; ++kv) {
+		for (int it = lane; it < D; it += 64) {
+			const int g = it / (D / 4), d = it % (D / 4) * 4;
+			unsigned w[4];
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				w[j] = 0;
+				if (pid >= 0) {
+					w[j] = kv ? ((const unsigned*)(a.p.v + page * (KV_PAGE * D)))[(size_t)(g * D + d + j) * 4 + blk]
+					          : *(const unsigned*)(a.p.k + page * (KV_PAGE * D) + (blk * KV_BLOCK + 4 * g + j) * D + d);
+				}
+			}
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				const long pos = b0 + 4 * g + t;
+				if (pos < first || pos >= last) {
+					continue;
+				}
+				float y[4];
+#pragma unroll
+				for (int c = 0; c < 4; ++c) {
+					const int code = (int)(signed char)(w[kv ? c : t] >> (8 * (kv ? t : c)));
+					y[c] = pos >= 0 && pos < len ? (float)code * (kv ? vs : ks) : 0.f;
+				}
+				kv_store4<DT>(kv ? a.v : a.k, (((size_t)s * a.count + (size_t)(pos - start)) * H + h) * D + d, y);
+			}
+		}
+	}
+}
+
+// ---- attention ------------------------------------------------------------------------------------------------------------------------
+//
+// Row (t, head) of sequence s stands at position p = lens[s] - n + t and sees tokens j <= p with no window, or j > p - window, or
+// j < sinks.  out = sum_j P_j V_j / sum_j P_j with P_j = 2^(x_j - m), x_j = (q . K_j) scale log2(e), m the running maximum.
+// Both products run on the matrix cores, transposed: S^T = K q^T puts a query row into a lane's column, so maximum, sum and rescaling
+// of a row are its lane's own (plus the other lanes of the same column), and the weights are already the operand layout that
+// O^T = V^T P^T wants.  Numerics: codes are exact binary16; q is one binary16 after its row is scaled by a power of two to at most 1
+// (fp16 and bf16 rows lose nothing above 2^-14 of their largest element), fp32 rows as the sum of two (22 bits); scores are fp32, times
+// the block's K scale; P_j times the block's V scale over the largest one met (E) is one binary16 for fp16 / bf16 outputs -- 2^-12 relative,
+// a third or less of the output's own rounding, since weights average -- and the sum of two for fp32; sums in fp32.  A weight below
+// 2^-14 of the largest (V scale included) keeps an absolute 2^-25 of it.
+
+struct KvAttnArgs {
+	KvLayer p;
+	KvRows r;
+	const void* q;
+	void* out; // [row][head][D]
+	long q_row, q_head;
+	float* part; // [row x head][split][D + 2]: partial sums, then the maximum and the sum of weights
+	int n_heads, group, window, sinks, chunk, n_splits;
+	float scale; // scale * log2(e)
+};
+
+// the pages that rows at positions p_min .. p_max see: [0, first tokens' pages) and [start, p_max / 64]
+struct KvSpan {
+	int ns, start, np;
+	__device__ __forceinline__ KvSpan(int p_min, int p_max, int window, int sinks) {
+		const int lo = window > 0 && p_min >= window ? p_min - window + 1 : 0;
+		const int s = sinks < lo ? sinks : lo;
+		ns = (s + KV_PAGE - 1) / KV_PAGE;
+		start = lo / KV_PAGE;
+		start = start < ns ? ns : start;
+		np = p_max < 0 ? 0 : ns + (p_max / KV_PAGE >= start ? p_max / KV_PAGE - start + 1 : 0);
+	}
+	__device__ __forceinline__ int page(int i) const {
+		return i < ns ? i : start + i - ns;
+	}
+};
+
+template <int DT, int N>
+__device__ __forceinline__ float kv_row_top(const float (&x)[N]) {
+	float m = 0.f;
+#pragma unroll
+	for (int i = 0; i < N; ++i) {
+		m = fmaxf(m, fabsf(x[i]));
+	}
+	return m;
+}
+__device__ __forceinline__ float kv_xor_max(float v, int o) {
+	return fmaxf(v, __shfl_xor(v, o));
+}
+__device__ __forceinline__ float kv_exp2(float x) {
+	return __builtin_amdgcn_exp2f(x); // one unit in the last place; below 2^-126 zero
+}
+// the power of two that brings a row with largest magnitude `top` to at most 1 (a row of zeros, or one with an infinity: 1 / a NaN product)
+__device__ __forceinline__ int kv_row_exp(float top) {
+	const unsigned b = __builtin_bit_cast(unsigned, top);
+	int e = (int)(b >> 23) - 126;
+	e = e < -126 ? -126 : e;
+	return e > 126 ? 126 : e;
+}
+
+// the result of a row, or its part of a split: `o` (a quad of dims) times f
+template <int D, int DT>
+__device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t row, int split, int d, const float (&o)[4]) {
+	if (direct) {
+		kv_store4<DT>(a.out, row * D + d, o);
+	} else {
+		float* const p = a.part + (row * a.n_splits + split) * (D + 4) + d;
+		*(kv_f32x4*)p = (kv_f32x4){o[0], o[1], o[2], o[3]};
+	}
+}
+
+// Few rows (one token of a sequence, or a few): the cache's bytes bound it.  A workgroup takes one sequence, one kv head, 16 x NR rows
+// (token x head of the group) and a range of pages, dealt to its four waves a page at a time; a wave holds a page's codes in registers as
+// the matrix operands they are, loads the next page's K behind the first product and its V behind the second, so 8 - 16 KiB per wave
+// are in flight throughout.  The waves' sums meet in LDS; ranges of one row meet in k_kv_merge.
+// grid = (splits, kv heads x tiles, seqs)
+template <int D, int DT, int NR>
+__global__ __launch_bounds__(256) void k_kv_decode(KvAttnArgs a) {
+	constexpr int KS = D / 32;  // k-steps of S^T
+	constexpr int ND = D / 16;  // dim tiles of O^T
+	constexpr int KW = D / 16;  // dwords of a K row per lane
+	constexpr bool HL = DT == KV_F32;
+	extern __shared__ float kv_lds[]; // [wave][NR x 16 rows][D + 4]
+	const int lane = lane_id(), wave = wave_id();
+	const int col = lane & 15, g = lane >> 4;
+	const int H = a.p.n_kv_heads, h = blockIdx.y % H, tile = blockIdx.y / H, s = blockIdx.z, split = blockIdx.x;
+	int row0, n, len;
+	kv_rows_of(a.r, s, row0, n, len);
+	const int nrows = n * a.group, r0 = tile * 16 * NR;
+	if (threadIdx.x == 0 && tile == 0 && h == 0 && split == 0 && n > a.r.max_rows) {
+		kv_flag(a.p.status, KV_BAD_BATCH);
+	}
+	if (r0 >= nrows) {
+		return;
+	}
+	const int rl = r0 + 16 * NR - 1 < nrows - 1 ? r0 + 16 * NR - 1 : nrows - 1;
+	const int p_min = len - n + r0 / a.group, p_max = len - n + rl / a.group;
+	const KvSpan sp(p_min, p_max, a.window, a.sinks);
+	const bool direct = sp.np <= a.chunk;
+	const int i0 = split * a.chunk, i1 = (split + 1) * a.chunk < sp.np ? (split + 1) * a.chunk : sp.np;
+	int pos[NR];
+	size_t row[NR];
+	bool live[NR];
+#pragma unroll
+	for (int c = 0; c < NR; ++c) {
+		const int rr = r0 + 16 * c + col;
+		live[c] = rr < nrows;
+		const int t = (live[c] ? rr : r0) / a.group, hd = h * a.group + (live[c] ? rr : r0) % a.group;
+		pos[c] = len - n + t;
+		row[c] = (size_t)(row0 + t) * a.n_heads + hd;
+	}
+	if (i0 >= i1 && split > 0) {
+		if (!direct && wave == 0 && g == 0) { // a range without pages: marked empty for k_kv_merge
+#pragma unroll
+			for (int c = 0; c < NR; ++c) {
+				if (live[c]) {
+					float* const p = a.part + (row[c] * a.n_splits + split) * (D + 4) + D;
+					p[0] = -__builtin_inff(), p[1] = 0.f;
+				}
+			}
+		}
+		return;
+	}
+	// q: lane (col, g) holds dims g D / 4 .. of its row, k-step i the eight at i 8 -- K's lanes take the same dims
+	kv_f16x8 qh[NR][KS], ql[NR][HL ? KS : 1];
+	float qf[NR];
+#pragma unroll
+	for (int c = 0; c < NR; ++c) {
+		float x[D / 4];
+		const size_t at = (row[c] / a.n_heads) * (size_t)a.q_row + (row[c] % a.n_heads) * (size_t)a.q_head + g * (D / 4);
+#pragma unroll
+		for (int i = 0; i < D / 16; ++i) {
+			float y[4];
+			kv_load4<DT>(a.q, at + 4 * i, y);
+			x[4 * i] = y[0], x[4 * i + 1] = y[1], x[4 * i + 2] = y[2], x[4 * i + 3] = y[3];
+		}
+		float top = kv_row_top<DT>(x);
+		top = kv_xor_max(kv_xor_max(top, 16), 32);
+		const int e = kv_row_exp(top);
+		const float inv = kv_exp2i(-e);
+		qf[c] = kv_exp2i(e) * a.scale;
+#pragma unroll
+		for (int i = 0; i < KS; ++i) {
+#pragma unroll
+			for (int j = 0; j < 8; ++j) {
+				const float y = x[8 * i + j] * inv;
+				qh[c][i][j] = (_Float16)y;
+				if constexpr (HL) {
+					ql[c][i][j] = (_Float16)(y - (float)qh[c][i][j]);
+				}
+			}
+		}
+	}
+	float m[NR], l[NR];
+	kv_f32x4 o[NR][ND];
+#pragma unroll
+	for (int c = 0; c < NR; ++c) {
+		m[c] = -__builtin_inff(), l[c] = 0.f;
+#pragma unroll
+		for (int d = 0; d < ND; ++d) {
+			o[c][d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
+		}
+	}
+	float E = 1.1754944e-38f; // the largest V scale met
+	// page ids of this wave's next 64 pages, one per lane
+	int ids = -1, ids0 = i0 + wave; // lane i: page ids0 + 4 i
+	const auto fetch_ids = [&](int first) {
+		ids0 = first;
+		const int i = first + 4 * lane;
+		ids = -1;
+		if (i < i1) {
+			const int pg = sp.page(i);
+			ids = pg < a.r.max_pages ? a.r.table[(size_t)s * a.r.max_pages + pg] : -1;
+			if (ids < 0 || ids >= a.p.n_pages) {
+				kv_flag(a.p.status, KV_BAD_PAGE);
+				ids = -1;
+			}
+		}
+	};
+	unsigned kr[4][KW];
+	u32x4 vr[ND];
+	kv_f32x4 ksc, vsc;
+	const auto load_k = [&](int pid) {
+		const size_t page = (size_t)(pid < 0 ? 0 : pid) * H + h;
+		const signed char* const p = a.p.k + page * (KV_PAGE * D) + (size_t)col * D + g * (D / 4);
+#pragma unroll
+		for (int t = 0; t < 4; ++t) {
+			if constexpr (D % 64 == 0) {
+#pragma unroll
+				for (int i = 0; i < KW / 4; ++i) {
+					const u32x4 w = *(const u32x4*)(p + t * 16 * D + 16 * i);
+					kr[t][4 * i] = w[0], kr[t][4 * i + 1] = w[1], kr[t][4 * i + 2] = w[2], kr[t][4 * i + 3] = w[3];
+				}
+			} else {
+#pragma unroll
+				for (int i = 0; i < KW / 2; ++i) {
+					const u32x2 w = *(const u32x2*)(p + t * 16 * D + 8 * i);
+					kr[t][2 * i] = w[0], kr[t][2 * i + 1] = w[1];
+				}
+			}
+		}
+		ksc = *(const kv_f32x4*)(a.p.ks + page * 4);
+	};
+	const auto load_v = [&](int pid) {
+		const size_t page = (size_t)(pid < 0 ? 0 : pid) * H + h;
+		const u32x4* const p = (const u32x4*)(a.p.v + page * (KV_PAGE * D)) + g * D + col;
+#pragma unroll
+		for (int d = 0; d < ND; ++d) {
+			vr[d] = p[16 * d];
+		}
+		vsc = *(const kv_f32x4*)(a.p.vs + page * 4);
+	};
+	int pid = -1;
+	if (i0 + wave < i1) {
+		fetch_ids(i0 + wave);
+		pid = __builtin_amdgcn_readlane(ids, 0);
+		load_k(pid);
+		load_v(pid);
+	}
+	for (int i = i0 + wave; i < i1; i += 4) {
+		const int pg = sp.page(i), j0 = pg * KV_PAGE;
+		const bool bad = pid < 0;
+		const bool more = i + 4 < i1;
+		if (more && i + 4 >= ids0 + 256) {
+			fetch_ids(i + 4);
+		}
+		const int next = more ? __builtin_amdgcn_readlane(ids, (i + 4 - ids0) >> 2) : -1;
+		// S^T of the page: tile t = block t, this lane's tokens 4 g + e
+		kv_f32x4 sc[NR][4];
+#pragma unroll
+		for (int t = 0; t < 4; ++t) {
+#pragma unroll
+			for (int c = 0; c < NR; ++c) {
+				sc[c][t] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
+			}
+#pragma unroll
+			for (int k = 0; k < KS; ++k) {
+				const kv_f16x8 kf = kv_codes8(kr[t][2 * k], kr[t][2 * k + 1]);
+#pragma unroll
+				for (int c = 0; c < NR; ++c) {
+					sc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[c][k], sc[c][t], 0, 0, 0);
+					if constexpr (HL) {
+						sc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[c][k], sc[c][t], 0, 0, 0);
+					}
+				}
+			}
+		}
+		const kv_f32x4 kscale = bad ? (kv_f32x4){__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")} : ksc;
+		if (more) {
+			load_k(next);
+		}
+		// every token of the page seen by every row of the tile?
+		const bool whole = j0 + KV_PAGE - 1 <= p_min && (a.window <= 0 || j0 > p_max - a.window || j0 + KV_PAGE <= a.sinks);
+		float Enew = E;
+#pragma unroll
+		for (int t = 0; t < 4; ++t) {
+			const int jb = j0 + 16 * t;
+			const bool seen = jb <= p_max && (a.window <= 0 || jb + 15 > p_min - a.window || jb < a.sinks);
+			Enew = fmaxf(Enew, seen ? fabsf(vsc[t]) : 0.f);
+		}
+		const float grow = E * __builtin_amdgcn_rcpf(Enew), rE = __builtin_amdgcn_rcpf(Enew);
+		E = Enew;
+		kv_f16x8 pf[NR][2], pl[NR][HL ? 2 : 1];
+#pragma unroll
+		for (int c = 0; c < NR; ++c) {
+			float top = m[c];
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				const float f = kscale[t] * qf[c];
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					float x = sc[c][t][e] * f;
+					if (!whole) {
+						const int j = j0 + 16 * t + 4 * g + e;
+						const bool seen = j <= pos[c] && (a.window <= 0 || j > pos[c] - a.window || j < a.sinks);
+						x = seen ? x : -__builtin_inff();
+					}
+					sc[c][t][e] = x;
+					top = fmaxf(top, x);
+				}
+			}
+			top = kv_xor_max(kv_xor_max(top, 16), 32);
+			const float ref = top == -__builtin_inff() ? 0.f : top;
+			const float alpha = kv_exp2(m[c] - ref); // (m = -inf: 0)
+			m[c] = top;
+			l[c] *= alpha;
+			const float og = alpha * grow;
+			if (__ballot(og != 1.f)) {
+#pragma unroll
+				for (int d = 0; d < ND; ++d) {
+					o[c][d] *= og;
+				}
+			}
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				const float f = vsc[t] * rE;
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					const float w = kv_exp2(sc[c][t][e] - ref);
+					l[c] += w;
+					float y = w * f;
+					if (!whole) { // (a NaN scale must not reach a row that does not see the token)
+						y = sc[c][t][e] == -__builtin_inff() ? 0.f : y;
+					}
+					pf[c][t >> 1][4 * (t & 1) + e] = (_Float16)y;
+					if constexpr (HL) {
+						pl[c][t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[c][t >> 1][4 * (t & 1) + e]);
+					}
+				}
+			}
+		}
+#pragma unroll
+		for (int d = 0; d < ND; ++d) {
+#pragma unroll
+			for (int u = 0; u < 2; ++u) {
+				const kv_f16x8 vf = kv_codes8(vr[d][2 * u], vr[d][2 * u + 1]);
+#pragma unroll
+				for (int c = 0; c < NR; ++c) {
+					o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[c][u], o[c][d], 0, 0, 0);
+					if constexpr (HL) {
+						o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[c][u], o[c][d], 0, 0, 0);
+					}
+				}
+			}
+		}
+		if (more) {
+			load_v(next);
+		}
+		pid = next;
+	}
+	// the four waves' sums
+	float* const mine = kv_lds + wave * (16 * NR * (D + 4));
+#pragma unroll
+	for (int c = 0; c < NR; ++c) {
+		l[c] += __shfl_xor(l[c], 16);
+		l[c] += __shfl_xor(l[c], 32);
+		float* const p = mine + (16 * c + col) * (D + 4);
+#pragma unroll
+		for (int d = 0; d < ND; ++d) {
+			*(kv_f32x4*)(p + 16 * d + 4 * g) = o[c][d];
+		}
+		if (g == 0) {
+			p[D] = m[c], p[D + 1] = l[c], p[D + 2] = E;
+		}
+	}
+	__syncthreads();
+	// a thread per (row, quad of dims)
+	for (int it = threadIdx.x; it < 16 * NR * (D / 4); it += 256) {
+		const int rr = it / (D / 4), d = it % (D / 4) * 4;
+		if (r0 + rr >= nrows) {
+			break;
+		}
+		const float* const p = kv_lds + rr * (D + 4);
+		constexpr int W = 16 * NR * (D + 4);
+		float M = fmaxf(fmaxf(p[D], p[W + D]), fmaxf(p[2 * W + D], p[3 * W + D]));
+		const float EM = fmaxf(fmaxf(p[D + 2], p[W + D + 2]), fmaxf(p[2 * W + D + 2], p[3 * W + D + 2]));
+		const float ref = M == -__builtin_inff() ? 0.f : M;
+		float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+		for (int w = 0; w < 4; ++w) {
+			const float f = kv_exp2(p[w * W + D] - ref), fe = f * (p[w * W + D + 2] / EM);
+			L += f * p[w * W + D + 1];
+			const kv_f32x4 x = *(const kv_f32x4*)(p + w * W + d);
+#pragma unroll
+			for (int e = 0; e < 4; ++e) {
+				y[e] += fe * x[e];
+			}
+		}
+		const int t = (r0 + rr) / a.group;
+		const size_t at = (size_t)(row0 + t) * a.n_heads + h * a.group + (r0 + rr) % a.group;
+		const float f = direct ? (L == 0.f ? 0.f : EM / L) : EM; // (no token seen: zeros)
+#pragma unroll
+		for (int e = 0; e < 4; ++e) {
+			y[e] *= f;
+		}
+		kv_put<D, DT>(a, direct, at, split, d, y);
+		if (d == 0 && a.n_splits > 1) {
+			float* const pm = a.part + (at * a.n_splits + split) * (D + 4) + D;
+			pm[0] = direct ? __builtin_inff() : M, pm[1] = L; // +inf: the row is written already
+		}
+	}
+}
+
+// the ranges of a row put together; a wave per row, the ranges' maxima across its lanes (n_splits <= 64)
+template <int D, int DT>
+__global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
+	const int lane = lane_id();
+	const size_t row = (size_t)blockIdx.x * 4 + wave_id();
+	const int last = a.r.cu[a.r.n_seqs] < a.r.n_rows ? a.r.cu[a.r.n_seqs] : a.r.n_rows;
+	if (row >= (size_t)(last < 0 ? 0 : last) * a.n_heads) {
+		return; // rows behind the last sequence stay as they are
+	}
+	const float* const p = a.part + row * a.n_splits * (D + 4);
+	float m = -__builtin_inff(), l = 0.f;
+	if (lane < a.n_splits) {
+		m = p[(size_t)lane * (D + 4) + D], l = p[(size_t)lane * (D + 4) + D + 1];
+	}
+	if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, m), 0) == 0x7f800000) {
+		return; // one range: written by its workgroup
+	}
+	const bool empty = m == -__builtin_inff() && l == 0.f;
+	const float M = wave_max_dpp(m);
+	const float w = kv_exp2(m - (M == -__builtin_inff() ? 0.f : M));
+	const float L = wave_sum(empty ? 0.f : w * l);
+	const unsigned long long some = __ballot(!empty);
+	constexpr int N = (D + 255) / 256;
+	const int d = lane * 4;
+	float y[4] = {0.f, 0.f, 0.f, 0.f};
+	static_assert(N == 1, "a quad of dims per lane");
+	for (int i = 0; i < a.n_splits; ++i) {
+		if ((some >> i) & 1) {
+			const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
+			if (d < D) {
+				const kv_f32x4 x = *(const kv_f32x4*)(p + (size_t)i * (D + 4) + d);
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					y[e] += f * x[e];
+				}
+			}
+		}
+	}
+	if (d < D) {
+		const float f = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+		for (int e = 0; e < 4; ++e) {
+			y[e] *= f;
+		}
+		kv_store4<DT>(a.out, row * D + d, y);
+	}
+}
+
+// Many rows (a prompt chunk): the matrix cores bound it.  A workgroup takes 128 rows (32 per wave) of one sequence and kv head and walks
+// the pages they see; a page's codes become binary16 ONCE per workgroup on their way into LDS (two buffers: the next page's loads are in
+// flight while a page is computed), laid out so that every operand is one 16-byte read of consecutive lanes.
+// grid = (row tiles, kv heads, seqs x splits)
+template <int D>
+struct KvChunk {
+	static constexpr int KROW = 65;                // 16-byte units between two (k-step, half) columns of K: 64 tokens and one of padding
+	static constexpr int KU = D / 8 * KROW, VU = 8 * D; // units of a page's K and V
+	static constexpr size_t LDS = (size_t)2 * (KU + VU) * 16;
+};
+
+template <int D, int DT>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a) {
+	constexpr int KS = D / 16, ND = D / 32;
+	constexpr bool HL = DT == KV_F32;
+	constexpr int NK = (4 * D + 255) / 256, NV = (2 * D + 255) / 256; // staging items per thread
+	constexpr int KROW = KvChunk<D>::KROW, KU = KvChunk<D>::KU, VU = KvChunk<D>::VU;
+	extern __shared__ u32x4 kv_st[];
+	const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
+	const int col = lane & 31, hh = lane >> 5;
+	const int H = a.p.n_kv_heads, h = blockIdx.y, s = blockIdx.z / a.n_splits, split = blockIdx.z % a.n_splits;
+	int row0, n, len;
+	kv_rows_of(a.r, s, row0, n, len);
+	const int nrows = n * a.group, r0 = blockIdx.x * 128;
+	if (tid == 0 && r0 == 0 && h == 0 && split == 0 && n > a.r.max_rows) {
+		kv_flag(a.p.status, KV_BAD_BATCH);
+	}
+	if (r0 >= nrows) {
+		return;
+	}
+	const int rl = r0 + 127 < nrows - 1 ? r0 + 127 : nrows - 1;
+	const int p_min = len - n + r0 / a.group, p_max = len - n + rl / a.group;
+	const KvSpan sp(p_min, p_max, a.window, a.sinks);
+	const bool direct = sp.np <= a.chunk;
+	const int i0 = split * a.chunk, i1 = (split + 1) * a.chunk < sp.np ? (split + 1) * a.chunk : sp.np;
+	// this wave's rows
+	const int rr = r0 + 32 * wave + col;
+	const bool live = rr < nrows;
+	const int t = (live ? rr : nrows - 1) / a.group, hd = h * a.group + (live ? rr : nrows - 1) % a.group;
+	const int pos = len - n + t;
+	const size_t row = (size_t)(row0 + t) * a.n_heads + hd;
+	const int wl = r0 + 32 * wave + 31 < nrows - 1 ? r0 + 32 * wave + 31 : nrows - 1;
+	const bool any = r0 + 32 * wave < nrows;
+	const int w_min = len - n + (any ? r0 + 32 * wave : 0) / a.group, w_max = any ? len - n + wl / a.group : -1;
+	if (i0 >= i1 && split > 0) {
+		if (!direct && live && hh == 0) {
+			float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
+			p[0] = -__builtin_inff(), p[1] = 0.f;
+		}
+		return;
+	}
+	kv_f16x8 qh[KS], ql[HL ? KS : 1];
+	float qf;
+	{
+		const size_t at = (size_t)(row0 + t) * (size_t)a.q_row + (size_t)hd * (size_t)a.q_head + hh * 8;
+		// (the row is read twice: its largest magnitude first -- half a row of fp32 in registers beside everything else would not fit)
+		float top = 0.f;
+#pragma unroll 4
+		for (int i = 0; i < 2 * KS; ++i) {
+			float y[4];
+			kv_load4<DT>(a.q, at + 16 * (i >> 1) + 4 * (i & 1), y);
+			top = fmaxf(top, kv_row_top<DT>(y));
+		}
+		top = kv_xor_max(top, 32);
+		const int e = kv_row_exp(top);
+		const float inv = kv_exp2i(-e);
+		qf = kv_exp2i(e) * a.scale;
+#pragma unroll
+		for (int i = 0; i < KS; ++i) {
+#pragma unroll
+			for (int j = 0; j < 2; ++j) {
+				float y[4];
+				kv_load4<DT>(a.q, at + 16 * i + 4 * j, y);
+#pragma unroll
+				for (int c = 0; c < 4; ++c) {
+					y[c] *= inv;
+					qh[i][4 * j + c] = (_Float16)y[c];
+					if constexpr (HL) {
+						ql[i][4 * j + c] = (_Float16)(y[c] - (float)qh[i][4 * j + c]);
+					}
+				}
+			}
+		}
+	}
+	float m = -__builtin_inff(), l = 0.f, E = 1.1754944e-38f;
+	kv_f32x16 o[ND];
+#pragma unroll
+	for (int d = 0; d < ND; ++d) {
+#pragma unroll
+		for (int e = 0; e < 16; ++e) {
+			o[d][e] = 0.f;
+		}
+	}
+	u32x4 kr[NK], vr[NV][2];
+	const auto id_of = [&](int i) {
+		int pid = -1;
+		const int pg = sp.page(i);
+		if (pg < a.r.max_pages) {
+			pid = a.r.table[(size_t)s * a.r.max_pages + pg];
+		}
+		if (pid < 0 || pid >= a.p.n_pages) {
+			if (tid == 0) {
+				kv_flag(a.p.status, KV_BAD_PAGE);
+			}
+			pid = -1;
+		}
+		return __builtin_amdgcn_readfirstlane(pid);
+	};
+	const auto load = [&](int pid) {
+		const size_t page = (size_t)(pid < 0 ? 0 : pid) * H + h;
+		const u32x4* const kp = (const u32x4*)(a.p.k + page * (KV_PAGE * D));
+		const u32x4* const vp = (const u32x4*)(a.p.v + page * (KV_PAGE * D));
+#pragma unroll
+		for (int i = 0; i < NK; ++i) {
+			const int it = tid + 256 * i; // 16 dims of a token: unit it of the page
+			if (4 * D % 256 == 0 || it < 4 * D) {
+				kr[i] = kp[it];
+			}
+		}
+#pragma unroll
+		for (int i = 0; i < NV; ++i) {
+			const int it = tid + 256 * i; // (half, dim): quads half and half + 2
+			if (2 * D % 256 == 0 || it < 2 * D) {
+				vr[i][0] = vp[it], vr[i][1] = vp[it + 2 * D];
+			}
+		}
+	};
+	const auto stage = [&](int buf) {
+		u32x4* const kl = kv_st + buf * (KU + VU);
+		u32x4* const vl = kl + KU;
+#pragma unroll
+		for (int i = 0; i < NK; ++i) {
+			const int it = tid + 256 * i, key = it / (D / 16), st = it % (D / 16);
+			if (4 * D % 256 == 0 || it < 4 * D) {
+				kl[(2 * st) * KROW + key] = __builtin_bit_cast(u32x4, kv_codes8(kr[i][0], kr[i][1]));
+				kl[(2 * st + 1) * KROW + key] = __builtin_bit_cast(u32x4, kv_codes8(kr[i][2], kr[i][3]));
+			}
+		}
+#pragma unroll
+		for (int i = 0; i < NV; ++i) {
+			const int it = tid + 256 * i, half = it / D, d = it % D;
+			if (2 * D % 256 == 0 || it < 2 * D) {
+#pragma unroll
+				for (int b = 0; b < 4; ++b) {
+					vl[(2 * b + half) * D + d] = __builtin_bit_cast(u32x4, kv_codes8(vr[i][0][b], vr[i][1][b]));
+				}
+			}
+		}
+	};
+	int pid = -1;
+	if (i0 < i1) {
+		pid = id_of(i0);
+		load(pid);
+		stage(0);
+	}
+	__syncthreads();
+	for (int i = i0; i < i1; ++i) {
+		const int buf = (i - i0) & 1;
+		const bool more = i + 1 < i1;
+		const bool bad = pid < 0;
+		const size_t page = (size_t)(bad ? 0 : pid) * H + h;
+		const kv_f32x4 ksc = *(const kv_f32x4*)(a.p.ks + page * 4), vsc = *(const kv_f32x4*)(a.p.vs + page * 4);
+		int next = -1;
+		if (more) {
+			next = id_of(i + 1);
+			load(next);
+		}
+		const int j0 = sp.page(i) * KV_PAGE;
+		const bool some = j0 <= w_max && (a.window <= 0 || j0 + KV_PAGE - 1 > w_min - a.window || j0 < a.sinks);
+		if (some) {
+			const u32x4* const kl = kv_st + buf * (KU + VU);
+			const u32x4* const vl = kl + KU;
+			kv_f32x16 sc[2];
+#pragma unroll
+			for (int b = 0; b < 2; ++b) {
+#pragma unroll
+				for (int e = 0; e < 16; ++e) {
+					sc[b][e] = 0.f;
+				}
+#pragma unroll
+				for (int k = 0; k < KS; ++k) {
+					const kv_f16x8 kf = __builtin_bit_cast(kv_f16x8, kl[(2 * k + hh) * KROW + 32 * b + col]);
+					sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], sc[b], 0, 0, 0);
+					if constexpr (HL) {
+						sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc[b], 0, 0, 0);
+					}
+				}
+			}
+			const bool whole = j0 + KV_PAGE - 1 <= w_min && (a.window <= 0 || j0 > w_max - a.window || j0 + KV_PAGE <= a.sinks);
+			float Enew = E;
+#pragma unroll
+			for (int b = 0; b < 4; ++b) {
+				const int jb = j0 + 16 * b;
+				const bool seen = jb <= w_max && (a.window <= 0 || jb + 15 > w_min - a.window || jb < a.sinks);
+				Enew = fmaxf(Enew, seen ? fabsf(vsc[b]) : 0.f);
+			}
+			const float rE = __builtin_amdgcn_rcpf(Enew), grow = E * rE;
+			E = Enew;
+			float top = m;
+#pragma unroll
+			for (int b = 0; b < 2; ++b) {
+#pragma unroll
+				for (int e = 0; e < 16; ++e) { // token 32 b + 8 (e / 4) + 4 hh + e % 4
+					float x = sc[b][e] * ((bad ? __builtin_nanf("") : ksc[2 * b + (e >> 3)]) * qf);
+					if (!whole) {
+						const int j = j0 + 32 * b + 8 * (e >> 2) + 4 * hh + (e & 3);
+						const bool seen = j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+						x = seen ? x : -__builtin_inff();
+					}
+					sc[b][e] = x;
+					top = fmaxf(top, x);
+				}
+			}
+			top = kv_xor_max(top, 32);
+			const float ref = top == -__builtin_inff() ? 0.f : top;
+			const float alpha = kv_exp2(m - ref);
+			m = top;
+			l *= alpha;
+			const float og = alpha * grow;
+			if (__ballot(og != 1.f)) {
+#pragma unroll
+				for (int d = 0; d < ND; ++d) {
+					o[d] *= og;
+				}
+			}
+#pragma unroll
+			for (int b = 0; b < 2; ++b) {
+#pragma unroll
+				for (int u = 0; u < 2; ++u) { // block 2 b + u
+					const float f = vsc[2 * b + u] * rE;
+					kv_f16x8 pf, pl;
+#pragma unroll
+					for (int e = 0; e < 8; ++e) {
+						const float x = sc[b][8 * u + e];
+						const float w = kv_exp2(x - ref);
+						l += w;
+						float y = w * f;
+						if (!whole) {
+							y = x == -__builtin_inff() ? 0.f : y;
+						}
+						pf[e] = (_Float16)y;
+						if constexpr (HL) {
+							pl[e] = (_Float16)(y - (float)pf[e]);
+						}
+					}
+#pragma unroll
+					for (int d = 0; d < ND; ++d) {
+						const kv_f16x8 vf = __builtin_bit_cast(kv_f16x8, vl[(2 * (2 * b + u) + hh) * D + 32 * d + col]);
+						o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[d], 0, 0, 0);
+						if constexpr (HL) {
+							o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[d], 0, 0, 0);
+						}
+					}
+				}
+			}
+		}
+		if (more) {
+			stage(buf ^ 1);
+		}
+		__syncthreads();
+		pid = next;
+	}
+	l += __shfl_xor(l, 32);
+	if (!live) {
+		return;
+	}
+	const float f = direct ? (l == 0.f ? 0.f : E / l) : E;
+#pragma unroll
+	for (int d = 0; d < ND; ++d) {
+#pragma unroll
+		for (int q = 0; q < 4; ++q) {
+			const float y[4] = {o[d][4 * q] * f, o[d][4 * q + 1] * f, o[d][4 * q + 2] * f, o[d][4 * q + 3] * f};
+			kv_put<D, DT>(a, direct, row, split, 32 * d + 8 * q + 4 * hh, y);
+		}
+	}
+	if (hh == 0 && a.n_splits > 1) {
+		float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
+		p[0] = direct ? __builtin_inff() : m, p[1] = l;
+	}
+}
+
+// ---- the pages themselves ---------------------------------------------------------------------------------------------------------------
+//
+// A table row lists a sequence's pages (-1: none), refs[p] counts the rows that list page p; a page with a count of 0 is free, and the
+// lowest free pages are taken first.  Full pages may be shared; a page that is not full, and pages behind it, belong to one row.
+// The bookkeeping is a few thousand integers: ONE workgroup does it (a grid-wide hand-off costs more than it spreads), with integer
+// atomics only, so results do not depend on their order; the page bytes move in a launch of their own.
+
+constexpr int KV_BOOK = 1024;     // threads of the bookkeeping workgroup
+constexpr int KV_MAX_ROWS = 4096; // rows of a table the bookkeeping holds in LDS
+
+// exclusive sum of one int per thread over the workgroup, and the total; `sm`: 17 ints
+__device__ __forceinline__ int kv_block_scan(int v, int* sm, int& total) {
+	const int lane = lane_id(), wave = threadIdx.x >> 6;
+	int sum = v;
+#pragma unroll
+	for (int o = 1; o < 64; o <<= 1) {
+		const int up = __shfl_up(sum, o);
+		sum += lane >= o ? up : 0;
+	}
+	__syncthreads(); // (sm of the call before has been read)
+	if (lane == 63) {
+		sm[wave] = sum;
+	}
+	__syncthreads();
+	int before = 0, all = 0;
+#pragma unroll
+	for (int w = 0; w < KV_BOOK / 64; ++w) {
+		const int x = sm[w];
+		before += w < wave ? x : 0;
+		all += x;
+	}
+	total = all;
+	return before + sum - v;
+}
+
+// list[k] <- the k-th free page (refs == 0) in ascending order, k < want; returns how many there are (at most want).  refs written by this
+// workgroup before: barrier and fence are the caller's.
+__device__ __forceinline__ int kv_free_pages(const int* refs, int n_pages, int want, int* list, int* sm) {
+	int have = 0;
+	for (int p0 = 0; p0 < n_pages && have < want; p0 += KV_BOOK * 8) {
+		unsigned mask = 0;
+		const int mine = p0 + (int)threadIdx.x * 8;
+#pragma unroll
+		for (int j = 0; j < 8; ++j) {
+			if (mine + j < n_pages && __hip_atomic_load(refs + mine + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) {
+				mask |= 1u << j;
+			}
+		}
+		int total;
+		int at = have + kv_block_scan(__builtin_popcount(mask), sm, total);
+		while (mask) {
+			const int j = __builtin_ctz(mask);
+			mask &= mask - 1;
+			if (at < want) {
+				list[at] = mine + j;
+			}
+			++at;
+		}
+		have += total;
+	}
+	__syncthreads();
+	return have < want ? have : want;
+}
+
+struct KvForkArgs {
+	const int *table, *lens, *refs, *parents;
+	int *table_out, *refs_out, *copy; // copy: [rows] x {from, to}, to = -1: none
+	unsigned* status;
+	int n_rows, max_pages, n_pages;
+};
+
+__global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
+	__shared__ int first[KV_MAX_ROWS], count[KV_MAX_ROWS], list[KV_MAX_ROWS], sm[KV_BOOK / 64];
+	const int tid = threadIdx.x, n = a.n_rows, mp = a.max_pages;
+	for (int i = tid; i < n; i += KV_BOOK) {
+		first[i] = n, count[i] = 0;
+	}
+	for (int p = tid; p < a.n_pages; p += KV_BOOK) {
+		a.refs_out[p] = a.refs[p];
+	}
+	__syncthreads();
+	for (int i = tid; i < n; i += KV_BOOK) {
+		const int par = a.parents[i];
+		if (par >= 0 && par < n) {
+			atomicMin(&first[par], i);
+			atomicAdd(&count[par], 1);
+		} else {
+			kv_flag(a.status, KV_BAD_PARENT);
+		}
+	}
+	__threadfence();
+	__syncthreads();
+	// counts: a full page of row r is listed by count[r] rows from now on, a page of its own by one of them at most
+	for (int k = tid; k < n * mp; k += KV_BOOK) {
+		const int r = k / mp, c = k - r * mp;
+		const int kids = count[r], full = a.lens[r] / KV_PAGE;
+		const int d = (c < full ? kids : (kids > 0 ? 1 : 0)) - 1;
+		const int p = d ? a.table[k] : -1;
+		if (d && p >= 0) {
+			if (p < a.n_pages) {
+				atomicAdd(&a.refs_out[p], d);
+			} else {
+				kv_flag(a.status, KV_BAD_PAGE);
+			}
+		}
+	}
+	__threadfence();
+	__syncthreads();
+	// rows that need a page of their own: not the first child, the parent's last page not full
+	int want = 0;
+	for (int i0 = 0; i0 < n; i0 += KV_BOOK) {
+		const int i = i0 + tid;
+		int need = 0;
+		if (i < n) {
+			const int par = a.parents[i];
+			if (par >= 0 && par < n && first[par] != i) {
+				const int len = a.lens[par], c = len / KV_PAGE;
+				const int p = len > 0 && len % KV_PAGE && c < mp ? a.table[par * mp + c] : -1;
+				need = p >= 0 && p < a.n_pages;
+			}
+		}
+		int total;
+		const int at = want + kv_block_scan(need, sm, total);
+		if (i < n) {
+			a.copy[2 * i] = need ? at : -1; // (its number, until the pages are known)
+		}
+		want += total;
+	}
+	const int have = kv_free_pages(a.refs_out, a.n_pages, want, list, sm);
+	if (have < want && tid == 0) {
+		kv_flag(a.status, KV_NO_PAGE);
+	}
+	for (int k = tid; k < n * mp; k += KV_BOOK) {
+		const int i = k / mp, c = k - i * mp, par = a.parents[i];
+		int p = -1;
+		if (par >= 0 && par < n && (first[par] == i || c < a.lens[par] / KV_PAGE)) {
+			p = a.table[par * mp + c];
+		}
+		a.table_out[k] = p;
+	}
+	__syncthreads();
+	for (int i = tid; i < n; i += KV_BOOK) {
+		const int at = a.copy[2 * i];
+		int from = -1, to = -1;
+		if (at >= 0 && at < have) {
+			const int par = a.parents[i], c = a.lens[par] / KV_PAGE;
+			from = a.table[par * mp + c], to = list[at];
+			a.table_out[i * mp + c] = to;
+			a.refs_out[to] = 1;
+		}
+		a.copy[2 * i] = from, a.copy[2 * i + 1] = to;
+	}
+}
+
+struct KvReserveArgs {
+	int *table, *refs;
+	const int *lens, *lens_new;
+	unsigned* status;
+	int n_rows, max_pages, n_pages;
+};
+
+// pages for the tokens [lens[r], lens_new[r]) of every row: rows in order, a row's pages in order, the lowest free page each
+__global__ __launch_bounds__(KV_BOOK) void k_kv_reserve(KvReserveArgs a) {
+	__shared__ int list[KV_MAX_ROWS], sm[KV_BOOK / 64];
+	const int tid = threadIdx.x, n = a.n_rows, mp = a.max_pages;
+	// a row at a time per thread; a call adds few pages to a row (a prompt: its pages)
+	for (int i0 = 0; i0 < n; i0 += KV_BOOK) {
+		const int i = i0 + tid;
+		int c0 = 0, c1 = 0;
+		if (i < n) {
+			const int len = a.lens[i] < 0 ? 0 : a.lens[i], to = a.lens_new[i] < 0 ? 0 : a.lens_new[i];
+			c0 = len / KV_PAGE, c1 = to > len ? (to - 1) / KV_PAGE + 1 : c0;
+			if (c1 > mp) {
+				kv_flag(a.status, KV_NO_PAGE);
+				c1 = mp;
+			}
+		}
+		int need = 0;
+		for (int c = c0; c < c1; ++c) {
+			need += a.table[(size_t)i * mp + c] < 0;
+		}
+		int total;
+		int at = kv_block_scan(need, sm, total);
+		// in portions of what `list` holds
+		for (int done = 0; done < total; done += KV_MAX_ROWS) {
+			const int want = total - done < KV_MAX_ROWS ? total - done : KV_MAX_ROWS;
+			const int have = kv_free_pages(a.refs, a.n_pages, want, list, sm);
+			if (have < want && tid == 0) {
+				kv_flag(a.status, KV_NO_PAGE);
+			}
+			while (c0 < c1 && at < done + want) {
+				if (a.table[(size_t)i * mp + c0] < 0) {
+					if (at - done < have) {
+						a.table[(size_t)i * mp + c0] = list[at - done];
+						__hip_atomic_store(a.refs + list[at - done], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+					}
+					++at;
+				}
+				++c0;
+			}
+			__threadfence();
+			__syncthreads();
+		}
+	}
+}
+
+// pages that no later token of their row sees: behind its tokens (lens[r] = 0: the whole row), or, under a window, before it and not
+// among the first tokens
+__global__ __launch_bounds__(256) void k_kv_trim(KvReserveArgs a, int window, int sinks) {
+	const int k = blockIdx.x * 256 + threadIdx.x, mp = a.max_pages;
+	if (k >= a.n_rows * mp) {
+		return;
+	}
+	const int r = k / mp, c = k - r * mp;
+	const int len = a.lens[r] < 0 ? 0 : a.lens[r];
+	const bool behind = c * KV_PAGE >= len;
+	const bool before = window > 0 && len >= window && c * KV_PAGE + KV_PAGE - 1 <= len - window && c * KV_PAGE >= sinks;
+	const int p = behind || before ? a.table[k] : -1;
+	if (p >= 0) {
+		a.table[k] = -1;
+		if (p < a.n_pages) {
+			atomicSub(&a.refs[p], 1);
+		} else {
+			kv_flag(a.status, KV_BAD_PAGE);
+		}
+	}
+}
+
+struct KvCompactArgs {
+	const int *table, *refs;
+	int *table_out, *refs_out, *n_live, *map, *copy; // map: [pages], copy: [pages / 2] x {from, to}
+	unsigned* status;
+	int n_rows, max_pages, n_pages;
+};
+
+// live pages at or beyond n_live (their number) move into the free ones below it, both in ascending order
+__global__ __launch_bounds__(KV_BOOK) void k_kv_compact(KvCompactArgs a) {
+	__shared__ int sm[KV_BOOK / 64];
+	const int tid = threadIdx.x, n = a.n_pages;
+	int live = 0;
+	for (int p0 = 0; p0 < n; p0 += KV_BOOK) {
+		const int p = p0 + tid;
+		int total;
+		kv_block_scan(p < n && a.refs[p] > 0, sm, total);
+		live += total;
+	}
+	if (tid == 0) {
+		*a.n_live = live;
+	}
+	int holes = 0, movers = 0;
+	for (int p0 = 0; p0 < n; p0 += KV_BOOK) {
+		const int p = p0 + tid, ref = p < n ? a.refs[p] : 0;
+		int nh, nm;
+		const bool hole = p < live && ref <= 0, mover = p < n && p >= live && ref > 0;
+		const int h = holes + kv_block_scan(hole, sm, nh), m = movers + kv_block_scan(mover, sm, nm);
+		if (hole) {
+			a.copy[2 * h + 1] = p;
+		}
+		if (mover) {
+			a.copy[2 * m] = p;
+		}
+		if (p < n) {
+			a.map[p] = p;
+			a.refs_out[p] = p < live ? ref : 0;
+		}
+		holes += nh, movers += nm;
+	}
+	__threadfence();
+	__syncthreads();
+	for (int i = tid; i < n / 2; i += KV_BOOK) {
+		if (i < movers) {
+			const int from = a.copy[2 * i], to = a.copy[2 * i + 1];
+			a.map[from] = to;
+			a.refs_out[to] = a.refs[from];
+		} else {
+			a.copy[2 * i + 1] = -1;
+		}
+	}
+	__threadfence();
+	__syncthreads();
+	for (int k = tid; k < a.n_rows * a.max_pages; k += KV_BOOK) {
+		const int p = a.table[k];
+		int q = p;
+		if (p >= n) {
+			kv_flag(a.status, KV_BAD_PAGE);
+		} else if (p >= 0) {
+			q = a.map[p];
+		}
+		a.table_out[k] = q;
+	}
+}
+
+struct KvCopyArgs {
+	signed char *k, *v;
+	float *ks, *vs;
+	const int* copy;
+	size_t page, pages; // bytes of a page's codes (K or V) of one layer; pages of a layer
+	int scales;         // floats of a page's scales of one layer
+};
+
+// grid = (copies at most, pieces of a page, layers): piece = 16 KiB of K and of V
+constexpr int KV_PIECE = 16384;
+__global__ __launch_bounds__(256) void k_kv_copy(KvCopyArgs a) {
+	const int from = a.copy[2 * blockIdx.x], to = a.copy[2 * blockIdx.x + 1];
+	if (to < 0) {
+		return;
+	}
+	const size_t l0 = blockIdx.z * a.pages;
+	const size_t src = (l0 + from) * a.page, dst = (l0 + to) * a.page;
+	const size_t b0 = (size_t)blockIdx.y * KV_PIECE + threadIdx.x * 16;
+	u32x4 x[2][KV_PIECE / 4096];
+#pragma unroll
+	for (int i = 0; i < KV_PIECE / 4096; ++i) {
+		const size_t b = b0 + 4096 * i;
+		if (b < a.page) {
+			x[0][i] = *(const u32x4*)(a.k + src + b), x[1][i] = *(const u32x4*)(a.v + src + b);
+		}
+	}
+#pragma unroll
+	for (int i = 0; i < KV_PIECE / 4096; ++i) {
+		const size_t b = b0 + 4096 * i;
+		if (b < a.page) {
+			*(u32x4*)(a.k + dst + b) = x[0][i], *(u32x4*)(a.v + dst + b) = x[1][i];
+		}
+	}
+	if (blockIdx.y == 0) {
+		for (int i = threadIdx.x; i < a.scales; i += 256) {
+			a.ks[(l0 + to) * a.scales + i] = a.ks[(l0 + from) * a.scales + i];
+			a.vs[(l0 + to) * a.scales + i] = a.vs[(l0 + from) * a.scales + i];
+		}
+	}
+}
+
+} // namespace calm

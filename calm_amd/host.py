@@ -30,6 +30,8 @@ TEST_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libcal
 EXPORTS = [
     "init_hip", "upload_hip", "alloc_hip", "prepare_hip", "forward_hip", "perf_hip", "calm_hip_device_count", "calm_hip_device_name", "calm_hip_configure", "calm_hip_query", "release_hip",
     "free_hip", "download_hip", "decode_greedy_hip", "decode_sample_hip", "prefill_hip", "prefill_logprobs_hip", "forward_stage_hip", "copy_hip", "perf_stage_hip",
+    "calm_hip_error", "calm_hip_stream", "kv_append_hip", "kv_read_hip", "kv_attend_hip", "kv_attend_workspace_hip", "kv_reserve_hip", "kv_trim_hip", "kv_fork_hip",
+    "kv_compact_hip", "beam_select_hip", "beam_workspace_hip",
 ]
 # include/calm_hip_test.h: libcalm_hip_test.so, tests and tools only
 TEST_EXPORTS = ["calm_hip_test_matvec", "calm_hip_test_norm_matvec", "calm_hip_test_attn", "calm_hip_test_argmax", "calm_hip_test_sample", "calm_hip_test_pf_gemm", "calm_hip_read_kv", "calm_hip_write_kv", "calm_hip_read_moe", "calm_hip_membench"]
@@ -102,6 +104,7 @@ def load_lib() -> "_Libs":
     lib = C.CDLL(LIB_PATH)
     T = C.POINTER(abi.Transformer)
     fp = C.POINTER(C.c_float)
+    p, i, n = C.c_void_p, C.c_int, C.c_long
     protos = {
         "init_hip": (None, []),
         "upload_hip": (C.c_void_p, [C.c_void_p, C.c_size_t]),
@@ -123,6 +126,19 @@ def load_lib() -> "_Libs":
         "forward_stage_hip": (fp, [T, C.c_int, C.c_int, C.c_uint, C.c_uint]),
         "copy_hip": (None, [C.c_void_p, C.c_void_p, C.c_size_t]),
         "perf_stage_hip": (C.c_double, [T, C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
+        # the operators on a paged cache and the beam selection (calm_amd/paged.py); struct KvPool / KvBatch go as addresses
+        "calm_hip_error": (C.c_char_p, []),
+        "calm_hip_stream": (p, []),
+        "kv_append_hip": (i, [p, p, i, p, p, i, n, n, n, n, p]),
+        "kv_read_hip": (i, [p, i, p, p, p, i, i, i, p, p, i, p]),
+        "kv_attend_workspace_hip": (C.c_longlong, [p, p, i, i, i, i]),
+        "kv_attend_hip": (i, [p, p, i, p, p, i, i, n, n, C.c_float, i, i, p, C.c_size_t, p]),
+        "kv_reserve_hip": (i, [p, p, p, p, p, i, i, p]),
+        "kv_trim_hip": (i, [p, p, p, p, i, i, i, i, p]),
+        "kv_fork_hip": (i, [p, p, p, p, p, i, i, p, p, p, C.c_size_t, p]),
+        "kv_compact_hip": (i, [p, p, p, i, i, p, p, p, p, C.c_size_t, p]),
+        "beam_workspace_hip": (C.c_longlong, [i, i, i]),
+        "beam_select_hip": (i, [p, i, n, i, i, i, p, p, i, p, p, p, p, p, C.c_size_t, p]),
     }
     for name, (res, args) in protos.items():
         fn = getattr(lib, name)  # raises AttributeError if the library does not export it

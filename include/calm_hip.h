@@ -192,6 +192,92 @@ int calm_hip_configure(const char* key, int value);
  * bounded waits that expired: 0 unless a launch lost a producer; the affected head's output is NaN).  -1 for an unknown key. */
 int calm_hip_query(const char* key, int value);
 
+/* ---- operators on a paged 8-bit cache, and the selection of a beam search ------------------------
+ *
+ * For hosts that keep several sequences: they take memory of the caller's (alloc_hip, or any device memory), launch on `stream` -- a
+ * hipStream_t of the current device; NULL is HIP's default stream, calm_hip_stream() the backend's own -- allocate nothing, do not
+ * synchronise, may be captured into a graph, and return 0, or -1 for a call they refuse (nothing has been launched then;
+ * calm_hip_error() says why).  Calls on one stream follow one another; calls on different streams need workspaces of their own.
+ *
+ * Types of rows: 0 = fp32, 1 = fp16, 2 = bf16.  Head sizes 64, 96, 128, 256. */
+
+/* A pool of pages of 64 tokens.  value = code * scale; a scale, a power of two, belongs to 16 tokens of one kv head:
+ *   k        int8  [n_layers][n_pages][n_kv_heads][64 tokens][head_dim]
+ *   v        int8  [n_layers][n_pages][n_kv_heads][4][head_dim][16]: byte 4 b + i of quad g and dim d is token 16 b + 4 g + i
+ *   k_scale, v_scale  float [n_layers][n_pages][n_kv_heads][4]
+ *   status   one device word that kernels OR what they find into (the host clears it): 1 a page that a call needs is missing from the
+ *            table or outside the pool (rows that see it are NaN, rows for it are not stored), 2 no page was free, 4 a sequence has more
+ *            new rows than the batch's max_rows, 8 a parent outside the table.
+ * Pages need no initialisation: nothing behind a sequence's tokens is read into a result. */
+struct KvPool {
+	signed char *k, *v;
+	float *k_scale, *v_scale;
+	unsigned* status;
+	int n_layers, n_pages, n_kv_heads, head_dim;
+};
+
+/* The rows of a call: rows starts[s] .. starts[s + 1] - 1 of the packed row arrays are the LAST tokens of sequence s, which has lens[s]
+ * tokens with them (device arrays: starts n_seqs + 1 ints, lens n_seqs, table n_seqs x max_pages page numbers, -1 where there is none).
+ * A sequence may have no rows; rows behind starts[n_seqs] are neither read nor written.  The host says how many rows there are
+ * (n_rows: the arrays hold that many), and bounds that only shape the launch: at most max_rows rows of one sequence, at most max_len
+ * tokens (a longer sequence is still attended in full; a sequence with more than max_rows rows is not: status 4). */
+struct KvBatch {
+	const int *table, *lens, *starts;
+	int n_seqs, max_pages, n_rows, max_rows, max_len;
+};
+
+/* why the last refused call of this thread was refused (static storage) */
+const char* calm_hip_error(void);
+
+/* the backend's own stream on the current stage's device (init_hip is run if it was not): what forward_hip and the others are ordered on */
+void* calm_hip_stream(void);
+
+/* Quantises the batch's K and V rows into their pages (which the table must hold already: kv_reserve_hip): element (row, head, dim) of k
+ * is at k[row * k_row + head * k_head + dim], strides in elements, multiples of 4.  A block's scale is the least power of two 2^e, e >=
+ * -126, with max|x| <= 127 * 2^e over its tokens; a block that holds older tokens keeps the larger of its scale and the new rows', and
+ * the older codes are rounded to it.  A block with an infinity or NaN is NaN from then on. */
+int kv_append_hip(const struct KvPool* pool, const struct KvBatch* batch, int layer, const void* k, const void* v, int type, long k_row, long k_head, long v_row, long v_head,
+                  void* stream);
+
+/* The values of tokens start[s] .. start[s] + count - 1 of every sequence, k and v dense [n_seqs][count][n_kv_heads][head_dim]; zeros
+ * where a sequence has no such token. */
+int kv_read_hip(const struct KvPool* pool, int layer, const int* table, const int* lens, const int* start, int n_seqs, int max_pages, int count, void* k, void* v, int type,
+                void* stream);
+
+/* Attention of the batch's query rows: a row at position p (its sequence's lens - rows + its place) sees tokens j <= p, with a window > 0
+ * only j > p - window or j < sinks; out = softmax(scale * q . K) . V over them, zeros where it sees none.  n_heads query heads, a multiple
+ * of the kv heads (head h reads kv head h / (n_heads / n_kv_heads)).  q strided like the rows above, out dense [n_rows][n_heads][head_dim]
+ * of q's type.  Table entries of pages that no row sees may be -1.  workspace: kv_attend_workspace_hip() bytes for the same arguments
+ * (0: none), written and read within the call. */
+long long kv_attend_workspace_hip(const struct KvPool* pool, const struct KvBatch* batch, int type, int n_heads, int window, int sinks);
+int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* batch, int layer, const void* q, void* out, int type, int n_heads, long q_row, long q_head, float scale, int window,
+                  int sinks, void* workspace, size_t workspace_size, void* stream);
+
+/* The upkeep of pages.  refs[p] = how many table rows list page p (int [n_pages], 0: free); a page that is not full belongs to one row.
+ * Up to 4096 table rows.  Free pages are taken lowest first, rows in order.
+ *   reserve  entries of the pages that tokens lens[r] .. lens_new[r] - 1 of row r need (in place)
+ *   trim     gives up pages behind lens[r] (0: all of them) and, with a window > 0, those that no later token sees (in place)
+ *   fork     row r becomes a copy of row parents[r] (out of place: table_out, refs_out; refs_out may be refs): full pages are shared, a
+ *            page that is not full stays with its row's first child and is copied, in all layers, for the others; rows without a
+ *            child give their pages up first.  workspace: 8 bytes a row
+ *   compact  the live pages beyond n_live = their number move, in all layers, into the free ones below it (table_out may be table; refs_out
+ *            is beside refs); pages n_live .. are free then.  workspace: 8 bytes a page */
+int kv_reserve_hip(const struct KvPool* pool, int* table, int* refs, const int* lens, const int* lens_new, int n_rows, int max_pages, void* stream);
+int kv_trim_hip(const struct KvPool* pool, int* table, int* refs, const int* lens, int n_rows, int max_pages, int window, int sinks, void* stream);
+int kv_fork_hip(const struct KvPool* pool, const int* table, const int* lens, const int* refs, const int* parents, int n_rows, int max_pages, int* table_out, int* refs_out,
+                void* workspace, size_t workspace_size, void* stream);
+int kv_compact_hip(const struct KvPool* pool, const int* table, const int* refs, int n_rows, int max_pages, int* table_out, int* refs_out, int* n_live, void* workspace,
+                   size_t workspace_size, void* stream);
+
+/* One selection step of a beam search over `groups` of `beams` (<= 32) hypotheses: the best `beams` of every group's beams x vocab
+ * continuations by scores[g][w] + log softmax(logits[g * beams + w])[v], best first, equal ones by w, then v.  logits: row stride `row`
+ * in elements.  A hypothesis with done[g][w] != 0 (done may be NULL) continues only with `eos`, its score unchanged; a continuation with
+ * eos is done.  eos < 0: none (done is not read).  A beam whose score is -inf or whose log-sum-exp is not finite offers only -inf.
+ * Outputs, [groups][beams] each, beside the inputs: scores, the beam that each continues (0 .. beams - 1), its token, done. */
+long long beam_workspace_hip(int groups, int beams, int vocab);
+int beam_select_hip(const void* logits, int type, long row, int groups, int beams, int vocab, const float* scores, const unsigned char* done, int eos, float* scores_out, int* parents,
+                    int* tokens, unsigned char* done_out, void* workspace, size_t workspace_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
