@@ -82,6 +82,12 @@ class Transformer(C.Structure):
     pass
 
 
+class BeamOptions(C.Structure):
+    """include/calm_hip.h: what decode_beam_hip searches with"""
+
+    _fields_ = [("n_beams", C.c_int), ("eos", C.c_int), ("window", C.c_int), ("sinks", C.c_int)]
+
+
 class Sampler(C.Structure):
     """reference src/sampler.h:3-9 (include/calm_abi.h)"""
 

@@ -14,6 +14,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <functional>
 #include <map>
 #include <mutex>
 #include <string>
@@ -230,6 +231,9 @@ struct GraphEntry {
 	hipGraphNode_t begin_node = nullptr;
 };
 
+struct BeamBuffers;
+void beam_free(BeamBuffers* b);
+
 struct Ctx {
 	struct Transformer* t = nullptr;
 	// shapes
@@ -274,6 +278,7 @@ struct Ctx {
 	float *pf_gate = nullptr, *pf_wsel = nullptr, *pf_xe = nullptr, *pf_y = nullptr;
 	int *pf_rows = nullptr, *pf_colexp = nullptr, *pf_slot = nullptr;
 	int pf_max_cols = 0;
+	struct BeamBuffers* beam = nullptr; // decode_beam_hip's memory, kept for the next call (beam_decode.hip.h)
 	// ... when the caller wants the log-probability of every next token: logits of the chunk, targets, results
 	int pf_score_nt = 0; // tokens per block of the scoring GEMM (pf_logits holds that many rows)
 	float *pf_logits = nullptr, *pf_lp = nullptr;
@@ -1295,15 +1300,24 @@ void launch_pf_attn(Ctx* c, int l, int nb, int pos0) {
 	}
 }
 
+// A chunk whose tokens are the next ones of several sequences instead of one prompt's: where their K / V rows go, and what attends to them
+// (decode_beam_hip: the paged cache)
+struct BatchStep {
+	const int* tokens;                   // device
+	void *k, *v;                         // this layer's new rows, [kv head][row][head_dim] binary16
+	std::function<void(int)> attend;     // layer: k, v and Ctx::pf_q -> Ctx::pf_att
+	float* logits;                       // [row][vocab]
+};
+
 // one chunk of nb <= Ctx::pf_nt tokens at positions pos0 .. pos0 + nb - 1 (no wrap of the rolling buffer):
-// the layer loop of src/infer.c:349-458 with a token dimension
+// the layer loop of src/infer.c:349-458 with a token dimension.  With `batch`: nb tokens of nb sequences, all at pos0.
 template <int DB, int KVB>
-void prefill_chunk(Ctx* c, int nb, int pos0, bool score, bool embed) {
+void prefill_chunk(Ctx* c, int nb, int pos0, bool score, bool embed, const BatchStep* batch = nullptr) {
 	struct Config* p = &c->t->config;
 	struct Weights* w = &c->t->weights;
 	const int half_hd = c->head_dim / 2;
 	const int n0 = c->dim > half_hd ? c->dim : half_hd;
-	hipLaunchKernelGGL((k_pf_begin<DB>), dim3((n0 + 255) / 256, nb), dim3(256), 0, g_stream, c->pf_tok, pos0, c->pf_x,
+	hipLaunchKernelGGL((k_pf_begin<DB>), dim3((n0 + 255) / 256, nb), dim3(256), 0, g_stream, batch ? batch->tokens : c->pf_tok, pos0, batch ? 0 : 1, c->pf_x,
 	                   embed ? w->token_embedding_table : nullptr, c->dim, c->rope_freq, c->pf_rope, half_hd);
 	const dim3 block(256);
 	const int cols = (nb + 63) / 64;
@@ -1480,9 +1494,16 @@ void prefill_chunk(Ctx* c, int nb, int pos0, bool score, bool embed) {
 		a.out = c->pf_q;
 		a.kc = (char*)c->kc + (size_t)l * c->kv_layer_bytes, a.vc = (char*)c->vc + (size_t)l * c->kv_layer_bytes;
 		a.vt = c->vt ? (char*)c->vt + (size_t)l * c->kv_layer_bytes : nullptr;
+		if (batch) { // a cache of nb positions that holds the new rows alone
+			a.kc = batch->k, a.vc = batch->v, a.vt = nullptr, a.seq_len = nb, a.kv_pos0 = 0;
+		}
 		gemm(a, EpiQkv(), cols);
 		// causal attention of every token of the chunk over the cache (its own row included)
-		launch_pf_attn<KVB>(c, l, nb, pos0);
+		if (batch) {
+			batch->attend(l);
+		} else {
+			launch_pf_attn<KVB>(c, l, nb, pos0);
+		}
 		// x += wo . att   (src/infer.c:408-415)
 		a.xin = (const float4*)c->pf_att, a.K = c->q_dim, a.M = c->dim, a.w0 = w->wo[l], a.out = c->pf_x;
 		gemm(a, EpiResid(), cols);
@@ -1515,6 +1536,11 @@ void prefill_chunk(Ctx* c, int nb, int pos0, bool score, bool embed) {
 		m.xin = (const float4*)c->pf_h, m.K = c->hidden, m.M = c->dim, m.w0 = w->w2[l], m.out = c->pf_y;
 		gemm(m, std::integral_constant<int, PF_EPI_STORE>(), ecols);
 		hipLaunchKernelGGL(k_pf_combine, dim3(nb), block, 0, g_stream, c->pf_x, c->pf_y, c->pf_slot, c->pf_wsel, c->n_active, c->dim);
+	}
+	if (batch) { // final norm + classifier (src/infer.c:465-469): the logits are the caller's
+		hipLaunchKernelGGL(k_pf_norm, pf_norm_grid(nb, c->dim, g_ncu), block, 0, g_stream, (float4*)c->pf_xn, c->pf_x, w->rms_final_weight, c->dim, p->norm_eps, (int)p->norm_ln, nb);
+		a.xin = (const float4*)c->pf_xn, a.K = c->dim, a.M = c->vocab, a.w0 = w->wcls, a.out = batch->logits;
+		gemm(a, std::integral_constant<int, PF_EPI_STORE>(), cols);
 	}
 	if (score) {
 		// final norm + classifier for every token of the chunk (src/infer.c:465-469), then log softmax of the target
@@ -2210,6 +2236,7 @@ extern "C" void release_hip(struct Transformer* t) {
 	if (c->pf_flag) {
 		HIP_CHECK(hipHostFree(c->pf_flag));
 	}
+	beam_free(c->beam);
 	if (g_prof_ctx == c) {
 		g_prof_ctx = nullptr;
 	}
@@ -2597,6 +2624,7 @@ extern "C" double perf_stage_hip(struct Transformer* t, int stage, int iters, ui
 // ---------------------------------------------------------------- paged cache, beam selection ----
 
 #include "paged_api.hip.h"
+#include "beam_decode.hip.h"
 
 #ifdef CALM_TIMELINE
 // tools/timeline.py only (a separate build with -DCALM_TIMELINE): arm / read the per-wave stamps of kernels.hip.h

@@ -110,17 +110,18 @@ __host__ __device__ inline int pf_steps(int n) {
 	return (n + 63) >> 6;
 }
 
-// embedding rows + RoPE table of a chunk of tokens   (src/infer.c:334-347, :223-236)
+// embedding rows + RoPE table of a chunk of tokens   (src/infer.c:334-347, :223-236); step: positions between two tokens (0: a token of each
+// of several sequences, all at pos0)
 // grid = (ceil(max(dim, head_dim/2) / 256), nb)
 template <int DB>
-__global__ void k_pf_begin(const int* tokens, int pos0, float* X, const void* embed, int dim, const float* rope_freq, float2* rope, int half_hd) {
+__global__ void k_pf_begin(const int* tokens, int pos0, int step, float* X, const void* embed, int dim, const float* rope_freq, float2* rope, int half_hd) {
 	const int b = blockIdx.y;
 	const int i = blockIdx.x * blockDim.x + threadIdx.x;
 	if (embed && i < dim) { // (a later pipeline stage receives X from the stage before it)
 		X[(size_t)b * dim + i] = decode_elem<DB>(embed, (size_t)tokens[b] * dim + i);
 	}
 	if (i < half_hd) {
-		float val = (float)(pos0 + b) * rope_freq[i]; // src/infer.c:227-229
+		float val = (float)(pos0 + b * step) * rope_freq[i]; // src/infer.c:227-229
 		rope[b * half_hd + i] = make_float2(cosf(val), sinf(val));
 	}
 }

@@ -29,7 +29,7 @@ TEST_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libcal
 # include/calm_hip.h: the drop-in library
 EXPORTS = [
     "init_hip", "upload_hip", "alloc_hip", "prepare_hip", "forward_hip", "perf_hip", "calm_hip_device_count", "calm_hip_device_name", "calm_hip_configure", "calm_hip_query", "release_hip",
-    "free_hip", "download_hip", "decode_greedy_hip", "decode_sample_hip", "prefill_hip", "prefill_logprobs_hip", "forward_stage_hip", "copy_hip", "perf_stage_hip",
+    "free_hip", "download_hip", "decode_greedy_hip", "decode_sample_hip", "decode_beam_hip", "prefill_hip", "prefill_logprobs_hip", "forward_stage_hip", "copy_hip", "perf_stage_hip",
     "calm_hip_error", "calm_hip_stream", "kv_append_hip", "kv_read_hip", "kv_attend_hip", "kv_attend_workspace_hip", "kv_reserve_hip", "kv_trim_hip", "kv_fork_hip",
     "kv_compact_hip", "beam_select_hip", "beam_workspace_hip",
 ]
@@ -121,6 +121,7 @@ def load_lib() -> "_Libs":
         "download_hip": (None, [C.c_void_p, C.c_void_p, C.c_size_t]),
         "decode_greedy_hip": (fp, [T, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int)]),
         "decode_sample_hip": (fp, [T, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(abi.Sampler)]),
+        "decode_beam_hip": (i, [T, i, i, i, C.POINTER(abi.BeamOptions), C.POINTER(i), fp]),
         "prefill_hip": (None, [T, C.POINTER(C.c_int), C.c_int, C.c_int]),
         "prefill_logprobs_hip": (None, [T, C.POINTER(C.c_int), C.c_int, C.c_int, fp]),
         "forward_stage_hip": (fp, [T, C.c_int, C.c_int, C.c_uint, C.c_uint]),
@@ -369,6 +370,17 @@ class HipBackend:
         out = (C.c_int * n_steps)()
         p = self.lib.decode_sample_hip(C.byref(self.t), token, pos, n_steps, out, C.byref(sampler))
         return np.array(out[:], dtype=np.int64), np.ctypeslib.as_array(p, shape=(self.vocab,))
+
+    def decode_beam(self, token: int, pos: int, n_steps: int, n_beams: int, eos: int = -1, window: int = 0, sinks: int = 0):
+        """the n_beams best continuations of n_steps tokens behind the cached positions [0, pos) and `token` (decode_beam_hip): (tokens [n_beams, n_steps],
+        scores [n_beams]), best first; a continuation that ends with `eos` is filled up with it"""
+        if n_steps < 1 or not 1 <= n_beams <= 32:
+            raise ValueError("at least one step, 1 to 32 beams")
+        toks, scores = np.empty((n_beams, n_steps), dtype=np.int32), np.empty(n_beams, dtype=np.float32)
+        opt = abi.BeamOptions(n_beams, eos, window, sinks)
+        if self.lib.decode_beam_hip(C.byref(self.t), token, pos, n_steps, C.byref(opt), toks.ctypes.data_as(C.POINTER(C.c_int)), fptr(scores)):
+            raise ValueError(self.lib.calm_hip_error().decode())
+        return toks.astype(np.int64), scores
 
     def prefill(self, tokens, pos: int) -> None:
         """KV-cache effect of forward(tokens[i], pos + i, FF_UPDATE_KV_ONLY) for every i, batched (prefill_hip)"""

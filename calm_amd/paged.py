@@ -28,6 +28,7 @@ PAGE, BLOCK = 64, 16
 HEAD_DIMS = (64, 96, 128, 256)
 MAX_BEAMS = 32
 _TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_NAMES = {}  # a dtype object -> its name (str(torch.float16) costs a microsecond)
 _SIZES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "int8": 1, "uint8": 1, "bool": 1}
 
 
@@ -105,8 +106,25 @@ def _lib():
 
 
 def _name(x) -> str:
-    d = str(x.dtype)
-    return d[6:] if d.startswith("torch.") else d
+    d = x.dtype
+    n = _NAMES.get(d)
+    if n is None:
+        n = str(d)
+        n = _NAMES[d] = n[6:] if n.startswith("torch.") else n
+    return n
+
+
+_torch = None  # torch and the functions that every call asks, once it is known to be there
+
+
+def _torch_calls():
+    global _torch
+    if _torch is None:
+        import torch
+
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle alone, without a Stream object around it
+        _torch = (torch, torch.Tensor, raw or (lambda i: torch.cuda.current_stream(i).cuda_stream), getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device))
+    return _torch
 
 
 class _On:
@@ -116,27 +134,29 @@ class _On:
 
     def __init__(self, arrays):
         first = arrays[0]
+        self._guard = None
         if isinstance(first, DeviceArray):
             for a in arrays:
                 if not isinstance(a, DeviceArray):
                     raise ValueError("tensors and DeviceArrays in one call")
-            self._guard = None
             self.stream = _lib().calm_hip_stream()
             return
-        import torch
-
+        torch, tensor, raw_stream, current = _torch or _torch_calls()
         dev = first.device
         if dev.type != "cuda":
             raise ValueError(f"arrays on {dev}: these operators run on the GPU only")
+        grads = torch.is_grad_enabled()
         for a in arrays:
-            if not isinstance(a, torch.Tensor):
+            if not isinstance(a, tensor):
                 raise ValueError("tensors and DeviceArrays in one call")
             if a.device != dev:
                 raise ValueError(f"arrays on {dev} and on {a.device} in one call")
-            if a.requires_grad and torch.is_grad_enabled():
+            if grads and a.requires_grad:
                 raise ValueError("there is no backward pass: call under torch.no_grad()")
-        self._guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-        self.stream = torch.cuda.current_stream(dev).cuda_stream
+        index = dev.index
+        if index != current():
+            self._guard = torch.cuda.device(dev)
+        self.stream = raw_stream(index)
 
     def __enter__(self):
         if self._guard is not None:
@@ -151,8 +171,7 @@ class _On:
 def _empty(like, shape, dtype: str):
     if isinstance(like, DeviceArray):
         return DeviceArray(shape, dtype)
-    import torch
-
+    torch = (_torch or _torch_calls())[0]
     return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
 
 

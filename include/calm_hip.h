@@ -103,6 +103,22 @@ float* decode_greedy_hip(struct Transformer* transformer, int token, int pos, in
  * and a bracketed running sum; the reference's own sum is compiled -ffast-math). */
 float* decode_sample_hip(struct Transformer* transformer, int token, int pos, int n_steps, int* out_tokens, struct Sampler* sampler);
 
+/* A beam search on the device: the n_beams best continuations of n_steps tokens that it finds behind the model's cached positions
+ * [0, pos) and `token` at pos -- the sum of log softmax over a continuation's tokens is its score, every step keeps the n_beams best of the
+ * n_beams x vocab extensions (beam_select_hip below; a hypothesis that took `eos` is finished and keeps its score).  Writes
+ * out_tokens[n_beams][n_steps], best first, filled up with eos behind a finished hypothesis' end, and out_scores[n_beams].  The hypotheses' rows
+ * live in a paged 8-bit cache of their own (the operators below) that takes the prompt from the model's cache, fp16 or e5m2; the model's
+ * cache is only read.  With a window > 0 a position sees the last `window` positions and the first `sinks` (the whole context otherwise).
+ * Weights are streamed once per step for all hypotheses (the batched layers of prefill_hip).  Returns 0, or -1 for a call it refuses
+ * (calm_hip_error()): positions at or beyond seq_len, more than 32 beams, head sizes other than 64, 96, 128, 256, and -- noticed at
+ * the end -- an activation that left binary16's range. */
+struct BeamOptions {
+	int n_beams;
+	int eos; /* -1: none */
+	int window, sinks;
+};
+int decode_beam_hip(struct Transformer* transformer, int token, int pos, int n_steps, const struct BeamOptions* options, int* out_tokens, float* out_scores);
+
 /* Batched prompt ingestion: the KV-cache effect of
  *     for (i = 0; i < n; ++i) forward_hip(transformer, tokens[i], pos + i, FF_UPDATE_KV_ONLY);
  * i.e. of the reference's serial prompt loop (src/run.c:208,216-218; README.md:80 "prompt processing is
