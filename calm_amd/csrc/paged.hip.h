@@ -24,6 +24,7 @@ enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
 typedef _Float16 kv_f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 kv_f16x8 __attribute__((ext_vector_type(8)));
 typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
+typedef int kv_i32x4 __attribute__((ext_vector_type(4)));
 typedef float kv_f32x16 __attribute__((ext_vector_type(16)));
 
 // one layer of a pool
@@ -399,8 +400,18 @@ __device__ __forceinline__ float kv_row_top(const float (&x)[N]) {
 	}
 	return m;
 }
-__device__ __forceinline__ float kv_xor_max(float v, int o) {
-	return fmaxf(v, __shfl_xor(v, o));
+// maximum with the lane 32 (16) away: a swap of register halves, no trip through the LDS crossbar
+__device__ __forceinline__ float kv_max32(float v) {
+	const unsigned b = __builtin_bit_cast(unsigned, v);
+	const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+	const unsigned x = r[0], y = r[1];
+	return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+__device__ __forceinline__ float kv_max16(float v) {
+	const unsigned b = __builtin_bit_cast(unsigned, v);
+	const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+	const unsigned x = r[0], y = r[1];
+	return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
 }
 __device__ __forceinline__ float kv_exp2(float x) {
 	return __builtin_amdgcn_exp2f(x); // one unit in the last place; below 2^-126 zero
@@ -430,8 +441,7 @@ __device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t 
 // are in flight throughout.  The waves' sums meet in LDS; ranges of one row meet in k_kv_merge.
 // grid = (splits, kv heads x tiles, seqs)
 template <int D, int DT, int NR>
-__global__ __launch_bounds__(256) void k_kv_decode(KvAttnArgs a) {
-	constexpr int KS = D / 32;  // k-steps of S^T
+__global__ __launch_bounds__(256, NR * D <= 128 ? 2 : 1) void k_kv_decode(KvAttnArgs a) {
 	constexpr int ND = D / 16;  // dim tiles of O^T
 	constexpr int KW = D / 16;  // dwords of a K row per lane
 	constexpr bool HL = DT == KV_F32;
@@ -476,48 +486,7 @@ __global__ __launch_bounds__(256) void k_kv_decode(KvAttnArgs a) {
 		}
 		return;
 	}
-	// q: lane (col, g) holds dims g D / 4 .. of its row, k-step i the eight at i 8 -- K's lanes take the same dims
-	kv_f16x8 qh[NR][KS], ql[NR][HL ? KS : 1];
-	float qf[NR];
-#pragma unroll
-	for (int c = 0; c < NR; ++c) {
-		float x[D / 4];
-		const size_t at = (row[c] / a.n_heads) * (size_t)a.q_row + (row[c] % a.n_heads) * (size_t)a.q_head + g * (D / 4);
-#pragma unroll
-		for (int i = 0; i < D / 16; ++i) {
-			float y[4];
-			kv_load4<DT>(a.q, at + 4 * i, y);
-			x[4 * i] = y[0], x[4 * i + 1] = y[1], x[4 * i + 2] = y[2], x[4 * i + 3] = y[3];
-		}
-		float top = kv_row_top<DT>(x);
-		top = kv_xor_max(kv_xor_max(top, 16), 32);
-		const int e = kv_row_exp(top);
-		const float inv = kv_exp2i(-e);
-		qf[c] = kv_exp2i(e) * a.scale;
-#pragma unroll
-		for (int i = 0; i < KS; ++i) {
-#pragma unroll
-			for (int j = 0; j < 8; ++j) {
-				const float y = x[8 * i + j] * inv;
-				qh[c][i][j] = (_Float16)y;
-				if constexpr (HL) {
-					ql[c][i][j] = (_Float16)(y - (float)qh[c][i][j]);
-				}
-			}
-		}
-	}
-	float m[NR], l[NR];
-	kv_f32x4 o[NR][ND];
-#pragma unroll
-	for (int c = 0; c < NR; ++c) {
-		m[c] = -__builtin_inff(), l[c] = 0.f;
-#pragma unroll
-		for (int d = 0; d < ND; ++d) {
-			o[c][d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
-		}
-	}
-	float E = 1.1754944e-38f; // the largest V scale met
-	// page ids of this wave's next 64 pages, one per lane
+	// page ids of this wave's next 64 pages, one per lane; the first pages' codes are asked for before q is looked at
 	int ids = -1, ids0 = i0 + wave; // lane i: page ids0 + 4 i
 	const auto fetch_ids = [&](int first) {
 		ids0 = first;
@@ -572,6 +541,69 @@ __global__ __launch_bounds__(256) void k_kv_decode(KvAttnArgs a) {
 		load_k(pid);
 		load_v(pid);
 	}
+	__builtin_amdgcn_sched_barrier(0); // (the loads stay ahead of what follows)
+	// q as NQ signed digits of eight bits, row / 2^e = (d0 + d1 / 254 + d2 / 254^2) / 127: lane (col, g) holds dims g D / 4 .. of its row
+	constexpr int NQ = HL ? 3 : 2;
+	unsigned qd[NR][NQ][KW];
+	float qf[NR];
+#pragma unroll
+	for (int c = 0; c < NR; ++c) {
+		float x[D / 4];
+		const size_t at = (row[c] / a.n_heads) * (size_t)a.q_row + (row[c] % a.n_heads) * (size_t)a.q_head + g * (D / 4);
+		unsigned top = 0;
+#pragma unroll
+		for (int i = 0; i < D / 16; ++i) {
+			float y[4];
+			kv_load4<DT>(a.q, at + 4 * i, y);
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				x[4 * i + j] = y[j];
+				const unsigned u = __builtin_bit_cast(unsigned, y[j]) & 0x7fffffffu;
+				top = top > u ? top : u;
+			}
+		}
+		const unsigned t1 = __shfl_xor(top, 16);
+		top = top > t1 ? top : t1;
+		const unsigned t2 = __shfl_xor(top, 32);
+		top = top > t2 ? top : t2;
+		const int e = kv_row_exp(__builtin_bit_cast(float, top));
+		const float inv = kv_exp2i(-e) * 127.f;
+		// (a row with an infinity or a NaN is NaN)
+		qf[c] = top >= 0x7f800000u ? __builtin_nanf("") : kv_exp2i(e) * a.scale * (1.f / 127.f);
+#pragma unroll
+		for (int i = 0; i < KW; ++i) {
+			unsigned w[NQ];
+#pragma unroll
+			for (int n = 0; n < NQ; ++n) {
+				w[n] = 0;
+			}
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				float y = x[4 * i + j] * inv; // (2^-126 * 127: no denormal)
+#pragma unroll
+				for (int n = 0; n < NQ; ++n) {
+					const float r = __builtin_rintf(y);
+					w[n] |= ((unsigned)(int)r & 0xffu) << (8 * j);
+					y = (y - r) * 254.f;
+				}
+			}
+#pragma unroll
+			for (int n = 0; n < NQ; ++n) {
+				qd[c][n][i] = w[n];
+			}
+		}
+	}
+	float m[NR], l[NR];
+	kv_f32x4 o[NR][ND];
+#pragma unroll
+	for (int c = 0; c < NR; ++c) {
+		m[c] = -__builtin_inff(), l[c] = 0.f;
+#pragma unroll
+		for (int d = 0; d < ND; ++d) {
+			o[c][d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
+		}
+	}
+	float E = 1.1754944e-38f; // the largest V scale met
 	for (int i = i0 + wave; i < i1; i += 4) {
 		const int pg = sp.page(i), j0 = pg * KV_PAGE;
 		const bool bad = pid < 0;
@@ -580,23 +612,39 @@ __global__ __launch_bounds__(256) void k_kv_decode(KvAttnArgs a) {
 			fetch_ids(i + 4);
 		}
 		const int next = more ? __builtin_amdgcn_readlane(ids, (i + 4 - ids0) >> 2) : -1;
-		// S^T of the page: tile t = block t, this lane's tokens 4 g + e
+		// S^T of the page: tile t = block t, this lane's tokens 4 g + e; whole numbers, exactly
 		kv_f32x4 sc[NR][4];
 #pragma unroll
 		for (int t = 0; t < 4; ++t) {
 #pragma unroll
 			for (int c = 0; c < NR; ++c) {
-				sc[c][t] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
-			}
+				kv_i32x4 acc[NQ];
 #pragma unroll
-			for (int k = 0; k < KS; ++k) {
-				const kv_f16x8 kf = kv_codes8(kr[t][2 * k], kr[t][2 * k + 1]);
+				for (int n = 0; n < NQ; ++n) {
+					acc[n] = (kv_i32x4){0, 0, 0, 0};
+					if constexpr (D % 64 == 0) {
 #pragma unroll
-				for (int c = 0; c < NR; ++c) {
-					sc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[c][k], sc[c][t], 0, 0, 0);
-					if constexpr (HL) {
-						sc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[c][k], sc[c][t], 0, 0, 0);
+						for (int k = 0; k < D / 64; ++k) {
+							const kv_i32x4 kf = {(int)kr[t][4 * k], (int)kr[t][4 * k + 1], (int)kr[t][4 * k + 2], (int)kr[t][4 * k + 3]};
+							const kv_i32x4 qv = {(int)qd[c][n][4 * k], (int)qd[c][n][4 * k + 1], (int)qd[c][n][4 * k + 2], (int)qd[c][n][4 * k + 3]};
+							acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qv, acc[n], 0, 0, 0);
+						}
+					} else {
+#pragma unroll
+						for (int k = 0; k < D / 32; ++k) {
+							const long kf = (long)(((unsigned long)kr[t][2 * k + 1] << 32) | kr[t][2 * k]);
+							const long qv = (long)(((unsigned long)qd[c][n][2 * k + 1] << 32) | qd[c][n][2 * k]);
+							acc[n] = __builtin_amdgcn_mfma_i32_16x16x32_i8(kf, qv, acc[n], 0, 0, 0);
+						}
 					}
+				}
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					float y = __builtin_fmaf((float)acc[1][e], 1.f / 254.f, (float)acc[0][e]);
+					if constexpr (HL) {
+						y = __builtin_fmaf((float)acc[2][e], 1.f / (254.f * 254.f), y);
+					}
+					sc[c][t][e] = y;
 				}
 			}
 		}
@@ -610,56 +658,77 @@ __global__ __launch_bounds__(256) void k_kv_decode(KvAttnArgs a) {
 #pragma unroll
 		for (int t = 0; t < 4; ++t) {
 			const int jb = j0 + 16 * t;
-			const bool seen = jb <= p_max && (a.window <= 0 || jb + 15 > p_min - a.window || jb < a.sinks);
+			const bool seen = whole || (jb <= p_max && (a.window <= 0 || jb + 15 > p_min - a.window || jb < a.sinks));
 			Enew = fmaxf(Enew, seen ? fabsf(vsc[t]) : 0.f);
 		}
-		const float grow = E * __builtin_amdgcn_rcpf(Enew), rE = __builtin_amdgcn_rcpf(Enew);
+		const float rE = __builtin_amdgcn_rcpf(Enew), grow = E * rE;
 		E = Enew;
 		kv_f16x8 pf[NR][2], pl[NR][HL ? 2 : 1];
 #pragma unroll
 		for (int c = 0; c < NR; ++c) {
-			float top = m[c];
+			float top = -__builtin_inff();
+			if (!whole) {
 #pragma unroll
-			for (int t = 0; t < 4; ++t) {
-				const float f = kscale[t] * qf[c];
+				for (int t = 0; t < 4; ++t) {
 #pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					float x = sc[c][t][e] * f;
-					if (!whole) {
+					for (int e = 0; e < 4; ++e) {
 						const int j = j0 + 16 * t + 4 * g + e;
 						const bool seen = j <= pos[c] && (a.window <= 0 || j > pos[c] - a.window || j < a.sinks);
-						x = seen ? x : -__builtin_inff();
+						sc[c][t][e] = seen ? sc[c][t][e] * (kscale[t] * qf[c]) : -__builtin_inff();
+						top = fmaxf(top, sc[c][t][e]);
 					}
-					sc[c][t][e] = x;
-					top = fmaxf(top, x);
+				}
+			} else {
+#pragma unroll
+				for (int t = 0; t < 4; ++t) {
+					const float f = kscale[t] * qf[c];
+					const float hi = fmaxf(fmaxf(sc[c][t][0], sc[c][t][1]), fmaxf(sc[c][t][2], sc[c][t][3])) * f;
+					const float lo = fminf(fminf(sc[c][t][0], sc[c][t][1]), fminf(sc[c][t][2], sc[c][t][3])) * f;
+					top = fmaxf(top, fmaxf(hi, lo)); // (a negative factor turns them round)
 				}
 			}
-			top = kv_xor_max(kv_xor_max(top, 16), 32);
-			const float ref = top == -__builtin_inff() ? 0.f : top;
-			const float alpha = kv_exp2(m[c] - ref); // (m = -inf: 0)
-			m[c] = top;
-			l[c] *= alpha;
+			top = kv_max32(kv_max16(top));
+			// the reference stays unless a score passes it by 2^8 (weights up to 2^8 are no less exact): sums are seldom rescaled
+			const float ref = top > m[c] + 8.f || m[c] == -__builtin_inff() ? fmaxf(top, m[c]) : m[c];
+			const float zero_ref = ref == -__builtin_inff() ? 0.f : ref;
+			const float alpha = kv_exp2(m[c] - zero_ref); // (m = -inf: 0)
+			m[c] = ref;
 			const float og = alpha * grow;
 			if (__ballot(og != 1.f)) {
+				l[c] *= alpha;
 #pragma unroll
 				for (int d = 0; d < ND; ++d) {
 					o[c][d] *= og;
 				}
 			}
+			if (!whole) {
 #pragma unroll
-			for (int t = 0; t < 4; ++t) {
-				const float f = vsc[t] * rE;
+				for (int t = 0; t < 4; ++t) {
+					const float f = vsc[t] * rE;
 #pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					const float w = kv_exp2(sc[c][t][e] - ref);
-					l[c] += w;
-					float y = w * f;
-					if (!whole) { // (a NaN scale must not reach a row that does not see the token)
-						y = sc[c][t][e] == -__builtin_inff() ? 0.f : y;
+					for (int e = 0; e < 4; ++e) {
+						const float w = kv_exp2(sc[c][t][e] - zero_ref);
+						l[c] += w;
+						const float y = sc[c][t][e] == -__builtin_inff() ? 0.f : w * f; // (a NaN scale must not reach a row that does not see the token)
+						pf[c][t >> 1][4 * (t & 1) + e] = (_Float16)y;
+						if constexpr (HL) {
+							pl[c][t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[c][t >> 1][4 * (t & 1) + e]);
+						}
 					}
-					pf[c][t >> 1][4 * (t & 1) + e] = (_Float16)y;
-					if constexpr (HL) {
-						pl[c][t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[c][t >> 1][4 * (t & 1) + e]);
+				}
+			} else {
+#pragma unroll
+				for (int t = 0; t < 4; ++t) {
+					const float f = kscale[t] * qf[c], fv = vsc[t] * rE;
+#pragma unroll
+					for (int e = 0; e < 4; ++e) {
+						const float w = kv_exp2(__builtin_fmaf(sc[c][t][e], f, -zero_ref));
+						l[c] += w;
+						const float y = w * fv;
+						pf[c][t >> 1][4 * (t & 1) + e] = (_Float16)y;
+						if constexpr (HL) {
+							pl[c][t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[c][t >> 1][4 * (t & 1) + e]);
+						}
 					}
 				}
 			}
@@ -787,7 +856,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 // Many rows (a prompt chunk): the matrix cores bound it.  A workgroup takes 128 rows (32 per wave) of one sequence and kv head and walks
 // the pages they see; a page's codes become binary16 ONCE per workgroup on their way into LDS (two buffers: the next page's loads are in
 // flight while a page is computed), laid out so that every operand is one 16-byte read of consecutive lanes.
-// grid = (row tiles, kv heads, seqs x splits)
+// grid = row tiles x seqs x splits x kv heads
 template <int D>
 struct KvChunk {
 	static constexpr int KROW = 65;                // 16-byte units between two (k-step, half) columns of K: 64 tokens and one of padding
@@ -795,8 +864,19 @@ struct KvChunk {
 	static constexpr size_t LDS = (size_t)2 * (KU + VU) * 16;
 };
 
+// n operands' LDS reads, KV_AHEAD of them ahead, each feeding m matrix instructions
+constexpr int KV_AHEAD = 6;
+#define KV_FEED(n, m)                                              \
+	do {                                                           \
+		__builtin_amdgcn_sched_group_barrier(0x100, KV_AHEAD, 0);  \
+		_Pragma("unroll") for (int mix_ = 0; mix_ < (n); ++mix_) { \
+			__builtin_amdgcn_sched_group_barrier(0x008, m, 0);     \
+			__builtin_amdgcn_sched_group_barrier(0x100, 1, 0);     \
+		}                                                          \
+	} while (0)
+
 template <int D, int DT>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a) {
+__global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) void k_kv_chunk(KvAttnArgs a) {
 	constexpr int KS = D / 16, ND = D / 32;
 	constexpr bool HL = DT == KV_F32;
 	constexpr int NK = (4 * D + 255) / 256, NV = (2 * D + 255) / 256; // staging items per thread
@@ -804,10 +884,20 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a)
 	extern __shared__ u32x4 kv_st[];
 	const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
 	const int col = lane & 31, hh = lane >> 5;
-	const int H = a.p.n_kv_heads, h = blockIdx.y, s = blockIdx.z / a.n_splits, split = blockIdx.z % a.n_splits;
+	const int H = a.p.n_kv_heads;
+	int r0, h, s, split;
+	{
+		// Workgroups in the order of their work, kv heads fastest: the tiles at a prompt's end see most pages and start first, and with the
+		// usual eight kv heads a head's pages meet in one XCD's L2 (tiles fastest: 125 instead of 79 us for ragged chunks under a window)
+		int i = (int)blockIdx.x;
+		h = i % H, i /= H;
+		split = i % a.n_splits, i /= a.n_splits;
+		s = i % a.r.n_seqs, i /= a.r.n_seqs;
+		r0 = ((int)gridDim.x / (H * a.n_splits * a.r.n_seqs) - 1 - i) * 128;
+	}
 	int row0, n, len;
 	kv_rows_of(a.r, s, row0, n, len);
-	const int nrows = n * a.group, r0 = blockIdx.x * 128;
+	const int nrows = n * a.group;
 	if (tid == 0 && r0 == 0 && h == 0 && split == 0 && n > a.r.max_rows) {
 		kv_flag(a.p.status, KV_BAD_BATCH);
 	}
@@ -847,10 +937,11 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a)
 			kv_load4<DT>(a.q, at + 16 * (i >> 1) + 4 * (i & 1), y);
 			top = fmaxf(top, kv_row_top<DT>(y));
 		}
-		top = kv_xor_max(top, 32);
+		top = kv_max32(top);
 		const int e = kv_row_exp(top);
 		const float inv = kv_exp2i(-e);
-		qf = kv_exp2i(e) * a.scale;
+		qf = kv_exp2i(e) * fabsf(a.scale);
+		const float sign = a.scale < 0.f ? -inv : inv;
 #pragma unroll
 		for (int i = 0; i < KS; ++i) {
 #pragma unroll
@@ -859,7 +950,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a)
 				kv_load4<DT>(a.q, at + 16 * i + 4 * j, y);
 #pragma unroll
 				for (int c = 0; c < 4; ++c) {
-					y[c] *= inv;
+					y[c] *= sign;
 					qh[i][4 * j + c] = (_Float16)y[c];
 					if constexpr (HL) {
 						ql[i][4 * j + c] = (_Float16)(y[c] - (float)qh[i][4 * j + c]);
@@ -869,29 +960,32 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a)
 		}
 	}
 	float m = -__builtin_inff(), l = 0.f, E = 1.1754944e-38f;
-	kv_f32x16 o[ND];
+	kv_f32x16 o[ND], zero;
+#pragma unroll
+	for (int e = 0; e < 16; ++e) {
+		zero[e] = 0.f;
+	}
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
-#pragma unroll
-		for (int e = 0; e < 16; ++e) {
-			o[d][e] = 0.f;
-		}
+		o[d] = zero;
 	}
-	u32x4 kr[NK], vr[NV][2];
-	const auto id_of = [&](int i) {
-		int pid = -1;
-		const int pg = sp.page(i);
-		if (pg < a.r.max_pages) {
-			pid = a.r.table[(size_t)s * a.r.max_pages + pg];
-		}
-		if (pid < 0 || pid >= a.p.n_pages) {
-			if (tid == 0) {
+	// page ids, 64 at a time across the lanes: a look-up per page would put two dependent round trips to memory into every step
+	int ids = -1, ids0 = i0;
+	const auto fetch_ids = [&](int first) {
+		ids0 = first;
+		const int i = first + lane;
+		ids = -1;
+		if (i < i1) {
+			const int pg = sp.page(i);
+			ids = pg < a.r.max_pages ? a.r.table[(size_t)s * a.r.max_pages + pg] : -1;
+			if (ids < 0 || ids >= a.p.n_pages) {
 				kv_flag(a.p.status, KV_BAD_PAGE);
+				ids = -1;
 			}
-			pid = -1;
 		}
-		return __builtin_amdgcn_readfirstlane(pid);
 	};
+	u32x4 kr[NK], vr[NV][2];
+	kv_f32x4 ksc_n, vsc_n; // the next page's scales
 	const auto load = [&](int pid) {
 		const size_t page = (size_t)(pid < 0 ? 0 : pid) * H + h;
 		const u32x4* const kp = (const u32x4*)(a.p.k + page * (KV_PAGE * D));
@@ -910,6 +1004,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a)
 				vr[i][0] = vp[it], vr[i][1] = vp[it + 2 * D];
 			}
 		}
+		ksc_n = *(const kv_f32x4*)(a.p.ks + page * 4), vsc_n = *(const kv_f32x4*)(a.p.vs + page * 4);
 	};
 	const auto stage = [&](int buf) {
 		u32x4* const kl = kv_st + buf * (KU + VU);
@@ -935,7 +1030,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a)
 	};
 	int pid = -1;
 	if (i0 < i1) {
-		pid = id_of(i0);
+		fetch_ids(i0);
+		pid = __builtin_amdgcn_readlane(ids, 0);
 		load(pid);
 		stage(0);
 	}
@@ -944,101 +1040,150 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_kv_chunk(KvAttnArgs a)
 		const int buf = (i - i0) & 1;
 		const bool more = i + 1 < i1;
 		const bool bad = pid < 0;
-		const size_t page = (size_t)(bad ? 0 : pid) * H + h;
-		const kv_f32x4 ksc = *(const kv_f32x4*)(a.p.ks + page * 4), vsc = *(const kv_f32x4*)(a.p.vs + page * 4);
+		const float none = __builtin_nanf("");
+		const kv_f32x4 ksc = bad ? (kv_f32x4){none, none, none, none} : ksc_n, vsc = vsc_n;
 		int next = -1;
 		if (more) {
-			next = id_of(i + 1);
+			if (i + 1 >= ids0 + 64) {
+				fetch_ids(i + 1);
+			}
+			next = __builtin_amdgcn_readlane(ids, i + 1 - ids0);
 			load(next);
 		}
 		const int j0 = sp.page(i) * KV_PAGE;
 		const bool some = j0 <= w_max && (a.window <= 0 || j0 + KV_PAGE - 1 > w_min - a.window || j0 < a.sinks);
 		if (some) {
-			const u32x4* const kl = kv_st + buf * (KU + VU);
-			const u32x4* const vl = kl + KU;
+			const bool whole = j0 + KV_PAGE - 1 <= w_min && (a.window <= 0 || j0 > w_max - a.window || j0 + KV_PAGE <= a.sinks);
+			// The operands' LDS reads run KV_AHEAD ahead of the matrix instructions, and the scheduler is held to it (left to itself it keeps two in
+			// flight: 190 instead of 187 us for 2049 rows on 4099 tokens); the scores go first where two waves want to issue (187 -> 183 us)
+			const u32x4* const kl = kv_st + buf * (KU + VU) + hh * KROW + col;
+			const u32x4* const vl = kv_st + buf * (KU + VU) + KU + hh * D + col;
 			kv_f32x16 sc[2];
+			__builtin_amdgcn_s_setprio(1);
+			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-			for (int b = 0; b < 2; ++b) {
+			for (int k = 0; k < KS; ++k) {
 #pragma unroll
-				for (int e = 0; e < 16; ++e) {
-					sc[b][e] = 0.f;
-				}
-#pragma unroll
-				for (int k = 0; k < KS; ++k) {
-					const kv_f16x8 kf = __builtin_bit_cast(kv_f16x8, kl[(2 * k + hh) * KROW + 32 * b + col]);
-					sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], sc[b], 0, 0, 0);
+				for (int b = 0; b < 2; ++b) {
+					const kv_f16x8 kf = __builtin_bit_cast(kv_f16x8, kl[2 * k * KROW + 32 * b]);
+					sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], k ? sc[b] : zero, 0, 0, 0);
 					if constexpr (HL) {
 						sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], sc[b], 0, 0, 0);
 					}
 				}
 			}
-			const bool whole = j0 + KV_PAGE - 1 <= w_min && (a.window <= 0 || j0 > w_max - a.window || j0 + KV_PAGE <= a.sinks);
-			float Enew = E;
+			KV_FEED(2 * KS, HL ? 2 : 1);
+			__builtin_amdgcn_sched_barrier(0);
+			__builtin_amdgcn_s_setprio(0);
+			float Enew = E, least = 3e38f;
+			unsigned odd = 0;
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
 				const int jb = j0 + 16 * b;
-				const bool seen = jb <= w_max && (a.window <= 0 || jb + 15 > w_min - a.window || jb < a.sinks);
-				Enew = fmaxf(Enew, seen ? fabsf(vsc[b]) : 0.f);
+				const bool seen = whole || (jb <= w_max && (a.window <= 0 || jb + 15 > w_min - a.window || jb < a.sinks));
+				const float vb = fabsf(vsc[b]), kb = ksc[b], vb0 = vsc[b];
+				Enew = fmaxf(Enew, seen ? vb : 0.f);
+				least = fminf(least, vb);
+				odd |= (__builtin_bit_cast(unsigned, vb0) & 0x807fffffu) | (__builtin_bit_cast(unsigned, kb) & 0x80000000u); // V: not a positive power of two, or NaN
 			}
-			const float rE = __builtin_amdgcn_rcpf(Enew), grow = E * rE;
+			const float rE = __builtin_amdgcn_rcpf(Enew);
+			float og = E * rE;
 			E = Enew;
-			float top = m;
+			odd |= __builtin_bit_cast(unsigned, E) & 0x807fffffu;
+			// token 32 (b / 2) + 8 (e / 4) + 4 hh + e % 4 of the page is element e % 16 of tile b / 2; block b holds elements 8 (b % 2) ..
+			kv_f16x8 pf[4], pl[HL ? 4 : 1];
+			if (whole && odd == 0 && least * 65536.f >= E) {
+				// Every row sees every token, and the V scales are powers of two within 2^-16 of E: the weight's V scale goes into its
+				// exponent, and the sum of weights takes it out again a block at a time -- 96 instructions of 300 less.
+				float top = m;
 #pragma unroll
-			for (int b = 0; b < 2; ++b) {
+				for (int b = 0; b < 4; ++b) {
+					float t = sc[b >> 1][8 * (b & 1)];
 #pragma unroll
-				for (int e = 0; e < 16; ++e) { // token 32 b + 8 (e / 4) + 4 hh + e % 4
-					float x = sc[b][e] * ((bad ? __builtin_nanf("") : ksc[2 * b + (e >> 3)]) * qf);
-					if (!whole) {
-						const int j = j0 + 32 * b + 8 * (e >> 2) + 4 * hh + (e & 3);
-						const bool seen = j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
-						x = seen ? x : -__builtin_inff();
+					for (int e = 1; e < 8; ++e) {
+						t = fmaxf(t, sc[b >> 1][8 * (b & 1) + e]);
 					}
-					sc[b][e] = x;
-					top = fmaxf(top, x);
+					top = fmaxf(top, t * (ksc[b] * qf)); // (the factor is not negative)
+				}
+				top = kv_max32(top);
+				// the reference stays unless a score passes it by 2^8: weights up to 2^8 are no less exact, and the sums are seldom rescaled
+				const float ref = top > m + 8.f ? top : m; // (finite: every row sees the page)
+				const float alpha = kv_exp2(m - ref); // (m = -inf: 0)
+				m = ref;
+				l *= alpha;
+				og *= alpha;
+#pragma unroll
+				for (int b = 0; b < 4; ++b) {
+					const float f = ksc[b] * qf, fv = vsc[b] * rE;
+					const float shift = (float)((int)(__builtin_bit_cast(unsigned, fv) >> 23) - 127) - ref;
+					float sum = 0.f;
+#pragma unroll
+					for (int e = 0; e < 8; ++e) {
+						const float y = kv_exp2(__builtin_fmaf(sc[b >> 1][8 * (b & 1) + e], f, shift));
+						sum += y;
+						pf[b][e] = (_Float16)y;
+						if constexpr (HL) {
+							pl[b][e] = (_Float16)(y - (float)pf[b][e]);
+						}
+					}
+					l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(fv), l);
+				}
+			} else {
+				float top = m;
+#pragma unroll
+				for (int b = 0; b < 4; ++b) {
+					const float f = ksc[b] * qf;
+#pragma unroll
+					for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; ++e) {
+						const int j = j0 + 32 * (b >> 1) + 8 * (e >> 2) + 4 * hh + (e & 3);
+						const bool seen = j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+						const float x = seen ? sc[b >> 1][e] * f : -__builtin_inff();
+						sc[b >> 1][e] = x;
+						top = fmaxf(top, x);
+					}
+				}
+				top = kv_max32(top);
+				const float ref = top == -__builtin_inff() ? 0.f : top;
+				const float alpha = kv_exp2(m - ref);
+				m = top;
+				l *= alpha;
+				og *= alpha;
+#pragma unroll
+				for (int b = 0; b < 4; ++b) {
+					const float fv = vsc[b] * rE;
+#pragma unroll
+					for (int e = 0; e < 8; ++e) {
+						const float x = sc[b >> 1][8 * (b & 1) + e];
+						const float w = kv_exp2(x - ref);
+						l += w;
+						const float y = x == -__builtin_inff() ? 0.f : w * fv; // (a NaN scale must not reach a row that does not see the token)
+						pf[b][e] = (_Float16)y;
+						if constexpr (HL) {
+							pl[b][e] = (_Float16)(y - (float)pf[b][e]);
+						}
+					}
 				}
 			}
-			top = kv_xor_max(top, 32);
-			const float ref = top == -__builtin_inff() ? 0.f : top;
-			const float alpha = kv_exp2(m - ref);
-			m = top;
-			l *= alpha;
-			const float og = alpha * grow;
 			if (__ballot(og != 1.f)) {
 #pragma unroll
 				for (int d = 0; d < ND; ++d) {
 					o[d] *= og;
 				}
 			}
+			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-			for (int b = 0; b < 2; ++b) {
+			for (int b = 0; b < 4; ++b) {
 #pragma unroll
-				for (int u = 0; u < 2; ++u) { // block 2 b + u
-					const float f = vsc[2 * b + u] * rE;
-					kv_f16x8 pf, pl;
-#pragma unroll
-					for (int e = 0; e < 8; ++e) {
-						const float x = sc[b][8 * u + e];
-						const float w = kv_exp2(x - ref);
-						l += w;
-						float y = w * f;
-						if (!whole) {
-							y = x == -__builtin_inff() ? 0.f : y;
-						}
-						pf[e] = (_Float16)y;
-						if constexpr (HL) {
-							pl[e] = (_Float16)(y - (float)pf[e]);
-						}
-					}
-#pragma unroll
-					for (int d = 0; d < ND; ++d) {
-						const kv_f16x8 vf = __builtin_bit_cast(kv_f16x8, vl[(2 * (2 * b + u) + hh) * D + 32 * d + col]);
-						o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[d], 0, 0, 0);
-						if constexpr (HL) {
-							o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[d], 0, 0, 0);
-						}
+				for (int d = 0; d < ND; ++d) {
+					const kv_f16x8 vf = __builtin_bit_cast(kv_f16x8, vl[2 * b * D + 32 * d]);
+					o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[b], o[d], 0, 0, 0);
+					if constexpr (HL) {
+						o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b], o[d], 0, 0, 0);
 					}
 				}
 			}
+			KV_FEED(4 * ND, HL ? 2 : 1);
+			__builtin_amdgcn_sched_barrier(0);
 		}
 		if (more) {
 			stage(buf ^ 1);

@@ -148,15 +148,31 @@ KvCut kv_cut(const struct KvPool* p, const struct KvBatch* b, int n_heads, int t
 		seen = span < seen ? span : seen;
 	}
 	seen = seen < 1 ? 1 : seen;
-	const long long wgs = (long long)b->n_seqs * p->n_kv_heads * c.tiles, want = (long long)kv_cus() * (c.chunked ? 2 : 4);
-	long long splits = (want + wgs - 1) / wgs;
-	splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
-	const int least = c.chunked ? 8 : 4; // pages: what a workgroup's start and the join of its sums are worth
-	long long chunk = (seen + splits - 1) / splits;
-	chunk = chunk < least ? least : chunk;
-	chunk = (chunk + 3) / 4 * 4;
-	c.chunk = (int)chunk;
-	c.n_splits = (int)((seen + chunk - 1) / chunk);
+	const long long wgs = (long long)b->n_seqs * p->n_kv_heads * c.tiles;
+	const int cus = kv_cus();
+	if (c.chunked) { // two workgroups per CU, at least 8 pages each (the join moves every row's partial sums through memory)
+		long long splits = (2ll * cus + wgs - 1) / wgs;
+		splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
+		const long long chunk = (seen + splits - 1) / splits;
+		c.chunk = (int)(chunk < 8 ? 8 : chunk);
+		c.n_splits = (int)((seen + c.chunk - 1) / c.chunk);
+		return c;
+	}
+	// What a cut into s ranges costs, in steps of a workgroup (a page for each of its four waves, about 1.5 us): two workgroups fit a CU, at 0.7
+	// of the time each, a round of them begins with the look-ups and first loads (2.5 steps), and ranges are joined by a second launch.
+	// Measured, s = 1 / 2 / 4 / 8: 8 sequences of 4093, 8 kv heads (64 workgroups uncut) - / - / 21.3 / 22.9 us; 64 of 91 - 8191, 4 kv heads (256)
+	// 49.7 / 39.3 / 41.5 / 46.4; one of 333 (8 workgroups, 6 pages) 10.7 / 15.
+	double best = 0;
+	for (long long n = 1; n <= 64 && (n == 1 || (n - 1) * 4 < seen); ++n) {
+		const double per_cu = (double)(wgs * n) / cus, rounds = ceil(per_cu / 2), step = per_cu <= 1 ? 1.0 : 1.4;
+		const long long chunk = ((seen + n - 1) / n + 3) / 4 * 4; // whole steps
+		const double cost = rounds * ((double)(chunk / 4) * step + 2.5) + (n > 1 ? 3.0 + 0.25 * (double)n : 0.0);
+		if (n == 1 || cost < 0.97 * best) {
+			best = cost;
+			c.chunk = (int)chunk;
+			c.n_splits = (int)((seen + chunk - 1) / chunk);
+		}
+	}
 	return c;
 }
 size_t kv_cut_bytes(const KvCut& c, const struct KvPool* p, const struct KvBatch* b, int n_heads) {
@@ -275,7 +291,7 @@ extern "C" int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* ba
 	a.n_heads = n_heads, a.group = n_heads / pool->n_kv_heads, a.window = window, a.sinks = sinks;
 	a.chunk = c.chunk, a.n_splits = c.n_splits, a.scale = scale * 1.4426950408889634f;
 	const int H = pool->n_kv_heads;
-	KV_CHECK(c.chunked ? (long long)batch->n_seqs * c.n_splits <= 65535 : (long long)H * c.tiles <= 65535, "too many sequences for rows this many and contexts this long");
+	KV_CHECK(c.chunked ? (long long)batch->n_seqs * c.n_splits * H * c.tiles <= 0x7fffffffll : (long long)H * c.tiles <= 65535, "too many sequences for rows this many and contexts this long");
 	return kv_dispatch(pool->head_dim, type, [&](auto Dc, auto Tc) {
 		constexpr int D = decltype(Dc)::value, T = decltype(Tc)::value;
 		const hipStream_t st = (hipStream_t)stream;
@@ -286,7 +302,7 @@ extern "C" int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* ba
 				if (kv_lds((const void*)kern, lds, "kv_attend_hip")) {
 					return -1;
 				}
-				hipLaunchKernelGGL(kern, dim3(c.tiles, H, batch->n_seqs * c.n_splits), dim3(256), lds, st, a);
+				hipLaunchKernelGGL(kern, dim3((unsigned)c.tiles * H * batch->n_seqs * c.n_splits), dim3(256), lds, st, a);
 			}
 		} else {
 			const auto go = [&](auto NRc) {
