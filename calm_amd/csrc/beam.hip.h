@@ -5,11 +5,11 @@
 // logit, or a NaN or +inf among them -- or whose score is -inf has totals of -inf; among those the lowest index comes first, too.
 //
 // Reading the logits once bounds it.  k_beam_rows: a workgroup takes a chunk of one row into registers, finds its maximum, the sum of
-// exponentials, and each wave its W best values (W rounds of a wave-wide maximum); four waves' lists become one.  k_beam_pick: one
-// workgroup per group joins the chunks' sums and lists into every row's W best, then the rows into the group's.
+// exponentials, and each wave its W best values (a bound that at least W reach, then an ordering of the few that do); four waves' lists
+// become one.  k_beam_pick: one workgroup per group joins the chunks' sums and lists into every row's W best, then the rows into the group's.
 //
-// The sum decides the order of continuations of DIFFERENT beams, where 32 bits lose what matters: differences and the sum are 64 bits
-// wide, the exponentials 32 (their errors, 2^-23 each, are not alike and average over the row).
+// The sum decides the order of continuations of DIFFERENT beams, where 32 bits lose what matters: sums and totals are 64 bits wide from a
+// lane's 32 values on; the exponentials are 32 (their errors, 2^-23 each, are not alike and average over the row).
 #pragma once
 
 namespace calm {
@@ -17,6 +17,7 @@ namespace calm {
 constexpr int BEAM_MAX = 32;
 constexpr int BEAM_VPT = 32;              // values per thread
 constexpr int BEAM_CHUNK = 256 * BEAM_VPT; // values per workgroup
+constexpr int BEAM_HITS = 16;              // lanes of a wave that k_beam_rows looks through one by one
 constexpr float BEAM_NONE = -__builtin_inff();
 
 struct BeamArgs {
@@ -53,6 +54,26 @@ __device__ __forceinline__ void beam_wave_best(T& v, int& i) {
 	}
 }
 
+// sum over the wave's lanes, in every lane (register moves, as wave_sum63)
+__device__ __forceinline__ double beam_wave_sum(double v) {
+	const auto dpp = [](double x, auto ctrl, auto row_mask) {
+		const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+		const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, decltype(ctrl)::value, decltype(row_mask)::value, 0xf, true);
+		const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), decltype(ctrl)::value, decltype(row_mask)::value, 0xf, true);
+		return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+	};
+	using F = std::integral_constant<int, 0xf>;
+	v += dpp(v, std::integral_constant<int, 0xb1>(), F());
+	v += dpp(v, std::integral_constant<int, 0x4e>(), F());
+	v += dpp(v, std::integral_constant<int, 0x114>(), F());
+	v += dpp(v, std::integral_constant<int, 0x118>(), F());
+	v += dpp(v, std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());
+	v += dpp(v, std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
+	const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+	const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, 63), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), 63);
+	return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+
 template <int DT>
 __device__ __forceinline__ float beam_load(const void* p, size_t i) {
 	if constexpr (DT == KV_F32) {
@@ -64,6 +85,21 @@ __device__ __forceinline__ float beam_load(const void* p, size_t i) {
 	}
 }
 
+// e^d, d <= 0: the product with log2 e takes the constant's second half along, so that its own rounding (the same for every value) does not add up
+__device__ __forceinline__ float beam_exp(float d) {
+	return kv_exp2(__builtin_fmaf(d, 1.44269502e+00f, d * 1.92596299e-08f)); // (-inf: 0)
+}
+
+// the waves' maxima and sums as the chunk's (64-bit exponentials here would take a workgroup longer than all its values' take)
+__device__ inline void beam_sums(const BeamArgs& a, size_t part, const float* m, const double* sum) {
+	const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+	double s = 0.;
+	for (int w = 0; w < 4; ++w) {
+		s += m[w] != BEAM_NONE ? sum[w] * (double)beam_exp(m[w] - M) : sum[w]; // (nothing: 0, or NaN)
+	}
+	a.sums[2 * part] = (double)M, a.sums[2 * part + 1] = s;
+}
+
 // grid = (chunks, rows)
 template <int DT>
 __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
@@ -71,7 +107,9 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	constexpr int NL = BEAM_VPT / VL;
 	__shared__ float sm_v[4 * BEAM_MAX];
 	__shared__ int sm_i[4 * BEAM_MAX];
-	__shared__ float sm_m[4];
+	__shared__ float sm_m[4], sm_c[256];
+	__shared__ int sm_ci[256], sm_n[4], sm_hl[4 * BEAM_HITS];
+	__shared__ __attribute__((aligned(16))) float sm_h[4 * BEAM_HITS][BEAM_VPT + 4];
 	__shared__ double sm_s[4];
 	const int lane = lane_id(), wave = wave_id(), chunk = blockIdx.x, row = blockIdx.y, W = a.beams;
 	const size_t part = (size_t)row * a.n_chunks + chunk;
@@ -119,31 +157,134 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 			}
 		}
 	}
-	float m = BEAM_NONE;
+	// this lane's largest value; the wave's
+	float mine = BEAM_NONE;
 #pragma unroll
 	for (int i = 0; i < BEAM_VPT; ++i) {
-		m = fmaxf(m, x[i]);
+		mine = fmaxf(mine, x[i]);
 	}
-	m = wave_max_dpp(m);
-	// sum of 2^((x - m) log2 e) relative to the wave's maximum
-	double sum = 0.;
+	const float m = wave_max_dpp(mine);
+	// sum of exponentials relative to the wave's maximum
 	const float ref = m == BEAM_NONE ? 0.f : m;
+	float part_sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 	for (int i = 0; i < BEAM_VPT; ++i) {
-		const double t = ((double)x[i] - (double)ref) * 1.4426950408889634074;
-		const double n = __builtin_rint(t);
-		// (-inf: n = -inf, the difference NaN)
-		const float f = x[i] == BEAM_NONE ? 0.f : ldexpf(kv_exp2((float)(t - n)), n < -200. ? -200 : (int)n);
-		sum += (double)f;
+		part_sum[i & 3] += beam_exp(x[i] - ref);
 	}
-#pragma unroll
-	for (int o = 32; o > 0; o >>= 1) {
-		sum += __shfl_xor(sum, o);
-	}
+	const double sum = beam_wave_sum(((double)part_sum[0] + (double)part_sum[1]) + ((double)part_sum[2] + (double)part_sum[3]));
 	if (lane == 0) {
 		sm_m[wave] = m, sm_s[wave] = sum;
 	}
-	// the wave's W best: its lanes' best, W times; the lane that gave one looks for its next
+	// The chunk's W best.  Its lanes are cut into groups, at least W of them; each group's largest value reaches the least of these, so at least W
+	// values of the chunk reach that bound.  What does (three times W on average, unless many are equal) goes to a list in LDS, a
+	// quarter a wave, where a candidate's place is the number of better ones.  Where a quarter would be longer than 64 -- equal values, the
+	// few values of a row's end -- rounds over all values find the best instead.  (One list with an atomic counter: 7 us more.)
+	float bound;
+	{
+		// (register moves across the lanes: through the LDS crossbar these few steps took as long as the logits)
+		const auto dpp = [](float x, auto ctrl) {
+			const int xi = __builtin_bit_cast(int, x);
+			return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(xi, xi, decltype(ctrl)::value, 0xf, 0xf, false));
+		};
+		float v = mine;
+		int size = 8; // lanes of a group; W <= 32 takes 8 groups a wave, 16: 4, 8: 2, 4: 1
+		v = fmaxf(v, dpp(v, std::integral_constant<int, 0xb1>()));
+		v = fmaxf(v, dpp(v, std::integral_constant<int, 0x4e>()));
+		v = fmaxf(v, dpp(v, std::integral_constant<int, 0x141>()));
+		if (W <= 16) {
+			v = fmaxf(v, dpp(v, std::integral_constant<int, 0x140>())), size = 16;
+		}
+		if (W <= 8) {
+			v = kv_max16(v), size = 32;
+		}
+		if (W <= 4) {
+			v = kv_max32(v), size = 64;
+		}
+		if (lane % size == 0) {
+			sm_c[wave * 8 + lane / size] = v;
+		}
+		__syncthreads();
+		const float least = -wave_max_dpp((lane & 7) < 64 / size && lane < 32 ? -sm_c[lane] : -__builtin_inff());
+		bound = least;
+	}
+	__syncthreads(); // (sm_c is the list from here on)
+	const auto place = [&](int i) { // the row's index of this lane's value i
+		return base + ((i / VL) * 256 + (int)threadIdx.x) * VL + i % VL;
+	};
+	const auto inside = [&](int at) { return at >= 0 && at < a.vocab; };
+	int mine_n = 0; // of the wave's own quarter of the list
+	const auto add = [&](bool in, float v, int at) {
+		const unsigned long long who = __ballot(in);
+		if (who) {
+			const int k = mine_n + __builtin_popcountll(who & ((1ull << lane) - 1));
+			if (in && k < 64) {
+				sm_c[wave * 64 + k] = v, sm_ci[wave * 64 + k] = at;
+			}
+			mine_n += __builtin_popcountll(who);
+		}
+	};
+	const unsigned long long hits = __ballot(mine >= bound);
+	const int n_hits = __builtin_popcountll(hits);
+	if (bound != BEAM_NONE && n_hits <= BEAM_HITS) {
+		// few lanes hold such values: they put all of theirs into LDS, and the wave looks through two lanes' at a time (a ballot for each of the
+		// 32 values of every lane: 6 us more for 16 x 8 beams over 128256)
+		if (mine >= bound) {
+			const int slot = wave * BEAM_HITS + __builtin_popcountll(hits & ((1ull << lane) - 1));
+			sm_hl[slot] = (int)threadIdx.x;
+#pragma unroll
+			for (int i = 0; i < BEAM_VPT; i += 4) {
+				*(kv_f32x4*)&sm_h[slot][i] = (kv_f32x4){x[i], x[i + 1], x[i + 2], x[i + 3]};
+			}
+		}
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		__builtin_amdgcn_wave_barrier();
+		for (int k = 0; k < n_hits; k += 2) {
+			const int slot = wave * BEAM_HITS + k + (lane >> 5), i = lane & 31;
+			const bool ok = k + (lane >> 5) < n_hits;
+			const float v = ok ? sm_h[slot][i] : BEAM_NONE;
+			add(v >= bound, v, ok ? base + ((i / VL) * 256 + sm_hl[slot]) * VL + i % VL : 0);
+		}
+	} else {
+#pragma unroll
+		for (int i = 0; i < BEAM_VPT; ++i) {
+			bool in = x[i] >= bound; // (false for a NaN)
+			if (bound == BEAM_NONE) {
+				in = in && inside(place(i)); // (what lies outside the row is -inf, too)
+			}
+			add(in, x[i], place(i));
+		}
+	}
+	if (lane == 0) {
+		sm_n[wave] = mine_n;
+	}
+	__syncthreads();
+	const int n0 = sm_n[0], n1 = sm_n[1], n2 = sm_n[2], n3 = sm_n[3], n = n0 + n1 + n2 + n3;
+	if (n0 <= 64 && n1 <= 64 && n2 <= 64 && n3 <= 64) {
+		const int t = threadIdx.x;
+		if (lane < mine_n) {
+			const float v = sm_c[t];
+			const int at = sm_ci[t];
+			int rank = 0;
+#pragma unroll
+			for (int w = 0; w < 4; ++w) {
+				const int nw = w == 0 ? n0 : w == 1 ? n1 : w == 2 ? n2 : n3;
+#pragma unroll 4
+				for (int k = 0; k < nw; ++k) {
+					rank += beam_better(sm_c[w * 64 + k], sm_ci[w * 64 + k], v, at) ? 1 : 0;
+				}
+			}
+			if (rank < W) {
+				a.val[part * W + rank] = v, a.idx[part * W + rank] = at;
+			}
+		}
+		if (t >= n && t < W) { // fewer than W values in all
+			a.val[part * W + t] = BEAM_NONE, a.idx[part * W + t] = -1;
+		}
+		if (t == 0) {
+			beam_sums(a, part, sm_m, sm_s);
+		}
+		return;
+	}
 	unsigned taken = 0;
 	float bv;
 	int bi;
@@ -151,8 +292,8 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 		bv = BEAM_NONE, bi = 0x7fffffff;
 #pragma unroll
 		for (int i = 0; i < BEAM_VPT; ++i) {
-			const int at = base + ((i / VL) * 256 + (int)threadIdx.x) * VL + i % VL;
-			const bool ok = !((taken >> i) & 1) && at >= 0 && at < a.vocab && x[i] == x[i];
+			const int at = place(i);
+			const bool ok = !((taken >> i) & 1) && inside(at) && x[i] == x[i];
 			if (ok && beam_better(x[i], at, bv, bi)) {
 				bv = x[i], bi = at;
 			}
@@ -176,45 +317,38 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	if (wave != 0) {
 		return;
 	}
-	// four lists (each sorted) into one: lane l < 4 W holds candidate l
-	float cv[2];
-	int ci[2];
-#pragma unroll
-	for (int j = 0; j < 2; ++j) {
-		const int c = lane + 64 * j;
-		const bool ok = c < 4 * W;
-		cv[j] = ok ? sm_v[(c / W) * BEAM_MAX + c % W] : BEAM_NONE;
-		ci[j] = ok ? sm_i[(c / W) * BEAM_MAX + c % W] : -1;
-		ci[j] = ci[j] < 0 ? 0x7fffffff : ci[j];
-	}
-	for (int k = 0; k < W; ++k) {
-		const bool second = beam_better(cv[1], ci[1], cv[0], ci[0]);
-		float v = second ? cv[1] : cv[0];
-		int i = second ? ci[1] : ci[0];
-		const int mine = i;
-		beam_wave_best(v, i);
-		if (lane == 0) {
-			a.val[part * W + k] = v, a.idx[part * W + k] = i == 0x7fffffff ? -1 : i;
-		}
-		if (mine == i && i != 0x7fffffff) {
-			if (second) {
-				ci[1] = 0x7fffffff, cv[1] = BEAM_NONE;
-			} else {
-				ci[0] = 0x7fffffff, cv[0] = BEAM_NONE;
+	// four lists (each sorted) into one: a candidate's place is its place in its own list plus the better ones of the others
+	for (int c = lane; c < 4 * W; c += 64) {
+		const int w = c / W, k = c % W;
+		const float v = sm_v[w * BEAM_MAX + k];
+		const int at = sm_i[w * BEAM_MAX + k];
+		int rank = k;
+		for (int u = 1; u < 4; ++u) {
+			const int q = ((w + u) & 3) * BEAM_MAX;
+			for (int j = 0; j < W; ++j) {
+				const int other = sm_i[q + j];
+				rank += other >= 0 && beam_better(sm_v[q + j], other, v, at) ? 1 : 0;
 			}
+		}
+		if (at >= 0 && rank < W) {
+			a.val[part * W + rank] = v, a.idx[part * W + rank] = at;
+		}
+	}
+	{ // fewer than W candidates: the places behind them are empty
+		int n = 0;
+		for (int c = lane; c < 4 * W; c += 64) {
+			n += sm_i[(c / W) * BEAM_MAX + c % W] >= 0;
+		}
+#pragma unroll
+		for (int o = 32; o > 0; o >>= 1) {
+			n += __shfl_xor(n, o);
+		}
+		for (int k = n + lane; k < W; k += 64) {
+			a.val[part * W + k] = BEAM_NONE, a.idx[part * W + k] = -1;
 		}
 	}
 	if (lane == 0) {
-		const float M = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-		double s = 0.;
-		for (int w = 0; w < 4; ++w) {
-			if (sm_m[w] != BEAM_NONE) {
-				s += sm_s[w] * exp((double)sm_m[w] - (double)M);
-			} else {
-				s += sm_s[w]; // 0, or NaN
-			}
-		}
-		a.sums[2 * part] = (double)M, a.sums[2 * part + 1] = s;
+		beam_sums(a, part, sm_m, sm_s);
 	}
 }
 
@@ -222,30 +356,33 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 __global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
 	__shared__ double sm_t[BEAM_MAX * BEAM_MAX];
 	__shared__ int sm_i[BEAM_MAX * BEAM_MAX];
+	__shared__ float sm_v[8][BEAM_MAX];
+	__shared__ int sm_j[8][BEAM_MAX];
 	const int lane = lane_id(), wave = wave_id(), W = a.beams, g = blockIdx.x;
 	for (int w = wave; w < W; w += 8) {
 		const int row = g * W + w;
 		const size_t part = (size_t)row * a.n_chunks;
+		const int nc = a.n_chunks * W;
+		float v_n;
+		int at_n;
+		const auto fetch = [&](int c) { // the next portion of candidates, a portion ahead
+			const bool ok = c + lane < nc;
+			v_n = ok ? a.val[part * W + c + lane] : BEAM_NONE;
+			at_n = ok ? a.idx[part * W + c + lane] : -1;
+		};
+		fetch(0);
 		// log of the sum over the chunks, by the same order of additions for every row
-		double M = (double)BEAM_NONE;
+		float top = BEAM_NONE; // (the maxima are fp32 numbers)
 		for (int c = lane; c < a.n_chunks; c += 64) {
-			const double m = a.sums[2 * (part + c)];
-			M = m > M ? m : M;
+			top = fmaxf(top, (float)a.sums[2 * (part + c)]);
 		}
-#pragma unroll
-		for (int o = 32; o > 0; o >>= 1) {
-			const double m = __shfl_xor(M, o);
-			M = m > M ? m : M;
-		}
+		const double M = (double)wave_max_dpp(top);
 		double s = 0.;
 		for (int c = lane; c < a.n_chunks; c += 64) {
 			const double m = a.sums[2 * (part + c)], x = a.sums[2 * (part + c) + 1];
-			s += m == (double)BEAM_NONE ? x : x * exp(m - M);
+			s += m == (double)BEAM_NONE ? x : x * (double)beam_exp((float)(m - M)); // (a difference of fp32 numbers)
 		}
-#pragma unroll
-		for (int o = 32; o > 0; o >>= 1) {
-			s += __shfl_xor(s, o);
-		}
+		s = beam_wave_sum(s);
 		const double lse = M + log(s), base = (double)a.score[row];
 		const bool dead = !(lse - lse == 0.) || !(base > (double)BEAM_NONE); // not finite (NaN included)
 		if (dead) {
@@ -254,74 +391,91 @@ __global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
 			}
 			continue;
 		}
-		// the W best of the chunks' lists: a lane walks the lists lane, lane + 64, ...; each list is sorted, so a lane's best is among
-		// the heads of its lists
-		const int nc = a.n_chunks * W;
-		float last = __builtin_inff();
-		int last_i = -1; // the one chosen before: the next is the best that is not better
-		for (int k = 0; k < W; ++k) {
-			float v = BEAM_NONE;
-			int i = 0x7fffffff;
-			for (int c = lane; c < nc; c += 64) {
-				const float x = a.val[part * W + c];
-				const int j = a.idx[part * W + c];
-				if (j >= 0 && beam_better(last, last_i, x, j) && beam_better(x, j, v, i)) {
-					v = x, i = j;
+		// the W best of the chunks' lists, in portions of 64 candidates: each joins the best so far (one a lane) by counting
+		float bv = BEAM_NONE;
+		int bi = -1;
+		for (int c0 = 0; c0 < nc; c0 += 64) {
+			const float v = v_n;
+			const int at = at_n;
+			fetch(c0 + 64);
+			// only what beats the last of the best so far matters
+			const float wv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bv), W - 1));
+			const int wi = __builtin_amdgcn_readlane(bi, W - 1);
+			bool in = at >= 0 && (wi < 0 || beam_better(v, at, wv, wi));
+			if (wi < 0) { // nothing to beat yet: the portion's W-th largest value
+				float left = in ? v : BEAM_NONE, low = BEAM_NONE;
+				for (int k = 0; k < W; ++k) {
+					low = wave_max_dpp(left);
+					left = lane == __builtin_ctzll(__ballot(left == low)) ? BEAM_NONE : left;
 				}
+				in = in && v >= low;
 			}
-			beam_wave_best(v, i);
-			last = v, last_i = i;
-			if (lane == 0) {
-				sm_t[w * W + k] = i == 0x7fffffff ? (double)BEAM_NONE : base + ((double)v - lse);
-				sm_i[w * W + k] = i == 0x7fffffff ? -1 : i;
+			const unsigned long long who = __ballot(in);
+			if (!who) {
+				continue;
 			}
+			int rank_old = bi >= 0 ? lane : 64, rank_new = 0; // lanes [0, W) hold the best so far in order
+			for (unsigned long long b = who; b; b &= b - 1) {
+				const int l = __builtin_ctzll(b);
+				const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+				const int j = __builtin_amdgcn_readlane(at, l);
+				rank_old += beam_better(x, j, bv, bi) ? 1 : 0;
+				rank_new += beam_better(x, j, v, at) ? 1 : 0;
+			}
+			for (int k = 0; k < W; ++k) {
+				const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bv), k));
+				const int j = __builtin_amdgcn_readlane(bi, k);
+				rank_new += j >= 0 && beam_better(x, j, v, at) ? 1 : 0;
+			}
+			if (bi >= 0 && lane < W && rank_old < W) {
+				sm_v[wave][rank_old] = bv, sm_j[wave][rank_old] = bi;
+			}
+			if (in && rank_new < W) {
+				sm_v[wave][rank_new] = v, sm_j[wave][rank_new] = at;
+			}
+			__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+			__builtin_amdgcn_wave_barrier();
+			const int total = __builtin_popcountll(__ballot(bi >= 0)) + __builtin_popcountll(who);
+			if (lane < W && lane < total) {
+				bv = sm_v[wave][lane], bi = sm_j[wave][lane];
+			}
+			__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+			__builtin_amdgcn_wave_barrier();
+		}
+		if (lane < W) {
+			sm_t[w * W + lane] = bi < 0 ? (double)BEAM_NONE : base + ((double)bv - lse);
+			sm_i[w * W + lane] = bi;
 		}
 	}
 	__syncthreads();
-	if (wave != 0) {
-		return;
-	}
-	double t[BEAM_MAX * BEAM_MAX / 64];
-	int f[BEAM_MAX * BEAM_MAX / 64]; // index in the group's W x W list; ordered by (beam, token) below
-#pragma unroll
-	for (int j = 0; j < BEAM_MAX * BEAM_MAX / 64; ++j) {
-		const int c = lane + 64 * j;
-		const bool ok = c < W * W && sm_i[c] >= 0;
-		t[j] = ok ? sm_t[c] : (double)BEAM_NONE;
-		f[j] = ok ? c : -1;
-	}
-	const auto flat = [&](int c) { // (w, token) as one number that fits: w * vocab + token can pass 32 bits
-		return c < 0 ? 0x7fffffffffffffffll : (long long)(c / W) * a.vocab + sm_i[c];
-	};
-	for (int k = 0; k < W; ++k) {
-		double bt = (double)BEAM_NONE;
-		int bc = -1;
-#pragma unroll
-		for (int j = 0; j < BEAM_MAX * BEAM_MAX / 64; ++j) {
-			if (64 * j < W * W && f[j] >= 0 && (t[j] > bt || (t[j] == bt && flat(f[j]) < flat(bc)))) {
-				bt = t[j], bc = f[j];
+	// A row's list is in order, so a candidate's place in the group is its place in its own list plus, for every other row, how many of that row
+	// are better: found by halving.  Equal totals: the lower row first (its indices are lower), a row's own in its order.
+	for (int c = threadIdx.x; c < W * W; c += 512) {
+		const int w = c / W, k = c % W, at = sm_i[c];
+		if (at < 0) {
+			continue;
+		}
+		const double t = sm_t[c];
+		int rank = k;
+		for (int u = 0; u < W && rank < W; ++u) {
+			if (u == w) {
+				continue;
 			}
-		}
-		long long bf = flat(bc);
-#pragma unroll
-		for (int o = 32; o > 0; o >>= 1) {
-			const double ot = __shfl_xor(bt, o);
-			const int oc = __shfl_xor(bc, o);
-			const long long of = __shfl_xor(bf, o);
-			if (ot > bt || (ot == bt && of < bf)) {
-				bt = ot, bc = oc, bf = of;
+			int lo = 0, hi = W; // entries [0, lo) are better, [hi, W) are not (empty places, at the end, never are)
+			while (lo < hi) {
+				const int mid = (lo + hi) >> 1;
+				const double x = sm_t[u * W + mid];
+				const bool better = sm_i[u * W + mid] >= 0 && (x > t || (x == t && u < w));
+				lo = better ? mid + 1 : lo, hi = better ? hi : mid;
 			}
+			rank += lo;
 		}
-#pragma unroll
-		for (int j = 0; j < BEAM_MAX * BEAM_MAX / 64; ++j) {
-			f[j] = f[j] == bc ? -1 : f[j];
-		}
-		if (lane == 0) {
-			const int w = bc / W, tok = sm_i[bc], row = g * W + w;
-			a.score_out[g * W + k] = (float)bt;
-			a.parent[g * W + k] = w;
-			a.token[g * W + k] = tok;
-			a.done_out[g * W + k] = (a.done && a.done[row]) || (a.eos >= 0 && tok == a.eos) ? 1 : 0;
+		if (rank < W) {
+			const int row = g * W + w, out = g * W + rank;
+			a.score_out[out] = (float)t;
+			a.parent[out] = w;
+			a.token[out] = at;
+			a.done_out[out] = (a.done && a.done[row]) || (a.eos >= 0 && at == a.eos) ? 1 : 0;
 		}
 	}
 }
