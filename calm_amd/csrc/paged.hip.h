@@ -56,22 +56,35 @@ __device__ __forceinline__ void kv_two(unsigned w, float& a, float& b) {
 		a = __builtin_bit_cast(float, w << 16), b = __builtin_bit_cast(float, w & 0xffff0000u);
 	}
 }
+// four values as they are stored
 template <int DT>
-__device__ __forceinline__ void kv_load4(const void* base, size_t at, float (&v)[4]) {
-	if constexpr (DT == KV_F32) {
-		const kv_f32x4 w = *(const kv_f32x4*)((const float*)base + at);
+struct KvQuad {
+	typename std::conditional<DT == KV_F32, u32x4, u32x2>::type w;
+	__device__ __forceinline__ void zero() {
+		w = w ^ w;
+	}
+	__device__ __forceinline__ void load(const void* base, size_t at) {
+		w = *(const decltype(w)*)((const char*)base + at * (DT == KV_F32 ? 4 : 2));
+	}
+	__device__ __forceinline__ void get(float (&v)[4]) const {
+		if constexpr (DT == KV_F32) {
 #pragma unroll
-		for (int i = 0; i < 4; ++i) {
-			v[i] = w[i];
-		}
-	} else {
-		const u32x2 w = *(const u32x2*)((const unsigned short*)base + at);
-#pragma unroll
-		for (int i = 0; i < 2; ++i) {
-			const unsigned two = w[i]; // (a bit_cast of the vector's element itself reads element 0)
-			kv_two<DT>(two, v[2 * i], v[2 * i + 1]);
+			for (int i = 0; i < 4; ++i) {
+				const unsigned one = w[i];
+				v[i] = __builtin_bit_cast(float, one);
+			}
+		} else {
+			const unsigned a = w[0], b = w[1]; // (a bit_cast of a vector's element itself reads element 0)
+			kv_two<DT>(a, v[0], v[1]);
+			kv_two<DT>(b, v[2], v[3]);
 		}
 	}
+};
+template <int DT>
+__device__ __forceinline__ void kv_load4(const void* base, size_t at, float (&v)[4]) {
+	KvQuad<DT> q;
+	q.load(base, at);
+	q.get(v);
 }
 template <int DT>
 __device__ __forceinline__ unsigned short kv_half(float x) { // to nearest even: half a step of the type
@@ -162,13 +175,16 @@ __device__ __forceinline__ void kv_rows_of(const KvRows& r, int s, int& row0, in
 	len = len < 0 ? 0 : len;
 }
 
-// One workgroup quantises what a call adds to one page and kv head, wave w the page's block w: rows in, the largest magnitude of the
-// block's new values, the scale, codes out.  Bytes bound it (a token's rows once in, a quarter or half of them out); a lane takes four
-// tokens x four dims, so K goes out as a dword per token and V as a dword per dim without crossing lanes.
+// One workgroup quantises what a call adds to one page and kv head, wave w the page's block w: rows in (K's and V's at once), the largest
+// magnitude of the block's new values, the scale, codes out.  Bytes bound it (a token's rows once in, a quarter or half of them out); a lane
+// takes four tokens x four dims, so K goes out as a dword per token and V as a dword per dim without crossing lanes.  Where all four blocks
+// get new tokens (a prompt's pages) V's dwords meet in LDS and go out as whole lines: four bytes every sixteen cost 5 of 48 us for the
+// 15k tokens of six prompts, 8 heads of 128.
 // grid = (pages touched at most, kv heads)
 template <int D, int DT>
-__global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
+__global__ __launch_bounds__(256, DT == KV_F32 || D > 128 ? 1 : D == 96 ? 7 : 8) void k_kv_append(KvAppendArgs a) {
 	constexpr int NI = (D + 63) / 64; // items (quad of tokens, four dims) per lane: 4 x D / 4 over 64 lanes
+	__shared__ u32x4 sm_v[4 * D];     // [quad][dim] x the four blocks' dwords, turned by dim / 4 (lanes four dims apart would meet in four banks)
 	const int lane = lane_id(), blk = wave_id(), h = blockIdx.y;
 	int s, at;
 	const KvRows& r = a.r;
@@ -187,7 +203,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
 		row0 += n - len, n = len;
 	}
 	const int before = len - n;
-	const int pg = before / KV_PAGE + at;
+	const int pg = before / KV_PAGE + at, p0 = pg * KV_PAGE;
 	const int pid = pg < r.max_pages ? r.table[(size_t)s * r.max_pages + pg] : -1;
 	if (pid < 0 || pid >= a.p.n_pages) {
 		if (threadIdx.x == 0 && h == 0) {
@@ -195,93 +211,128 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
 		}
 		return;
 	}
-	const int b0 = pg * KV_PAGE + blk * KV_BLOCK; // first position of the block
+	const bool all = before < p0 + KV_BLOCK && len > p0 + 3 * KV_BLOCK; // every block of the page gets new tokens
+	const int b0 = p0 + blk * KV_BLOCK; // first position of the block
 	const int lo = before > b0 ? before - b0 : 0, hi = len - b0 < KV_BLOCK ? len - b0 : KV_BLOCK; // its new tokens
 	if (lo >= hi) {
-		return;
+		return; // (not where `all`)
 	}
 	const size_t page = (size_t)pid * a.p.n_kv_heads + h;
 	signed char* const kp = a.p.k + page * (KV_PAGE * D) + blk * KV_BLOCK * D;
 	unsigned* const vp = (unsigned*)(a.p.v + page * (KV_PAGE * D)) + blk; // + (quad * D + dim) * 4
+	KvQuad<DT> x[2][NI][4]; // [K, V][item][token], four dims each
 #pragma unroll
 	for (int kv = 0; kv < 2; ++kv) {
-		const void* const src = kv ? a.v : a.k;
-		const size_t src0 = (size_t)(row0 + b0 + lo - before) * (size_t)(kv ? a.v_row : a.k_row) + (size_t)h * (size_t)(kv ? a.v_head : a.k_head);
-		float x[NI][4][4]; // [item][token][dim]
-		unsigned top = 0;
+		const long row = kv ? a.v_row : a.k_row;
+		const size_t src0 = (size_t)(row0 + b0 + lo - before) * (size_t)row + (size_t)h * (size_t)(kv ? a.v_head : a.k_head);
 #pragma unroll
 		for (int i = 0; i < NI; ++i) {
 			const int it = lane + 64 * i, g = it / (D / 4), d = it % (D / 4) * 4;
 #pragma unroll
 			for (int t = 0; t < 4; ++t) {
-				x[i][t][0] = x[i][t][1] = x[i][t][2] = x[i][t][3] = 0.f;
+				x[kv][i][t].zero();
 				if (it < D && 4 * g + t >= lo && 4 * g + t < hi) {
-					kv_load4<DT>(src, src0 + (size_t)(4 * g + t - lo) * (size_t)(kv ? a.v_row : a.k_row) + d, x[i][t]);
-				}
-#pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					const unsigned m = __builtin_bit_cast(unsigned, x[i][t][e]) & 0x7fffffffu;
-					top = top > m ? top : m;
+					x[kv][i][t].load(kv ? a.v : a.k, src0 + (size_t)(4 * g + t - lo) * (size_t)row + d);
 				}
 			}
 		}
+	}
 #pragma unroll
-		for (int o = 32; o > 0; o >>= 1) {
-			const unsigned m = __shfl_xor(top, o);
-			top = top > m ? top : m;
+	for (int kv = 0; kv < 2; ++kv) {
+		float big = 0.f, odd = 0.f; // odd: NaN once an infinity or a NaN came by (fmaxf passes over a NaN)
+#pragma unroll
+		for (int i = 0; i < NI; ++i) {
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				float y[4];
+				x[kv][i][t].get(y);
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					big = fmaxf(big, fabsf(y[e]));
+					odd = __builtin_fmaf(y[e], 0.f, odd);
+				}
+			}
 		}
+		const bool wild = __ballot(odd != 0.f) != 0;
+		const unsigned top = __builtin_bit_cast(unsigned, wave_max_dpp(big));
 		float* const sp = (kv ? a.p.vs : a.p.ks) + page * 4 + blk;
 		const unsigned was = lo > 0 ? __builtin_bit_cast(unsigned, *sp) & 0x7fffffffu : 0;
-		const bool poison = top >= 0x7f800000u || was >= 0x7f800000u;
-		int e = top >= 0x7f800000u ? -126 : kv_scale_exp(top);
+		const bool poison = wild || was >= 0x7f800000u;
+		int e = wild ? -126 : kv_scale_exp(top);
 		const int e_was = was >= 0x00800000u && was < 0x7f800000u ? (int)(was >> 23) - 127 : -126;
 		e = e > e_was ? e : e_was; // (no old tokens: e_was is the least there is)
-		// 2^-e; e <= 122
-		const float inv = kv_exp2i(-e);
+		// A code is the low byte of 1.5 * 2^23 + x 2^-e: the product is exact, the one rounding of the sum is to a whole number, to even; e <= 122.
+		// (A poisoned block's codes are 0: 0 * x would not be.)
+		const float inv = poison ? 0.f : kv_exp2i(-e);
 		const bool shift = lo > 0 && e > e_was;
 		const float shrink = shift ? kv_exp2i(e_was - e < -126 ? -126 : e_was - e) : 1.f;
 #pragma unroll
 		for (int i = 0; i < NI; ++i) {
 			const int it = lane + 64 * i, g = it / (D / 4), d = it % (D / 4) * 4;
-			if (it >= D || 4 * g >= hi || (4 * g + 3 < lo && !shift)) {
+			const bool changes = 4 * g < hi && (4 * g + 3 >= lo || shift);
+			if (it >= D || (!changes && !(kv && all))) {
 				continue; // nothing of this quad changes
+			}
+			unsigned code[4][4]; // [token][dim], in the low byte
+#pragma unroll
+			for (int t = 0; t < 4; ++t) {
+				float y[4];
+				x[kv][i][t].get(y);
+#pragma unroll
+				for (int c = 0; c < 4; ++c) {
+					code[t][c] = __builtin_bit_cast(unsigned, __builtin_fmaf(poison ? 0.f : y[c], inv, 12582912.f));
+				}
 			}
 			unsigned out[4]; // K: a token's four dims; V: a dim's four tokens
 #pragma unroll
 			for (int j = 0; j < 4; ++j) {
-				out[j] = 0;
-				if (kv ? 4 * g < lo : 4 * g + j < lo) { // old tokens among them
-					out[j] = kv ? vp[(size_t)(g * D + d + j) * 4] : *(const unsigned*)(kp + (4 * g + j) * D + d);
-				}
+				const unsigned c0 = kv ? code[0][j] : code[j][0], c1 = kv ? code[1][j] : code[j][1], c2 = kv ? code[2][j] : code[j][2], c3 = kv ? code[3][j] : code[j][3];
+				out[j] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c3, c2, 0x0c0c0400u), __builtin_amdgcn_perm(c1, c0, 0x0c0c0400u), 0x05040100u);
 			}
+			if (4 * g < lo) { // old tokens among them
 #pragma unroll
-			for (int t = 0; t < 4; ++t) {
-				const bool fresh = 4 * g + t >= lo;
+				for (int j = 0; j < 4; ++j) {
+					unsigned old = kv ? vp[(size_t)(g * D + d + j) * 4] : 4 * g + j < lo ? *(const unsigned*)(kp + (4 * g + j) * D + d) : 0;
+					if (shift) {
+						unsigned w = 0;
 #pragma unroll
-				for (int c = 0; c < 4; ++c) {
-					unsigned& w = out[kv ? c : t];
-					const int sh = 8 * (kv ? t : c);
-					if (fresh) {
-						const float y = poison ? 0.f : x[i][t][c] * inv; // exact but where it underflows, to zero
-						w = (w & ~(0xffu << sh)) | (((unsigned)(int)__builtin_rintf(y) & 0xffu) << sh);
-					} else if (shift) {
-						const int old = (int)(signed char)(w >> sh);
-						w = (w & ~(0xffu << sh)) | (((unsigned)(int)__builtin_rintf((float)old * shrink) & 0xffu) << sh);
+						for (int c = 0; c < 4; ++c) {
+							w |= ((unsigned)(int)__builtin_rintf((float)(int)(signed char)(old >> (8 * c)) * shrink) & 0xffu) << (8 * c);
+						}
+						old = w;
 					}
+					const int olds = lo - 4 * g < 4 ? lo - 4 * g : 4; // V: this many of the dword's bytes
+					const unsigned keep = kv ? (olds >= 4 ? ~0u : (1u << (8 * olds)) - 1) : 4 * g + j < lo ? ~0u : 0u;
+					out[j] = (out[j] & ~keep) | (old & keep);
 				}
 			}
 #pragma unroll
 			for (int j = 0; j < 4; ++j) {
-				if (kv) {
+				if (!kv) {
+					if (4 * g + j < hi && (4 * g + j >= lo || shift)) {
+						*(unsigned*)(kp + (4 * g + j) * D + d) = out[j];
+					}
+				} else if (all) {
+					((unsigned*)sm_v)[(g * D + d + j) * 4 + ((blk + (d >> 2)) & 3)] = out[j];
+				} else {
 					vp[(size_t)(g * D + d + j) * 4] = out[j];
-				} else if (4 * g + j < hi && (4 * g + j >= lo || shift)) {
-					*(unsigned*)(kp + (4 * g + j) * D + d) = out[j];
 				}
 			}
 		}
 		if (lane == 0) {
 			*(unsigned*)sp = poison ? 0x7fc00000u : __builtin_bit_cast(unsigned, kv_exp2i(e));
 		}
+	}
+	if (!all) {
+		return;
+	}
+	__syncthreads();
+	u32x4* const dst = (u32x4*)(a.p.v + page * (KV_PAGE * D));
+	for (int it = threadIdx.x; it < 4 * D; it += 256) {
+		const u32x4 w = sm_v[it];
+		const int turn = (it % D) >> 2; // word (blk + turn) & 3 is block blk's
+		const u32x4 y = turn & 1 ? (u32x4){w[1], w[2], w[3], w[0]} : w;
+		dst[it] = turn & 2 ? (u32x4){y[2], y[3], y[0], y[1]} : y;
 	}
 }
 
@@ -1218,7 +1269,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 // atomics only, so results do not depend on their order; the page bytes move in a launch of their own.
 
 constexpr int KV_BOOK = 1024;     // threads of the bookkeeping workgroup
-constexpr int KV_MAX_ROWS = 4096; // rows of a table the bookkeeping holds in LDS
+constexpr int KV_MAX_ROWS = 2048; // rows of a table the bookkeeping holds in LDS
 
 // exclusive sum of one int per thread over the workgroup, and the total; `sm`: 17 ints
 __device__ __forceinline__ int kv_block_scan(int v, int* sm, int& total) {
@@ -1281,86 +1332,83 @@ struct KvForkArgs {
 	int n_rows, max_pages, n_pages;
 };
 
+// (its time is round trips to memory, one behind another: parents and lengths are kept in LDS, and what does not depend on the new counts --
+// the shared part of the new table, who needs a page -- is done beside them: 13.2 -> 11.8 us for 48 rows of 19 pages)
 __global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
-	__shared__ int first[KV_MAX_ROWS], count[KV_MAX_ROWS], list[KV_MAX_ROWS], sm[KV_BOOK / 64];
+	__shared__ int first[KV_MAX_ROWS], count[KV_MAX_ROWS], list[KV_MAX_ROWS], par[KV_MAX_ROWS], len[KV_MAX_ROWS], sm[KV_BOOK / 64];
 	const int tid = threadIdx.x, n = a.n_rows, mp = a.max_pages;
 	for (int i = tid; i < n; i += KV_BOOK) {
+		const int p = a.parents[i], l = a.lens[i];
 		first[i] = n, count[i] = 0;
+		par[i] = p >= 0 && p < n ? p : -1, len[i] = l < 0 ? 0 : l;
+		if (par[i] < 0) {
+			kv_flag(a.status, KV_BAD_PARENT);
+		}
 	}
 	for (int p = tid; p < a.n_pages; p += KV_BOOK) {
 		a.refs_out[p] = a.refs[p];
 	}
 	__syncthreads();
 	for (int i = tid; i < n; i += KV_BOOK) {
-		const int par = a.parents[i];
-		if (par >= 0 && par < n) {
-			atomicMin(&first[par], i);
-			atomicAdd(&count[par], 1);
-		} else {
-			kv_flag(a.status, KV_BAD_PARENT);
+		if (par[i] >= 0) {
+			atomicMin(&first[par[i]], i);
+			atomicAdd(&count[par[i]], 1);
 		}
 	}
 	__threadfence();
 	__syncthreads();
-	// counts: a full page of row r is listed by count[r] rows from now on, a page of its own by one of them at most
 	for (int k = tid; k < n * mp; k += KV_BOOK) {
+		// counts: a full page of row r is listed by count[r] rows from now on, a page of its own by one of them at most
 		const int r = k / mp, c = k - r * mp;
-		const int kids = count[r], full = a.lens[r] / KV_PAGE;
-		const int d = (c < full ? kids : (kids > 0 ? 1 : 0)) - 1;
-		const int p = d ? a.table[k] : -1;
-		if (d && p >= 0) {
-			if (p < a.n_pages) {
-				atomicAdd(&a.refs_out[p], d);
+		const int d = (c < len[r] / KV_PAGE ? count[r] : (count[r] > 0 ? 1 : 0)) - 1;
+		const int old = d ? a.table[k] : -1;
+		// the new row: all of its parent's for a first child, the full pages for the others
+		int p = -1;
+		if (par[r] >= 0 && (first[par[r]] == r || c < len[par[r]] / KV_PAGE)) {
+			p = a.table[par[r] * mp + c];
+		}
+		a.table_out[k] = p;
+		if (old >= 0) {
+			if (old < a.n_pages) {
+				atomicAdd(&a.refs_out[old], d);
 			} else {
 				kv_flag(a.status, KV_BAD_PAGE);
 			}
 		}
 	}
-	__threadfence();
-	__syncthreads();
 	// rows that need a page of their own: not the first child, the parent's last page not full
 	int want = 0;
 	for (int i0 = 0; i0 < n; i0 += KV_BOOK) {
 		const int i = i0 + tid;
-		int need = 0;
-		if (i < n) {
-			const int par = a.parents[i];
-			if (par >= 0 && par < n && first[par] != i) {
-				const int len = a.lens[par], c = len / KV_PAGE;
-				const int p = len > 0 && len % KV_PAGE && c < mp ? a.table[par * mp + c] : -1;
-				need = p >= 0 && p < a.n_pages;
-			}
+		int from = -1;
+		if (i < n && par[i] >= 0 && first[par[i]] != i) {
+			const int l = len[par[i]], c = l / KV_PAGE;
+			from = l % KV_PAGE && c < mp ? a.table[par[i] * mp + c] : -1;
+			from = from < a.n_pages ? from : -1;
 		}
 		int total;
-		const int at = want + kv_block_scan(need, sm, total);
+		const int at = want + kv_block_scan(from >= 0, sm, total);
 		if (i < n) {
-			a.copy[2 * i] = need ? at : -1; // (its number, until the pages are known)
+			a.copy[2 * i] = from;
+			count[i] = from >= 0 ? at : -1; // (every thread is through with count: the scan's barriers)
 		}
 		want += total;
 	}
+	__threadfence();
+	__syncthreads();
 	const int have = kv_free_pages(a.refs_out, a.n_pages, want, list, sm);
 	if (have < want && tid == 0) {
 		kv_flag(a.status, KV_NO_PAGE);
 	}
-	for (int k = tid; k < n * mp; k += KV_BOOK) {
-		const int i = k / mp, c = k - i * mp, par = a.parents[i];
-		int p = -1;
-		if (par >= 0 && par < n && (first[par] == i || c < a.lens[par] / KV_PAGE)) {
-			p = a.table[par * mp + c];
-		}
-		a.table_out[k] = p;
-	}
-	__syncthreads();
 	for (int i = tid; i < n; i += KV_BOOK) {
-		const int at = a.copy[2 * i];
-		int from = -1, to = -1;
+		const int at = count[i];
+		int to = -1;
 		if (at >= 0 && at < have) {
-			const int par = a.parents[i], c = a.lens[par] / KV_PAGE;
-			from = a.table[par * mp + c], to = list[at];
-			a.table_out[i * mp + c] = to;
+			to = list[at];
+			a.table_out[i * mp + len[par[i]] / KV_PAGE] = to;
 			a.refs_out[to] = 1;
 		}
-		a.copy[2 * i] = from, a.copy[2 * i + 1] = to;
+		a.copy[2 * i + 1] = to;
 	}
 }
 

@@ -339,7 +339,7 @@ static const char* kv_table_fault(const struct KvPool* pool, const int* table, c
 		return "table, lengths or counts are missing";
 	}
 	if (n_rows < 1 || n_rows > KV_MAX_ROWS || max_pages < 1 || (long long)n_rows * max_pages > 0x7fffffffll) {
-		return "1 to 4096 table rows, at least one page column, less than 2^31 entries";
+		return "1 to 2048 table rows, at least one page column, less than 2^31 entries";
 	}
 	return nullptr;
 }

@@ -16,6 +16,7 @@ torch has to be imported before the library is loaded in a process that uses bot
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import sys
 from typing import Optional
@@ -114,6 +115,7 @@ def _name(x) -> str:
     return n
 
 
+_nothing = contextlib.nullcontext()
 _torch = None  # torch and the functions that every call asks, once it is known to be there
 
 
@@ -127,45 +129,39 @@ def _torch_calls():
     return _torch
 
 
-class _On:
-    """the device and stream of a call's arrays: the device is current inside, `stream` is a hipStream_t"""
-
-    __slots__ = ("stream", "_guard")
-
-    def __init__(self, arrays):
-        first = arrays[0]
-        self._guard = None
-        if isinstance(first, DeviceArray):
-            for a in arrays:
-                if not isinstance(a, DeviceArray):
-                    raise ValueError("tensors and DeviceArrays in one call")
-            self.stream = _lib().calm_hip_stream()
-            return
-        torch, tensor, raw_stream, current = _torch or _torch_calls()
-        dev = first.device
-        if dev.type != "cuda":
-            raise ValueError(f"arrays on {dev}: these operators run on the GPU only")
-        grads = torch.is_grad_enabled()
+def _on(arrays):
+    """(stream, guard) of a call's arrays: a hipStream_t, and None or a context that makes their device current"""
+    first = arrays[0]
+    if isinstance(first, DeviceArray):
         for a in arrays:
-            if not isinstance(a, tensor):
+            if not isinstance(a, DeviceArray):
                 raise ValueError("tensors and DeviceArrays in one call")
-            if a.device != dev:
-                raise ValueError(f"arrays on {dev} and on {a.device} in one call")
-            if grads and a.requires_grad:
-                raise ValueError("there is no backward pass: call under torch.no_grad()")
-        index = dev.index
-        if index != current():
-            self._guard = torch.cuda.device(dev)
-        self.stream = raw_stream(index)
+        return _lib().calm_hip_stream(), None
+    torch, tensor, raw_stream, current = _torch or _torch_calls()
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError(f"arrays on {dev}: these operators run on the GPU only")
+    grads = torch.is_grad_enabled()
+    for a in arrays:
+        if not isinstance(a, tensor):
+            raise ValueError("tensors and DeviceArrays in one call")
+        if a.device != dev:
+            raise ValueError(f"arrays on {dev} and on {a.device} in one call")
+        if grads and a.requires_grad:
+            raise ValueError("there is no backward pass: call under torch.no_grad()")
+    index = dev.index
+    return raw_stream(index), None if index == current() else torch.cuda.device(dev)
 
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return self.stream
 
-    def __exit__(self, *e):
-        if self._guard is not None:
-            self._guard.__exit__(*e)
+def _call(guard, entry, *args) -> None:
+    """the C entry, on the arrays' device; ValueError if it refuses"""
+    if guard is None:
+        rc = entry(*args)
+    else:
+        with guard:
+            rc = entry(*args)
+    if rc:
+        raise ValueError(_lib().calm_hip_error().decode())
 
 
 def _empty(like, shape, dtype: str):
@@ -204,11 +200,6 @@ def _rows(x, name: str, rows: int, heads: Optional[int], dim: int):
     if r % 4 or h % 4:
         raise ValueError(f"{name}: row and head strides {r}, {h} are not multiples of four elements")
     return r, h
-
-
-def _called(rc: int) -> None:
-    if rc != 0:
-        raise ValueError(_lib().calm_hip_error().decode())
 
 
 class KvPool:
@@ -290,6 +281,7 @@ class KvBatch:
         self.n_seqs, self.rows, self.max_rows, self.max_len = n, rows, max_rows, max_len
         self._c = _Batch(table.data_ptr(), lens.data_ptr(), starts.data_ptr(), n, mp, rows, max_rows, max_len)
         self._ref = C.byref(self._c)
+        self._work = {}  # workspace sizes of attention
 
 
 def append(pool: KvPool, batch: KvBatch, k, v, layer: int = 0) -> None:
@@ -297,8 +289,8 @@ def append(pool: KvPool, batch: KvBatch, k, v, layer: int = 0) -> None:
     kr, kh = _rows(k, "k", batch.rows, pool.n_kv_heads, pool.head_dim)
     vr, vh = _rows(v, "v", batch.rows, pool.n_kv_heads, pool.head_dim)
     _need(_name(k) == _name(v), "k and v of different types")
-    with _On((k, v, pool.k, batch.table)) as stream:
-        _called(_lib().kv_append_hip(pool._ref, batch._ref, layer, k.data_ptr(), v.data_ptr(), _TYPES[_name(k)], kr, kh, vr, vh, stream))
+    stream, guard = _on((k, v, pool.k, batch.table))
+    _call(guard, _lib().kv_append_hip, pool._ref, batch._ref, layer, k.data_ptr(), v.data_ptr(), _TYPES[_name(k)], kr, kh, vr, vh, stream)
 
 
 def attend(pool: KvPool, batch: KvBatch, q, layer: int = 0, window: int = 0, sinks: int = 0, scale: Optional[float] = None, out=None):
@@ -311,14 +303,20 @@ def attend(pool: KvPool, batch: KvBatch, q, layer: int = 0, window: int = 0, sin
         out = _empty(q, (int(q.shape[0]), heads, dim), _name(q))
     else:
         _array(out, "out", (_name(q),), tuple(q.shape))
-    lib = _lib()
-    with _On((q, out, pool.k, batch.table)) as stream:
-        need = lib.kv_attend_workspace_hip(pool._ref, batch._ref, _TYPES[_name(q)], heads, window, sinks)
+    lib, kind = _lib(), _TYPES[_name(q)]
+    stream, guard = _on((q, out, pool.k, batch.table))
+    # (the workspace's size follows from shapes and bounds alone)
+    key = (kind, heads, window, sinks, pool.n_kv_heads, dim)
+    need = batch._work.get(key)
+    if need is None:
+        with guard or _nothing:
+            need = lib.kv_attend_workspace_hip(pool._ref, batch._ref, kind, heads, window, sinks)
         if need < 0:
-            _called(-1)
-        work = _empty(q, (need // 4,), "float32") if need else None
-        _called(lib.kv_attend_hip(pool._ref, batch._ref, layer, q.data_ptr(), out.data_ptr(), _TYPES[_name(q)], heads, qr, qh, dim ** -0.5 if scale is None else scale,
-                                  window, sinks, work.data_ptr() if need else None, need, stream))
+            raise ValueError(lib.calm_hip_error().decode())
+        batch._work[key] = need
+    work = _empty(q, (need // 4,), "float32") if need else None
+    _call(guard, lib.kv_attend_hip, pool._ref, batch._ref, layer, q.data_ptr(), out.data_ptr(), kind, heads, qr, qh, dim ** -0.5 if scale is None else scale, window, sinks,
+          work.data_ptr() if need else None, need, stream)
     return out
 
 
@@ -330,9 +328,9 @@ def read(pool: KvPool, table, lens, start, count: int, layer: int = 0, dtype: st
     _array(start, "start", ("int32",), (n,))
     _need(dtype in _TYPES, f"{dtype} where float32, float16 or bfloat16 is wanted")
     _need(count >= 0, "a negative count")
-    with _On((pool.k, table, lens, start)) as stream:
-        k, v = (_empty(pool.k, (n, count, pool.n_kv_heads, pool.head_dim), dtype) for _ in range(2))
-        _called(_lib().kv_read_hip(pool._ref, layer, table.data_ptr(), lens.data_ptr(), start.data_ptr(), n, mp, count, k.data_ptr(), v.data_ptr(), _TYPES[dtype], stream))
+    stream, guard = _on((pool.k, table, lens, start))
+    k, v = (_empty(pool.k, (n, count, pool.n_kv_heads, pool.head_dim), dtype) for _ in range(2))
+    _call(guard, _lib().kv_read_hip, pool._ref, layer, table.data_ptr(), lens.data_ptr(), start.data_ptr(), n, mp, count, k.data_ptr(), v.data_ptr(), _TYPES[dtype], stream)
     return k, v
 
 
@@ -347,16 +345,16 @@ def reserve(pool: KvPool, table, refs, lens, lens_new) -> None:
     n, mp = _table(pool, table, refs)
     _array(lens, "lens", ("int32",), (n,))
     _array(lens_new, "lens_new", ("int32",), (n,))
-    with _On((table, refs, lens, lens_new, pool.k)) as stream:
-        _called(_lib().kv_reserve_hip(pool._ref, table.data_ptr(), refs.data_ptr(), lens.data_ptr(), lens_new.data_ptr(), n, mp, stream))
+    stream, guard = _on((table, refs, lens, lens_new, pool.k))
+    _call(guard, _lib().kv_reserve_hip, pool._ref, table.data_ptr(), refs.data_ptr(), lens.data_ptr(), lens_new.data_ptr(), n, mp, stream)
 
 
 def trim(pool: KvPool, table, refs, lens, window: int = 0, sinks: int = 0) -> None:
     """gives up, in place, the pages behind lens[r] (0: the whole row) and, with a window > 0, those that no later token of the row sees"""
     n, mp = _table(pool, table, refs)
     _array(lens, "lens", ("int32",), (n,))
-    with _On((table, refs, lens, pool.k)) as stream:
-        _called(_lib().kv_trim_hip(pool._ref, table.data_ptr(), refs.data_ptr(), lens.data_ptr(), n, mp, window, sinks, stream))
+    stream, guard = _on((table, refs, lens, pool.k))
+    _call(guard, _lib().kv_trim_hip, pool._ref, table.data_ptr(), refs.data_ptr(), lens.data_ptr(), n, mp, window, sinks, stream)
 
 
 def fork(pool: KvPool, table, lens, refs, parents):
@@ -365,21 +363,21 @@ def fork(pool: KvPool, table, lens, refs, parents):
     n, mp = _table(pool, table, refs)
     _array(lens, "lens", ("int32",), (n,))
     _array(parents, "parents", ("int32",), (n,))
-    with _On((table, refs, lens, parents, pool.k)) as stream:
-        new, now, work = _empty(table, (n, mp), "int32"), _empty(table, (pool.n_pages,), "int32"), _empty(table, (2 * n,), "int32")
-        _called(_lib().kv_fork_hip(pool._ref, table.data_ptr(), lens.data_ptr(), refs.data_ptr(), parents.data_ptr(), n, mp, new.data_ptr(), now.data_ptr(),
-                                   work.data_ptr(), 8 * n, stream))
+    stream, guard = _on((table, refs, lens, parents, pool.k))
+    new, now, work = _empty(table, (n, mp), "int32"), _empty(table, (pool.n_pages,), "int32"), _empty(table, (2 * n,), "int32")
+    _call(guard, _lib().kv_fork_hip, pool._ref, table.data_ptr(), lens.data_ptr(), refs.data_ptr(), parents.data_ptr(), n, mp, new.data_ptr(), now.data_ptr(),
+          work.data_ptr(), 8 * n, stream)
     return new, now
 
 
 def compact(pool: KvPool, table, refs):
     """(table, refs, number of live pages) after the live pages at or behind that number have moved into the free ones before it"""
     n, mp = _table(pool, table, refs)
-    with _On((table, refs, pool.k)) as stream:
-        new, now, live = _empty(table, (n, mp), "int32"), _empty(table, (pool.n_pages,), "int32"), _empty(table, (1,), "int32")
-        work = _empty(table, (2 * pool.n_pages,), "int32")
-        _called(_lib().kv_compact_hip(pool._ref, table.data_ptr(), refs.data_ptr(), n, mp, new.data_ptr(), now.data_ptr(), live.data_ptr(), work.data_ptr(),
-                                      8 * pool.n_pages, stream))
+    stream, guard = _on((table, refs, pool.k))
+    new, now, live = _empty(table, (n, mp), "int32"), _empty(table, (pool.n_pages,), "int32"), _empty(table, (1,), "int32")
+    work = _empty(table, (2 * pool.n_pages,), "int32")
+    _call(guard, _lib().kv_compact_hip, pool._ref, table.data_ptr(), refs.data_ptr(), n, mp, new.data_ptr(), now.data_ptr(), live.data_ptr(), work.data_ptr(),
+          8 * pool.n_pages, stream)
     return new, now, live
 
 
@@ -400,13 +398,12 @@ def beam_select(logits, scores, done=None, eos: int = -1):
         _array(done, "done", ("uint8", "bool"), (groups, beams))
         arrays.append(done)
     lib = _lib()
-    with _On(arrays) as stream:
-        need = lib.beam_workspace_hip(groups, beams, vocab)
-        if need < 0:
-            _called(-1)
-        best, parents, tokens, ended = (_empty(scores, (groups, beams), d) for d in ("float32", "int32", "int32", "uint8"))
-        work = _empty(scores, (-(-need // 4),), "float32")
-        _called(lib.beam_select_hip(logits.data_ptr(), _TYPES[_name(logits)], row if groups * beams > 1 else max(row, vocab), groups, beams, vocab, scores.data_ptr(),
-                                    done.data_ptr() if done is not None else None, eos, best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ended.data_ptr(),
-                                    work.data_ptr(), need, stream))
+    stream, guard = _on(arrays)
+    need = lib.beam_workspace_hip(groups, beams, vocab)
+    if need < 0:
+        raise ValueError(lib.calm_hip_error().decode())
+    best, parents, tokens, ended = (_empty(scores, (groups, beams), d) for d in ("float32", "int32", "int32", "uint8"))
+    work = _empty(scores, (-(-need // 4),), "float32")
+    _call(guard, lib.beam_select_hip, logits.data_ptr(), _TYPES[_name(logits)], row if groups * beams > 1 else max(row, vocab), groups, beams, vocab, scores.data_ptr(),
+          done.data_ptr() if done is not None else None, eos, best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ended.data_ptr(), work.data_ptr(), need, stream)
     return best, parents, tokens, ended

@@ -270,7 +270,7 @@ int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* batch, int la
                   int sinks, void* workspace, size_t workspace_size, void* stream);
 
 /* The upkeep of pages.  refs[p] = how many table rows list page p (int [n_pages], 0: free); a page that is not full belongs to one row.
- * Up to 4096 table rows.  Free pages are taken lowest first, rows in order.
+ * Up to 2048 table rows.  Free pages are taken lowest first, rows in order.
  *   reserve  entries of the pages that tokens lens[r] .. lens_new[r] - 1 of row r need (in place)
  *   trim     gives up pages behind lens[r] (0: all of them) and, with a window > 0, those that no later token sees (in place)
  *   fork     row r becomes a copy of row parents[r] (out of place: table_out, refs_out; refs_out may be refs): full pages are shared, a

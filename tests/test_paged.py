@@ -809,7 +809,7 @@ def test_entries_refuse_bad_arguments(hiplib):
     refused(hiplib.kv_read_hip(P, 0, 4096, 0, 4096, 2, 4, 1, 4096, 4096, 0, None), hiplib, "missing")
     refused(hiplib.kv_read_hip(P, 0, 4096, 4096, 4096, 2, 4, 1, 4098, 4096, 1, None), hiplib, "aligned")
     refused(hiplib.kv_reserve_hip(P, 4096, 4096, 4096, None, 2, 4, None), hiplib, "missing")
-    refused(hiplib.kv_reserve_hip(P, 4096, 4096, 4096, 4096, 5000, 4, None), hiplib, "4096 table rows")
+    refused(hiplib.kv_reserve_hip(P, 4096, 4096, 4096, 4096, 5000, 4, None), hiplib, "2048 table rows")
     refused(hiplib.kv_trim_hip(P, 4096, 4096, 4096, 2, 4, -1, 0, None), hiplib, "negative")
     refused(hiplib.kv_fork_hip(P, 4096, 4096, 4096, 4096, 2, 4, 4096, 8192, 4096, 64, None), hiplib, "beside")
     refused(hiplib.kv_fork_hip(P, 4096, 4096, 4096, 4096, 2, 4, 8192, 8192, 4096, 15, None), hiplib, "workspace")
