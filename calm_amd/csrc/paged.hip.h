@@ -486,62 +486,53 @@ __device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t 
 	}
 }
 
-// Few rows (one token of a sequence, or a few): the cache's bytes bound it.  A workgroup takes one sequence, one kv head, 16 x NR rows
-// (token x head of the group) and a range of pages, dealt to its four waves a page at a time; a wave holds a page's codes in registers as
+// Few rows (one token of a sequence, or a few): the cache's bytes bound it.  A workgroup takes one sequence, one kv head, 16 rows (token x head
+// of the group) and a range of pages, dealt to its NW waves a page at a time; a wave holds a page's codes in registers as
 // the matrix operands they are, loads the next page's K behind the first product and its V behind the second, so 8 - 16 KiB per wave
 // are in flight throughout.  The waves' sums meet in LDS; ranges of one row meet in k_kv_merge.
 // grid = (splits, kv heads x tiles, seqs)
-template <int D, int DT, int NR>
-__global__ __launch_bounds__(256, NR * D <= 128 ? 2 : 1) void k_kv_decode(KvAttnArgs a) {
+template <int D, int DT, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnArgs a) {
 	constexpr int ND = D / 16;  // dim tiles of O^T
 	constexpr int KW = D / 16;  // dwords of a K row per lane
 	constexpr bool HL = DT == KV_F32;
-	extern __shared__ float kv_lds[]; // [wave][NR x 16 rows][D + 4]
+	extern __shared__ float kv_lds[]; // [wave][16 rows][D + 4]
 	const int lane = lane_id(), wave = wave_id();
 	const int col = lane & 15, g = lane >> 4;
 	const int H = a.p.n_kv_heads, h = blockIdx.y % H, tile = blockIdx.y / H, s = blockIdx.z, split = blockIdx.x;
 	int row0, n, len;
 	kv_rows_of(a.r, s, row0, n, len);
-	const int nrows = n * a.group, r0 = tile * 16 * NR;
+	const int nrows = n * a.group, r0 = tile * 16;
 	if (threadIdx.x == 0 && tile == 0 && h == 0 && split == 0 && n > a.r.max_rows) {
 		kv_flag(a.p.status, KV_BAD_BATCH);
 	}
 	if (r0 >= nrows) {
 		return;
 	}
-	const int rl = r0 + 16 * NR - 1 < nrows - 1 ? r0 + 16 * NR - 1 : nrows - 1;
+	const int rl = r0 + 15 < nrows - 1 ? r0 + 15 : nrows - 1;
 	const int p_min = len - n + r0 / a.group, p_max = len - n + rl / a.group;
 	const KvSpan sp(p_min, p_max, a.window, a.sinks);
 	const bool direct = sp.np <= a.chunk;
 	const int i0 = split * a.chunk, i1 = (split + 1) * a.chunk < sp.np ? (split + 1) * a.chunk : sp.np;
-	int pos[NR];
-	size_t row[NR];
-	bool live[NR];
-#pragma unroll
-	for (int c = 0; c < NR; ++c) {
-		const int rr = r0 + 16 * c + col;
-		live[c] = rr < nrows;
-		const int t = (live[c] ? rr : r0) / a.group, hd = h * a.group + (live[c] ? rr : r0) % a.group;
-		pos[c] = len - n + t;
-		row[c] = (size_t)(row0 + t) * a.n_heads + hd;
-	}
+	const int rr = r0 + col;
+	const bool live = rr < nrows;
+	const int t = (live ? rr : r0) / a.group, hd = h * a.group + (live ? rr : r0) % a.group;
+	const int pos = len - n + t;
+	const size_t row = (size_t)(row0 + t) * a.n_heads + hd;
 	if (i0 >= i1 && split > 0) {
 		if (!direct && wave == 0 && g == 0) { // a range without pages: marked empty for k_kv_merge
-#pragma unroll
-			for (int c = 0; c < NR; ++c) {
-				if (live[c]) {
-					float* const p = a.part + (row[c] * a.n_splits + split) * (D + 4) + D;
-					p[0] = -__builtin_inff(), p[1] = 0.f;
-				}
+			if (live) {
+				float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
+				p[0] = -__builtin_inff(), p[1] = 0.f;
 			}
 		}
 		return;
 	}
 	// page ids of this wave's next 64 pages, one per lane; the first pages' codes are asked for before q is looked at
-	int ids = -1, ids0 = i0 + wave; // lane i: page ids0 + 4 i
+	int ids = -1, ids0 = i0 + wave; // lane i: page ids0 + NW i
 	const auto fetch_ids = [&](int first) {
 		ids0 = first;
-		const int i = first + 4 * lane;
+		const int i = first + NW * lane;
 		ids = -1;
 		if (i < i1) {
 			const int pg = sp.page(i);
@@ -595,108 +586,97 @@ __global__ __launch_bounds__(256, NR * D <= 128 ? 2 : 1) void k_kv_decode(KvAttn
 	__builtin_amdgcn_sched_barrier(0); // (the loads stay ahead of what follows)
 	// q as NQ signed digits of eight bits, row / 2^e = (d0 + d1 / 254 + d2 / 254^2) / 127: lane (col, g) holds dims g D / 4 .. of its row
 	constexpr int NQ = HL ? 3 : 2;
-	unsigned qd[NR][NQ][KW];
-	float qf[NR];
+	unsigned qd[NQ][KW];
+	float x[D / 4];
+	const size_t at = (row / a.n_heads) * (size_t)a.q_row + (row % a.n_heads) * (size_t)a.q_head + g * (D / 4);
+	unsigned top = 0;
 #pragma unroll
-	for (int c = 0; c < NR; ++c) {
-		float x[D / 4];
-		const size_t at = (row[c] / a.n_heads) * (size_t)a.q_row + (row[c] % a.n_heads) * (size_t)a.q_head + g * (D / 4);
-		unsigned top = 0;
+	for (int i = 0; i < D / 16; ++i) {
+		float y[4];
+		kv_load4<DT>(a.q, at + 4 * i, y);
 #pragma unroll
-		for (int i = 0; i < D / 16; ++i) {
-			float y[4];
-			kv_load4<DT>(a.q, at + 4 * i, y);
-#pragma unroll
-			for (int j = 0; j < 4; ++j) {
-				x[4 * i + j] = y[j];
-				const unsigned u = __builtin_bit_cast(unsigned, y[j]) & 0x7fffffffu;
-				top = top > u ? top : u;
-			}
-		}
-		const unsigned t1 = __shfl_xor(top, 16);
-		top = top > t1 ? top : t1;
-		const unsigned t2 = __shfl_xor(top, 32);
-		top = top > t2 ? top : t2;
-		const int e = kv_row_exp(__builtin_bit_cast(float, top));
-		const float inv = kv_exp2i(-e) * 127.f;
-		// (a row with an infinity or a NaN is NaN)
-		qf[c] = top >= 0x7f800000u ? __builtin_nanf("") : kv_exp2i(e) * a.scale * (1.f / 127.f);
-#pragma unroll
-		for (int i = 0; i < KW; ++i) {
-			unsigned w[NQ];
-#pragma unroll
-			for (int n = 0; n < NQ; ++n) {
-				w[n] = 0;
-			}
-#pragma unroll
-			for (int j = 0; j < 4; ++j) {
-				float y = x[4 * i + j] * inv; // (2^-126 * 127: no denormal)
-#pragma unroll
-				for (int n = 0; n < NQ; ++n) {
-					const float r = __builtin_rintf(y);
-					w[n] |= ((unsigned)(int)r & 0xffu) << (8 * j);
-					y = (y - r) * 254.f;
-				}
-			}
-#pragma unroll
-			for (int n = 0; n < NQ; ++n) {
-				qd[c][n][i] = w[n];
-			}
+		for (int j = 0; j < 4; ++j) {
+			x[4 * i + j] = y[j];
+			const unsigned u = __builtin_bit_cast(unsigned, y[j]) & 0x7fffffffu;
+			top = top > u ? top : u;
 		}
 	}
-	float m[NR], l[NR];
-	kv_f32x4 o[NR][ND];
+	const unsigned t1 = __shfl_xor(top, 16);
+	top = top > t1 ? top : t1;
+	const unsigned t2 = __shfl_xor(top, 32);
+	top = top > t2 ? top : t2;
+	const int e0 = kv_row_exp(__builtin_bit_cast(float, top)), e = e0 < -119 ? -119 : e0; // (2^119 * 127 is a number; smaller rows' scores are none)
+	const float inv = kv_exp2i(-e) * 127.f;
+	// (a row with an infinity or a NaN is NaN)
+	const float qf = top >= 0x7f800000u ? __builtin_nanf("") : kv_exp2i(e) * a.scale * (1.f / 127.f);
 #pragma unroll
-	for (int c = 0; c < NR; ++c) {
-		m[c] = -__builtin_inff(), l[c] = 0.f;
+	for (int i = 0; i < KW; ++i) {
+		unsigned w[NQ];
 #pragma unroll
-		for (int d = 0; d < ND; ++d) {
-			o[c][d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
+		for (int n = 0; n < NQ; ++n) {
+			w[n] = 0;
 		}
+#pragma unroll
+		for (int j = 0; j < 4; ++j) {
+			float y = top >= 0x7f800000u ? 0.f : x[4 * i + j] * inv;
+#pragma unroll
+			for (int n = 0; n < NQ; ++n) {
+				const float r = __builtin_rintf(y);
+				w[n] |= ((unsigned)(int)r & 0xffu) << (8 * j);
+				y = (y - r) * 254.f;
+			}
+		}
+#pragma unroll
+		for (int n = 0; n < NQ; ++n) {
+			qd[n][i] = w[n];
+		}
+	}
+	kv_f32x4 o[ND];
+	float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+	for (int d = 0; d < ND; ++d) {
+		o[d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
 	}
 	float E = 1.1754944e-38f; // the largest V scale met
-	for (int i = i0 + wave; i < i1; i += 4) {
+	for (int i = i0 + wave; i < i1; i += NW) {
 		const int pg = sp.page(i), j0 = pg * KV_PAGE;
 		const bool bad = pid < 0;
-		const bool more = i + 4 < i1;
-		if (more && i + 4 >= ids0 + 256) {
-			fetch_ids(i + 4);
+		const bool more = i + NW < i1;
+		if (more && i + NW >= ids0 + 64 * NW) {
+			fetch_ids(i + NW);
 		}
-		const int next = more ? __builtin_amdgcn_readlane(ids, (i + 4 - ids0) >> 2) : -1;
+		const int next = more ? __builtin_amdgcn_readlane(ids, (i + NW - ids0) / NW) : -1;
 		// S^T of the page: tile t = block t, this lane's tokens 4 g + e; whole numbers, exactly
-		kv_f32x4 sc[NR][4];
+		kv_f32x4 sc[4];
 #pragma unroll
 		for (int t = 0; t < 4; ++t) {
+			kv_i32x4 acc[NQ];
 #pragma unroll
-			for (int c = 0; c < NR; ++c) {
-				kv_i32x4 acc[NQ];
+			for (int n = 0; n < NQ; ++n) {
+				acc[n] = (kv_i32x4){0, 0, 0, 0};
+				if constexpr (D % 64 == 0) {
 #pragma unroll
-				for (int n = 0; n < NQ; ++n) {
-					acc[n] = (kv_i32x4){0, 0, 0, 0};
-					if constexpr (D % 64 == 0) {
+					for (int k = 0; k < D / 64; ++k) {
+						const kv_i32x4 kf = {(int)kr[t][4 * k], (int)kr[t][4 * k + 1], (int)kr[t][4 * k + 2], (int)kr[t][4 * k + 3]};
+						const kv_i32x4 qv = {(int)qd[n][4 * k], (int)qd[n][4 * k + 1], (int)qd[n][4 * k + 2], (int)qd[n][4 * k + 3]};
+						acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qv, acc[n], 0, 0, 0);
+					}
+				} else {
 #pragma unroll
-						for (int k = 0; k < D / 64; ++k) {
-							const kv_i32x4 kf = {(int)kr[t][4 * k], (int)kr[t][4 * k + 1], (int)kr[t][4 * k + 2], (int)kr[t][4 * k + 3]};
-							const kv_i32x4 qv = {(int)qd[c][n][4 * k], (int)qd[c][n][4 * k + 1], (int)qd[c][n][4 * k + 2], (int)qd[c][n][4 * k + 3]};
-							acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qv, acc[n], 0, 0, 0);
-						}
-					} else {
-#pragma unroll
-						for (int k = 0; k < D / 32; ++k) {
-							const long kf = (long)(((unsigned long)kr[t][2 * k + 1] << 32) | kr[t][2 * k]);
-							const long qv = (long)(((unsigned long)qd[c][n][2 * k + 1] << 32) | qd[c][n][2 * k]);
-							acc[n] = __builtin_amdgcn_mfma_i32_16x16x32_i8(kf, qv, acc[n], 0, 0, 0);
-						}
+					for (int k = 0; k < D / 32; ++k) {
+						const long kf = (long)(((unsigned long)kr[t][2 * k + 1] << 32) | kr[t][2 * k]);
+						const long qv = (long)(((unsigned long)qd[n][2 * k + 1] << 32) | qd[n][2 * k]);
+						acc[n] = __builtin_amdgcn_mfma_i32_16x16x32_i8(kf, qv, acc[n], 0, 0, 0);
 					}
 				}
+			}
 #pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					float y = __builtin_fmaf((float)acc[1][e], 1.f / 254.f, (float)acc[0][e]);
-					if constexpr (HL) {
-						y = __builtin_fmaf((float)acc[2][e], 1.f / (254.f * 254.f), y);
-					}
-					sc[c][t][e] = y;
+			for (int e = 0; e < 4; ++e) {
+				float y = __builtin_fmaf((float)acc[1][e], 1.f / 254.f, (float)acc[0][e]);
+				if constexpr (HL) {
+					y = __builtin_fmaf((float)acc[2][e], 1.f / (254.f * 254.f), y);
 				}
+				sc[t][e] = y;
 			}
 		}
 		const kv_f32x4 kscale = bad ? (kv_f32x4){__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")} : ksc;
@@ -714,72 +694,69 @@ __global__ __launch_bounds__(256, NR * D <= 128 ? 2 : 1) void k_kv_decode(KvAttn
 		}
 		const float rE = __builtin_amdgcn_rcpf(Enew), grow = E * rE;
 		E = Enew;
-		kv_f16x8 pf[NR][2], pl[NR][HL ? 2 : 1];
+		kv_f16x8 pf[2], pl[HL ? 2 : 1];
+		float top = -__builtin_inff();
+		if (!whole) {
 #pragma unroll
-		for (int c = 0; c < NR; ++c) {
-			float top = -__builtin_inff();
-			if (!whole) {
+			for (int t = 0; t < 4; ++t) {
 #pragma unroll
-				for (int t = 0; t < 4; ++t) {
-#pragma unroll
-					for (int e = 0; e < 4; ++e) {
-						const int j = j0 + 16 * t + 4 * g + e;
-						const bool seen = j <= pos[c] && (a.window <= 0 || j > pos[c] - a.window || j < a.sinks);
-						sc[c][t][e] = seen ? sc[c][t][e] * (kscale[t] * qf[c]) : -__builtin_inff();
-						top = fmaxf(top, sc[c][t][e]);
-					}
-				}
-			} else {
-#pragma unroll
-				for (int t = 0; t < 4; ++t) {
-					const float f = kscale[t] * qf[c];
-					const float hi = fmaxf(fmaxf(sc[c][t][0], sc[c][t][1]), fmaxf(sc[c][t][2], sc[c][t][3])) * f;
-					const float lo = fminf(fminf(sc[c][t][0], sc[c][t][1]), fminf(sc[c][t][2], sc[c][t][3])) * f;
-					top = fmaxf(top, fmaxf(hi, lo)); // (a negative factor turns them round)
+				for (int e = 0; e < 4; ++e) {
+					const int j = j0 + 16 * t + 4 * g + e;
+					const bool seen = j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+					sc[t][e] = seen ? sc[t][e] * (kscale[t] * qf) : -__builtin_inff();
+					top = fmaxf(top, sc[t][e]);
 				}
 			}
-			top = kv_max32(kv_max16(top));
-			// the reference stays unless a score passes it by 2^8 (weights up to 2^8 are no less exact): sums are seldom rescaled
-			const float ref = top > m[c] + 8.f || m[c] == -__builtin_inff() ? fmaxf(top, m[c]) : m[c];
-			const float zero_ref = ref == -__builtin_inff() ? 0.f : ref;
-			const float alpha = kv_exp2(m[c] - zero_ref); // (m = -inf: 0)
-			m[c] = ref;
-			const float og = alpha * grow;
-			if (__ballot(og != 1.f)) {
-				l[c] *= alpha;
+		} else {
 #pragma unroll
-				for (int d = 0; d < ND; ++d) {
-					o[c][d] *= og;
-				}
+			for (int t = 0; t < 4; ++t) {
+				const float f = kscale[t] * qf;
+				const float hi = fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])) * f;
+				const float lo = fminf(fminf(sc[t][0], sc[t][1]), fminf(sc[t][2], sc[t][3])) * f;
+				top = fmaxf(top, fmaxf(hi, lo)); // (a negative factor turns them round)
 			}
-			if (!whole) {
+		}
+		top = kv_max32(kv_max16(top));
+		// the reference stays unless a score passes it by 2^8 (weights up to 2^8 are no less exact): sums are seldom rescaled
+		const float ref = top > m + 8.f || m == -__builtin_inff() ? fmaxf(top, m) : m;
+		const float zero_ref = ref == -__builtin_inff() ? 0.f : ref;
+		const float alpha = kv_exp2(m - zero_ref); // (m = -inf: 0)
+		m = ref;
+		const float og = alpha * grow;
+		if (__ballot(og != 1.f)) {
+			l *= alpha;
 #pragma unroll
-				for (int t = 0; t < 4; ++t) {
-					const float f = vsc[t] * rE;
+			for (int d = 0; d < ND; ++d) {
+				o[d] *= og;
+			}
+		}
+		if (!whole) {
 #pragma unroll
-					for (int e = 0; e < 4; ++e) {
-						const float w = kv_exp2(sc[c][t][e] - zero_ref);
-						l[c] += w;
-						const float y = sc[c][t][e] == -__builtin_inff() ? 0.f : w * f; // (a NaN scale must not reach a row that does not see the token)
-						pf[c][t >> 1][4 * (t & 1) + e] = (_Float16)y;
-						if constexpr (HL) {
-							pl[c][t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[c][t >> 1][4 * (t & 1) + e]);
-						}
+			for (int t = 0; t < 4; ++t) {
+				const float f = vsc[t] * rE;
+#pragma unroll
+				for (int e = 0; e < 4; ++e) {
+					const float w = kv_exp2(sc[t][e] - zero_ref);
+					l += w;
+					const float y = sc[t][e] == -__builtin_inff() ? 0.f : w * f; // (a NaN scale must not reach a row that does not see the token)
+					pf[t >> 1][4 * (t & 1) + e] = (_Float16)y;
+					if constexpr (HL) {
+						pl[t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[t >> 1][4 * (t & 1) + e]);
 					}
 				}
-			} else {
+			}
+		} else {
 #pragma unroll
-				for (int t = 0; t < 4; ++t) {
-					const float f = kscale[t] * qf[c], fv = vsc[t] * rE;
+			for (int t = 0; t < 4; ++t) {
+				const float f = kscale[t] * qf, fv = vsc[t] * rE;
 #pragma unroll
-					for (int e = 0; e < 4; ++e) {
-						const float w = kv_exp2(__builtin_fmaf(sc[c][t][e], f, -zero_ref));
-						l[c] += w;
-						const float y = w * fv;
-						pf[c][t >> 1][4 * (t & 1) + e] = (_Float16)y;
-						if constexpr (HL) {
-							pl[c][t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[c][t >> 1][4 * (t & 1) + e]);
-						}
+				for (int e = 0; e < 4; ++e) {
+					const float w = kv_exp2(__builtin_fmaf(sc[t][e], f, -zero_ref));
+					l += w;
+					const float y = w * fv;
+					pf[t >> 1][4 * (t & 1) + e] = (_Float16)y;
+					if constexpr (HL) {
+						pl[t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[t >> 1][4 * (t & 1) + e]);
 					}
 				}
 			}
@@ -789,12 +766,9 @@ __global__ __launch_bounds__(256, NR * D <= 128 ? 2 : 1) void k_kv_decode(KvAttn
 #pragma unroll
 			for (int u = 0; u < 2; ++u) {
 				const kv_f16x8 vf = kv_codes8(vr[d][2 * u], vr[d][2 * u + 1]);
-#pragma unroll
-				for (int c = 0; c < NR; ++c) {
-					o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[c][u], o[c][d], 0, 0, 0);
-					if constexpr (HL) {
-						o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[c][u], o[c][d], 0, 0, 0);
-					}
+				o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[u], o[d], 0, 0, 0);
+				if constexpr (HL) {
+					o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[u], o[d], 0, 0, 0);
 				}
 			}
 		}
@@ -803,36 +777,36 @@ __global__ __launch_bounds__(256, NR * D <= 128 ? 2 : 1) void k_kv_decode(KvAttn
 		}
 		pid = next;
 	}
-	// the four waves' sums
-	float* const mine = kv_lds + wave * (16 * NR * (D + 4));
+	// the waves' sums
+	float* const mine = kv_lds + wave * (16 * (D + 4));
+	l += __shfl_xor(l, 16);
+	l += __shfl_xor(l, 32);
+	float* const p = mine + (col) * (D + 4);
 #pragma unroll
-	for (int c = 0; c < NR; ++c) {
-		l[c] += __shfl_xor(l[c], 16);
-		l[c] += __shfl_xor(l[c], 32);
-		float* const p = mine + (16 * c + col) * (D + 4);
-#pragma unroll
-		for (int d = 0; d < ND; ++d) {
-			*(kv_f32x4*)(p + 16 * d + 4 * g) = o[c][d];
-		}
-		if (g == 0) {
-			p[D] = m[c], p[D + 1] = l[c], p[D + 2] = E;
-		}
+	for (int d = 0; d < ND; ++d) {
+		*(kv_f32x4*)(p + 16 * d + 4 * g) = o[d];
+	}
+	if (g == 0) {
+		p[D] = m, p[D + 1] = l, p[D + 2] = E;
 	}
 	__syncthreads();
 	// a thread per (row, quad of dims)
-	for (int it = threadIdx.x; it < 16 * NR * (D / 4); it += 256) {
+	for (int it = threadIdx.x; it < 16 * (D / 4); it += 64 * NW) {
 		const int rr = it / (D / 4), d = it % (D / 4) * 4;
 		if (r0 + rr >= nrows) {
 			break;
 		}
 		const float* const p = kv_lds + rr * (D + 4);
-		constexpr int W = 16 * NR * (D + 4);
-		float M = fmaxf(fmaxf(p[D], p[W + D]), fmaxf(p[2 * W + D], p[3 * W + D]));
-		const float EM = fmaxf(fmaxf(p[D + 2], p[W + D + 2]), fmaxf(p[2 * W + D + 2], p[3 * W + D + 2]));
+		constexpr int W = 16 * (D + 4);
+		float M = -__builtin_inff(), EM = 0.f;
+#pragma unroll
+		for (int w = 0; w < NW; ++w) {
+			M = fmaxf(M, p[w * W + D]), EM = fmaxf(EM, p[w * W + D + 2]);
+		}
 		const float ref = M == -__builtin_inff() ? 0.f : M;
 		float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-		for (int w = 0; w < 4; ++w) {
+		for (int w = 0; w < NW; ++w) {
 			const float f = kv_exp2(p[w * W + D] - ref), fe = f * (p[w * W + D + 2] / EM);
 			L += f * p[w * W + D + 1];
 			const kv_f32x4 x = *(const kv_f32x4*)(p + w * W + d);

@@ -129,28 +129,28 @@ int kv_dispatch(int head_dim, int type, F f) {
 
 // How attention is cut: rows per workgroup, and the pages a workgroup walks.
 struct KvCut {
-	bool chunked;           // k_kv_chunk (128 rows a workgroup), else k_kv_decode (16 or 32)
-	int nr, tiles, n_splits, chunk;
+	bool chunked;           // k_kv_chunk (128 rows a workgroup), else k_kv_decode (16)
+	int nw, tiles, n_splits, chunk;
 };
 KvCut kv_cut(const struct KvPool* p, const struct KvBatch* b, int n_heads, int type, int window, int sinks) {
 	KvCut c;
-	const int group = n_heads / p->n_kv_heads;
+	const int group = n_heads / p->n_kv_heads, cus = kv_cus();
 	const long long rows = (long long)(b->max_rows < 1 ? 1 : b->max_rows) * group; // rows of a sequence and kv head
+	const long long base = (long long)b->n_seqs * p->n_kv_heads;
+	// pages that a tile of `per` rows sees at most
+	const auto pages = [&](int per) {
+		long long seen = ((long long)b->max_len + KV_PAGE - 1) / KV_PAGE;
+		if (window > 0) {
+			const long long span = ((long long)window + per / group + 2 * KV_PAGE) / KV_PAGE + 1 + ((long long)sinks + KV_PAGE - 1) / KV_PAGE;
+			seen = span < seen ? span : seen;
+		}
+		return seen < 1 ? 1 : seen;
+	};
 	// (fp32 rows of 256: both halves of q and the sums do not fit a wave's registers)
 	c.chunked = rows > 32 && !(p->head_dim == 256 && type == KV_F32);
-	c.nr = rows > 16 && p->head_dim <= 128 ? 2 : 1;
-	const int per = c.chunked ? 128 : 16 * c.nr;
-	c.tiles = (int)((rows + per - 1) / per);
-	// pages a row tile sees at most
-	long long seen = ((long long)b->max_len + KV_PAGE - 1) / KV_PAGE;
-	if (window > 0) {
-		const long long span = ((long long)window + per / group + 2 * KV_PAGE) / KV_PAGE + 1 + ((long long)sinks + KV_PAGE - 1) / KV_PAGE;
-		seen = span < seen ? span : seen;
-	}
-	seen = seen < 1 ? 1 : seen;
-	const long long wgs = (long long)b->n_seqs * p->n_kv_heads * c.tiles;
-	const int cus = kv_cus();
 	if (c.chunked) { // two workgroups per CU, at least 8 pages each (the join moves every row's partial sums through memory)
+		c.nw = 4, c.tiles = (int)((rows + 127) / 128);
+		const long long wgs = base * c.tiles, seen = pages(128);
 		long long splits = (2ll * cus + wgs - 1) / wgs;
 		splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
 		const long long chunk = (seen + splits - 1) / splits;
@@ -158,15 +158,18 @@ KvCut kv_cut(const struct KvPool* p, const struct KvBatch* b, int n_heads, int t
 		c.n_splits = (int)((seen + c.chunk - 1) / c.chunk);
 		return c;
 	}
-	// What a cut into s ranges costs, in steps of a workgroup (a page for each of its four waves, about 1.5 us): two workgroups fit a CU, at 0.7
-	// of the time each, a round of them begins with the look-ups and first loads (2.5 steps), and ranges are joined by a second launch.
-	// Measured, s = 1 / 2 / 4 / 8: 8 sequences of 4093, 8 kv heads (64 workgroups uncut) - / - / 21.3 / 22.9 us; 64 of 91 - 8191, 4 kv heads (256)
-	// 49.7 / 39.3 / 41.5 / 46.4; one of 333 (8 workgroups, 6 pages) 10.7 / 15.
+	// What a cut into n ranges costs, in steps of a workgroup (a page for each of its waves, about 2 us): workgroups run in rounds of one
+	// to a CU (their registers fill it), a round begins with look-ups and first loads (2 steps), and ranges are joined by a second launch.
+	// Measured, n = 1 / 2 / 4 / 8, in us: 8 sequences of 4093, 8 kv heads of 128 (64 workgroups uncut) 32.2 / 24.7 / 21.8 / 30.7; 64 of 91 - 8191, 4 kv
+	// heads of 64 (256) 36.3 / 43.2 / 50.2 / 63.5; 24 of 13.9 - 16.4k (192) 136 / 158 / 144 / 151; 16 under a window of 1024 (256) 13.7 / 27.3 / 27.8.
+	const int nw = p->head_dim <= 128 ? 8 : 4;
+	c.nw = nw, c.tiles = (int)((rows + 15) / 16);
+	const long long wgs = base * c.tiles, seen = pages(16);
 	double best = 0;
-	for (long long n = 1; n <= 64 && (n == 1 || (n - 1) * 4 < seen); ++n) {
-		const double per_cu = (double)(wgs * n) / cus, rounds = ceil(per_cu / 2), step = per_cu <= 1 ? 1.0 : 1.4;
-		const long long chunk = ((seen + n - 1) / n + 3) / 4 * 4; // whole steps
-		const double cost = rounds * ((double)(chunk / 4) * step + 2.5) + (n > 1 ? 3.0 + 0.25 * (double)n : 0.0);
+	for (long long n = 1; n <= 64 && (n == 1 || (n - 1) * nw < seen); ++n) {
+		const double rounds = ceil((double)(wgs * n) / cus);
+		const long long chunk = ((seen + n - 1) / n + nw - 1) / nw * nw; // whole steps
+		const double cost = rounds * ((double)(chunk / nw) + 2.0) + (n > 1 ? 2.0 + 0.2 * (double)n : 0.0);
 		if (n == 1 || cost < 0.97 * best) {
 			best = cost;
 			c.chunk = (int)chunk;
@@ -305,23 +308,13 @@ extern "C" int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* ba
 				hipLaunchKernelGGL(kern, dim3((unsigned)c.tiles * H * batch->n_seqs * c.n_splits), dim3(256), lds, st, a);
 			}
 		} else {
-			const auto go = [&](auto NRc) {
-				constexpr int NR = decltype(NRc)::value;
-				auto kern = k_kv_decode<D, T, NR>;
-				constexpr size_t lds = (size_t)4 * 16 * NR * (D + 4) * sizeof(float);
-				if (kv_lds((const void*)kern, lds, "kv_attend_hip")) {
-					return -1;
-				}
-				hipLaunchKernelGGL(kern, dim3(c.n_splits, H * c.tiles, batch->n_seqs), dim3(256), lds, st, a);
-				return 0;
-			};
-			if constexpr (D <= 128) {
-				if (c.nr == 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>())) {
-					return -1;
-				}
-			} else if (go(std::integral_constant<int, 1>())) {
+			constexpr int NW = D <= 128 ? 8 : 4;
+			auto kern = k_kv_decode<D, T, NW>;
+			constexpr size_t lds = (size_t)NW * 16 * (D + 4) * sizeof(float);
+			if (kv_lds((const void*)kern, lds, "kv_attend_hip")) {
 				return -1;
 			}
+			hipLaunchKernelGGL(kern, dim3(c.n_splits, H * c.tiles, batch->n_seqs), dim3(64 * NW), lds, st, a);
 		}
 		if (c.n_splits > 1) {
 			hipLaunchKernelGGL((k_kv_merge<D, T>), dim3(((unsigned)batch->n_rows * n_heads + 3) / 4), dim3(256), 0, st, a);
