@@ -166,10 +166,15 @@ __device__ __forceinline__ bool kv_find(int n_seqs, int target, F count, int& se
 	return false;
 }
 
+// does sequence s of a batch fit its bounds?
+__device__ __forceinline__ bool kv_rows_fit(const KvRows& r, int s) {
+	const int row0 = r.cu[s], n = r.cu[s + 1] - row0;
+	return row0 >= 0 && n >= 0 && n <= r.max_rows && r.n_rows - row0 >= n;
+}
 // the rows of sequence s that count: inside the packed arrays, at positions >= 0
 __device__ __forceinline__ void kv_rows_of(const KvRows& r, int s, int& row0, int& n, int& len) {
 	row0 = r.cu[s], n = r.cu[s + 1] - row0, len = r.lens[s];
-	if (row0 < 0 || n < 0 || row0 + n > r.n_rows) {
+	if (row0 < 0 || n < 0 || r.n_rows - row0 < n) {
 		n = 0;
 	}
 	len = len < 0 ? 0 : len;
@@ -190,6 +195,9 @@ __global__ __launch_bounds__(256, DT == KV_F32 || D > 128 ? 1 : D == 96 ? 7 : 8)
 	const KvRows& r = a.r;
 	const auto pages = [&](int i) {
 		int row0, n, len;
+		if (blockIdx.x == 0 && h == 0 && blk == 0 && !kv_rows_fit(r, i)) {
+			kv_flag(a.p.status, KV_BAD_BATCH);
+		}
 		kv_rows_of(r, i, row0, n, len);
 		n = n < len ? n : len;
 		return n > 0 ? (len - 1) / KV_PAGE - (len - n) / KV_PAGE + 1 : 0;
@@ -503,7 +511,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 	int row0, n, len;
 	kv_rows_of(a.r, s, row0, n, len);
 	const int nrows = n * a.group, r0 = tile * 16;
-	if (threadIdx.x == 0 && tile == 0 && h == 0 && split == 0 && n > a.r.max_rows) {
+	if (threadIdx.x == 0 && tile == 0 && h == 0 && split == 0 && !kv_rows_fit(a.r, s)) {
 		kv_flag(a.p.status, KV_BAD_BATCH);
 	}
 	if (r0 >= nrows) {
@@ -512,8 +520,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 	const int rl = r0 + 15 < nrows - 1 ? r0 + 15 : nrows - 1;
 	const int p_min = len - n + r0 / a.group, p_max = len - n + rl / a.group;
 	const KvSpan sp(p_min, p_max, a.window, a.sinks);
-	const bool direct = sp.np <= a.chunk;
-	const int i0 = split * a.chunk, i1 = (split + 1) * a.chunk < sp.np ? (split + 1) * a.chunk : sp.np;
+	// ranges of a.chunk pages; the last takes what a sequence longer than the host's bound has beyond them
+	const bool direct = sp.np <= a.chunk || a.n_splits == 1;
+	const int i0 = split * a.chunk, i1 = split + 1 < a.n_splits && (split + 1) * a.chunk < sp.np ? (split + 1) * a.chunk : sp.np;
 	const int rr = r0 + col;
 	const bool live = rr < nrows;
 	const int t = (live ? rr : r0) / a.group, hd = h * a.group + (live ? rr : r0) % a.group;
@@ -679,7 +688,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 				sc[t][e] = y;
 			}
 		}
-		const kv_f32x4 kscale = bad ? (kv_f32x4){__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")} : ksc;
+		// (a missing page: NaN through K; its V scale must not become the reference of rows that do not see it)
+		const float none = __builtin_nanf("");
+		const kv_f32x4 kscale = bad ? (kv_f32x4){none, none, none, none} : ksc, vscale = bad ? (kv_f32x4){0.f, 0.f, 0.f, 0.f} : vsc;
 		if (more) {
 			load_k(next);
 		}
@@ -690,7 +701,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		for (int t = 0; t < 4; ++t) {
 			const int jb = j0 + 16 * t;
 			const bool seen = whole || (jb <= p_max && (a.window <= 0 || jb + 15 > p_min - a.window || jb < a.sinks));
-			Enew = fmaxf(Enew, seen ? fabsf(vsc[t]) : 0.f);
+			Enew = fmaxf(Enew, seen ? fabsf(vscale[t]) : 0.f);
 		}
 		const float rE = __builtin_amdgcn_rcpf(Enew), grow = E * rE;
 		E = Enew;
@@ -733,7 +744,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		if (!whole) {
 #pragma unroll
 			for (int t = 0; t < 4; ++t) {
-				const float f = vsc[t] * rE;
+				const float f = vscale[t] * rE;
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
 					const float w = kv_exp2(sc[t][e] - zero_ref);
@@ -748,7 +759,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		} else {
 #pragma unroll
 			for (int t = 0; t < 4; ++t) {
-				const float f = kscale[t] * qf, fv = vsc[t] * rE;
+				const float f = kscale[t] * qf, fv = vscale[t] * rE;
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
 					const float w = kv_exp2(__builtin_fmaf(sc[t][e], f, -zero_ref));
@@ -835,8 +846,8 @@ template <int D, int DT>
 __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 	const int lane = lane_id();
 	const size_t row = (size_t)blockIdx.x * 4 + wave_id();
-	const int last = a.r.cu[a.r.n_seqs] < a.r.n_rows ? a.r.cu[a.r.n_seqs] : a.r.n_rows;
-	if (row >= (size_t)(last < 0 ? 0 : last) * a.n_heads) {
+	const int first = a.r.cu[0] < 0 ? 0 : a.r.cu[0], end = a.r.cu[a.r.n_seqs], last = end < a.r.n_rows ? end : a.r.n_rows;
+	if (row >= (size_t)(last < 0 ? 0 : last) * a.n_heads || row < (size_t)first * a.n_heads) {
 		return; // rows behind the last sequence stay as they are
 	}
 	const float* const p = a.part + row * a.n_splits * (D + 4);
@@ -923,7 +934,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	int row0, n, len;
 	kv_rows_of(a.r, s, row0, n, len);
 	const int nrows = n * a.group;
-	if (tid == 0 && r0 == 0 && h == 0 && split == 0 && n > a.r.max_rows) {
+	if (tid == 0 && r0 == 0 && h == 0 && split == 0 && !kv_rows_fit(a.r, s)) {
 		kv_flag(a.p.status, KV_BAD_BATCH);
 	}
 	if (r0 >= nrows) {
@@ -932,8 +943,9 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	const int rl = r0 + 127 < nrows - 1 ? r0 + 127 : nrows - 1;
 	const int p_min = len - n + r0 / a.group, p_max = len - n + rl / a.group;
 	const KvSpan sp(p_min, p_max, a.window, a.sinks);
-	const bool direct = sp.np <= a.chunk;
-	const int i0 = split * a.chunk, i1 = (split + 1) * a.chunk < sp.np ? (split + 1) * a.chunk : sp.np;
+	// ranges of a.chunk pages; the last takes what a sequence longer than the host's bound has beyond them
+	const bool direct = sp.np <= a.chunk || a.n_splits == 1;
+	const int i0 = split * a.chunk, i1 = split + 1 < a.n_splits && (split + 1) * a.chunk < sp.np ? (split + 1) * a.chunk : sp.np;
 	// this wave's rows
 	const int rr = r0 + 32 * wave + col;
 	const bool live = rr < nrows;
@@ -1066,7 +1078,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 		const bool more = i + 1 < i1;
 		const bool bad = pid < 0;
 		const float none = __builtin_nanf("");
-		const kv_f32x4 ksc = bad ? (kv_f32x4){none, none, none, none} : ksc_n, vsc = vsc_n;
+		const kv_f32x4 ksc = bad ? (kv_f32x4){none, none, none, none} : ksc_n, vsc = bad ? (kv_f32x4){0.f, 0.f, 0.f, 0.f} : vsc_n;
 		int next = -1;
 		if (more) {
 			if (i + 1 >= ids0 + 64) {

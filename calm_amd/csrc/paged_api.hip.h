@@ -67,8 +67,8 @@ const char* kv_pool_fault(const struct KvPool* p) {
 	if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale || !p->status) {
 		return "a pool pointer is missing";
 	}
-	if (p->n_layers < 1 || p->n_layers > 65535 || p->n_pages < 1 || p->n_kv_heads < 1 || p->n_kv_heads > 1024) {
-		return "the pool has no layers, pages or heads, or more than 65535 layers or 1024 heads";
+	if (p->n_layers < 1 || p->n_layers > 65535 || p->n_pages < 1 || p->n_pages > 1 << 30 || p->n_kv_heads < 1 || p->n_kv_heads > 1024) {
+		return "the pool has no layers, pages or heads, or more than 65535 layers, 2^30 pages or 1024 heads";
 	}
 	if (p->head_dim != 64 && p->head_dim != 96 && p->head_dim != 128 && p->head_dim != 256) {
 		return "head sizes 64, 96, 128 and 256";
@@ -85,8 +85,8 @@ const char* kv_batch_fault(const struct KvBatch* b) {
 	if (b->n_seqs < 1 || b->n_seqs > 65535 || b->max_pages < 1 || b->n_rows < 0 || b->max_rows < 0 || b->max_len < 0) {
 		return "a batch has 1 to 65535 sequences, at least one page column and no negative counts";
 	}
-	if ((long long)b->n_seqs * b->max_pages > 0x7fffffffll) {
-		return "a table of more than 2^31 entries";
+	if ((long long)b->n_seqs * b->max_pages > 1 << 30) {
+		return "a table of more than 2^30 entries";
 	}
 	return nullptr;
 }
@@ -288,6 +288,12 @@ extern "C" int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* ba
 	const KvCut c = kv_cut(pool, batch, n_heads, type, window, sinks);
 	const size_t need = kv_cut_bytes(c, pool, batch, n_heads);
 	KV_CHECK(need == 0 || (workspace && workspace_size >= need && kv_aligned(workspace, 16)), "the workspace is missing, too small (kv_attend_workspace_hip) or not 16-byte aligned");
+	{ // (a row of out may be written while another workgroup still reads that row of q)
+		const long rows = batch->n_rows, item = type == KV_F32 ? 4 : 2, dr = (rows - 1) * q_row, dh = (n_heads - 1) * q_head;
+		const char* const q0 = (const char*)q + item * ((dr < 0 ? dr : 0) + (dh < 0 ? dh : 0));
+		const char* const q1 = (const char*)q + item * ((dr > 0 ? dr : 0) + (dh > 0 ? dh : 0) + pool->head_dim);
+		KV_CHECK((const char*)out + item * rows * n_heads * pool->head_dim <= q0 || (const char*)out >= q1, "the output overlaps the query rows");
+	}
 	KvAttnArgs a;
 	a.p = kv_layer(pool, layer), a.r = kv_rows(batch);
 	a.q = q, a.out = out, a.q_row = q_row, a.q_head = q_head, a.part = (float*)workspace;
@@ -331,8 +337,8 @@ static const char* kv_table_fault(const struct KvPool* pool, const int* table, c
 	if (!table || !refs || !lens) {
 		return "table, lengths or counts are missing";
 	}
-	if (n_rows < 1 || n_rows > KV_MAX_ROWS || max_pages < 1 || (long long)n_rows * max_pages > 0x7fffffffll) {
-		return "1 to 2048 table rows, at least one page column, less than 2^31 entries";
+	if (n_rows < 1 || n_rows > KV_MAX_ROWS || max_pages < 1 || (long long)n_rows * max_pages > 1 << 30) {
+		return "1 to 2048 table rows, at least one page column, at most 2^30 entries";
 	}
 	return nullptr;
 }

@@ -116,6 +116,7 @@ def _name(x) -> str:
 
 
 _nothing = contextlib.nullcontext()
+_INT = 2 ** 31 - 1
 _torch = None  # torch and the functions that every call asks, once it is known to be there
 
 
@@ -174,6 +175,23 @@ def _empty(like, shape, dtype: str):
 def _need(cond, what: str) -> None:
     if not cond:
         raise ValueError(what)
+
+
+def _together(arrays) -> None:
+    """arrays that are kept for later calls: of one kind, on one device"""
+    first = arrays[0]
+    for a in arrays[1:]:
+        if isinstance(a, DeviceArray) != isinstance(first, DeviceArray):
+            raise ValueError("tensors and DeviceArrays in one call")
+        if getattr(a, "device", None) != getattr(first, "device", None):
+            raise ValueError(f"arrays on {first.device} and on {a.device} in one call")
+
+
+def _sees(layer: int, layers: int, window: int, sinks: int) -> None:
+    if not 0 <= layer < layers:
+        raise ValueError(f"no such layer: {layer} of {layers}")
+    if not (0 <= window <= _INT and 0 <= sinks <= _INT):
+        raise ValueError(f"window {window} and first tokens {sinks}: 0 to {_INT}")
 
 
 def _array(x, name: str, dtypes, shape) -> None:
@@ -236,6 +254,7 @@ class KvPool:
         _array(v, "v", ("int8",), (layers, pages, heads, 4, dim, 16))
         for x, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
             _array(x, name, ("float32",), (layers, pages, heads, 4))
+        _together((k, v, k_scale, v_scale))
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_layers, self.n_pages, self.n_kv_heads, self.head_dim = layers, pages, heads, dim
         if isinstance(k, DeviceArray):
@@ -260,7 +279,7 @@ class KvPool:
             if found:
                 self.status.zero_()
         words = [(1, "a page that was needed is missing from the table or outside the pool"), (2, "no page was free"),
-                 (4, "a sequence has more new rows than max_rows"), (8, "a parent outside the table")]
+                 (4, "a sequence has more new rows than max_rows, or row starts that do not fit the rows"), (8, "a parent outside the table")]
         if found:
             raise RuntimeError("paged cache: " + "; ".join(w for bit, w in words if found & bit))
 
@@ -275,7 +294,9 @@ class KvBatch:
         n, mp = (int(x) for x in table.shape)
         _array(lens, "lens", ("int32",), (n,))
         _array(starts, "starts", ("int32",), (n + 1,))
+        _together((table, lens, starts))
         _need(n > 0 and mp > 0, "a table without rows or columns")
+        _need(rows <= _INT and max_len <= _INT, f"rows and max_len are at most {_INT}")
         _need(rows >= 0 and 0 <= max_rows <= rows and max_len >= 0, "rows, max_rows and max_len are not negative, max_rows is at most rows")
         self.table, self.lens, self.starts = table, lens, starts
         self.n_seqs, self.rows, self.max_rows, self.max_len = n, rows, max_rows, max_len
@@ -289,14 +310,16 @@ def append(pool: KvPool, batch: KvBatch, k, v, layer: int = 0) -> None:
     kr, kh = _rows(k, "k", batch.rows, pool.n_kv_heads, pool.head_dim)
     vr, vh = _rows(v, "v", batch.rows, pool.n_kv_heads, pool.head_dim)
     _need(_name(k) == _name(v), "k and v of different types")
+    _sees(layer, pool.n_layers, 0, 0)
     stream, guard = _on((k, v, pool.k, batch.table))
     _call(guard, _lib().kv_append_hip, pool._ref, batch._ref, layer, k.data_ptr(), v.data_ptr(), _TYPES[_name(k)], kr, kh, vr, vh, stream)
 
 
 def attend(pool: KvPool, batch: KvBatch, q, layer: int = 0, window: int = 0, sinks: int = 0, scale: Optional[float] = None, out=None):
     """softmax(scale q . K) . V for query rows [rows][query heads][dim]: a row at position p sees tokens j <= p, with a window > 0 those of them
-    with j > p - window or j < sinks; zeros where it sees none.  scale: dim ** -0.5 if not given"""
+    with j > p - window or j < sinks; zeros where it sees none.  scale: dim ** -0.5 if not given; out does not overlap q"""
     dim = pool.head_dim
+    _sees(layer, pool.n_layers, window, sinks)
     qr, qh = _rows(q, "q", batch.rows, None, dim)
     heads = int(q.shape[1])
     if out is None:
@@ -327,7 +350,8 @@ def read(pool: KvPool, table, lens, start, count: int, layer: int = 0, dtype: st
     _array(lens, "lens", ("int32",), (n,))
     _array(start, "start", ("int32",), (n,))
     _need(dtype in _TYPES, f"{dtype} where float32, float16 or bfloat16 is wanted")
-    _need(count >= 0, "a negative count")
+    _need(0 <= count <= _INT, f"{count} tokens")
+    _sees(layer, pool.n_layers, 0, 0)
     stream, guard = _on((pool.k, table, lens, start))
     k, v = (_empty(pool.k, (n, count, pool.n_kv_heads, pool.head_dim), dtype) for _ in range(2))
     _call(guard, _lib().kv_read_hip, pool._ref, layer, table.data_ptr(), lens.data_ptr(), start.data_ptr(), n, mp, count, k.data_ptr(), v.data_ptr(), _TYPES[dtype], stream)
@@ -353,6 +377,7 @@ def trim(pool: KvPool, table, refs, lens, window: int = 0, sinks: int = 0) -> No
     """gives up, in place, the pages behind lens[r] (0: the whole row) and, with a window > 0, those that no later token of the row sees"""
     n, mp = _table(pool, table, refs)
     _array(lens, "lens", ("int32",), (n,))
+    _sees(0, 1, window, sinks)
     stream, guard = _on((table, refs, lens, pool.k))
     _call(guard, _lib().kv_trim_hip, pool._ref, table.data_ptr(), refs.data_ptr(), lens.data_ptr(), n, mp, window, sinks, stream)
 
@@ -397,6 +422,7 @@ def beam_select(logits, scores, done=None, eos: int = -1):
     if done is not None:
         _array(done, "done", ("uint8", "bool"), (groups, beams))
         arrays.append(done)
+    _need(-_INT <= eos <= _INT, f"eos {eos}")
     lib = _lib()
     stream, guard = _on(arrays)
     need = lib.beam_workspace_hip(groups, beams, vocab)

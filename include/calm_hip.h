@@ -223,7 +223,7 @@ int calm_hip_query(const char* key, int value);
  *   k_scale, v_scale  float [n_layers][n_pages][n_kv_heads][4]
  *   status   one device word that kernels OR what they find into (the host clears it): 1 a page that a call needs is missing from the
  *            table or outside the pool (rows that see it are NaN, rows for it are not stored), 2 no page was free, 4 a sequence has more
- *            new rows than the batch's max_rows, 8 a parent outside the table.
+ *            new rows than the batch's max_rows, or starts outside its rows, 8 a parent outside the table.
  * Pages need no initialisation: nothing behind a sequence's tokens is read into a result. */
 struct KvPool {
 	signed char *k, *v;
@@ -263,14 +263,14 @@ int kv_read_hip(const struct KvPool* pool, int layer, const int* table, const in
 /* Attention of the batch's query rows: a row at position p (its sequence's lens - rows + its place) sees tokens j <= p, with a window > 0
  * only j > p - window or j < sinks; out = softmax(scale * q . K) . V over them, zeros where it sees none.  n_heads query heads, a multiple
  * of the kv heads (head h reads kv head h / (n_heads / n_kv_heads)).  q strided like the rows above, out dense [n_rows][n_heads][head_dim]
- * of q's type.  Table entries of pages that no row sees may be -1.  workspace: kv_attend_workspace_hip() bytes for the same arguments
+ * of q's type, not overlapping q.  Table entries of pages that no row sees may be -1.  workspace: kv_attend_workspace_hip() bytes for the same arguments
  * (0: none), written and read within the call. */
 long long kv_attend_workspace_hip(const struct KvPool* pool, const struct KvBatch* batch, int type, int n_heads, int window, int sinks);
 int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* batch, int layer, const void* q, void* out, int type, int n_heads, long q_row, long q_head, float scale, int window,
                   int sinks, void* workspace, size_t workspace_size, void* stream);
 
 /* The upkeep of pages.  refs[p] = how many table rows list page p (int [n_pages], 0: free); a page that is not full belongs to one row.
- * Up to 2048 table rows.  Free pages are taken lowest first, rows in order.
+ * Up to 2048 table rows, 2^30 entries and pages.  Free pages are taken lowest first, rows in order.
  *   reserve  entries of the pages that tokens lens[r] .. lens_new[r] - 1 of row r need (in place)
  *   trim     gives up pages behind lens[r] (0: all of them) and, with a window > 0, those that no later token sees (in place)
  *   fork     row r becomes a copy of row parents[r] (out of place: table_out, refs_out; refs_out may be refs): full pages are shared, a

@@ -406,11 +406,74 @@ def test_batches_that_lie_are_reported(hiplib):
     paged.attend(r.pool, b, q)
     with pytest.raises(RuntimeError, match="max_rows"):
         r.pool.check()
-    # a max_len that is too small only shapes the launch
-    b = paged.KvBatch(b.table, b.lens, b.starts, rows=50, max_rows=40, max_len=1)
-    got = paged.attend(r.pool, b, q).numpy()
-    want = paged.attend(r.pool, paged.KvBatch(b.table, b.lens, b.starts, rows=50, max_rows=40, max_len=60), q).numpy()
-    np.testing.assert_allclose(got, want, rtol=0, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 9, 50])
+def test_bounds_that_are_too_small_only_shape_the_launch(hiplib, rows):
+    """a max_len far below the longest sequence: it is attended in full, cut or not"""
+    r = Rig(2, 3000, 2, 64, np.random.default_rng(18))
+    r.add([2990, 700], "float32")
+    q = dev(to_type(r.rng.standard_normal((2 * rows, 4, 64)), "float32"))
+    b = r.batch([rows, rows])
+    want = paged.attend(r.pool, b, q).numpy()
+    for most in (1, 500, 1100):
+        got = paged.attend(r.pool, paged.KvBatch(b.table, b.lens, b.starts, rows=2 * rows, max_rows=rows, max_len=most), q).numpy()
+        np.testing.assert_allclose(got, want, rtol=0, atol=1e-5)
+    r.pool.check()
+
+
+@pytest.mark.gpu
+def test_rows_outside_the_sequences_are_left_alone(hiplib):
+    """starts that begin behind row 0 and end before the last; starts that do not add up are reported"""
+    r = Rig(2, 2100, 1, 64, np.random.default_rng(19))
+    r.add([2050, 300], "float32")
+    q = dev(to_type(r.rng.standard_normal((8, 2, 64)), "float32"))
+    want = paged.attend(r.pool, r.batch([2, 3]), View(q, 2 * 128, (5, 2, 64))).numpy()
+    out = dev(np.full((8, 2, 64), 5.0, dtype=np.float32))
+    paged.attend(r.pool, paged.KvBatch(r.dtable, ints(r.lens), ints([2, 4, 7]), rows=8, max_rows=3, max_len=2100), q, out=out)
+    got = out.numpy()
+    np.testing.assert_array_equal(got[2:7], want)
+    assert (got[:2] == 5).all() and (got[7:] == 5).all()
+    r.pool.check()
+    for starts in ([0, 9, 9], [0, 5, 3], [-1, 2, 4]):
+        paged.attend(r.pool, paged.KvBatch(r.dtable, ints(r.lens), ints(starts), rows=8, max_rows=8, max_len=2100), q)
+        with pytest.raises(RuntimeError, match="max_rows"):
+            r.pool.check()
+        x = dev(np.zeros((8, 1, 64), dtype=np.float32))
+        paged.append(r.pool, paged.KvBatch(r.dtable, ints([0, 0]), ints(starts), rows=8, max_rows=8, max_len=2100), x, x)
+        with pytest.raises(RuntimeError, match="max_rows"):
+            r.pool.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [12, 60])
+def test_a_missing_page_spares_the_rows_that_do_not_see_it(hiplib, rows):
+    """rows of one tile on both sides of a window's end inside a missing page, with infinities where its stand-in's scales would be"""
+    r = Rig(1, 400, 1, 64, np.random.default_rng(20))
+    r.add([400], "float32")
+    t = r.table.copy()
+    spare = [p for p in range(r.pages) if p not in set(t[0])]
+    if 0 not in spare:  # page 0 out of use
+        t[0, list(t[0]).index(0)] = spare[0]
+        r.table = t
+        r.dtable = dev(t)
+        r.k, r.v, r.lens = Cache(1, 64), Cache(1, 64), [0]
+        r.add([400], "float32")
+    for x in (r.pool.k_scale, r.pool.v_scale):
+        one = np.full(4, np.inf, dtype=np.float32)
+        x._lib.copy_hip(x.data_ptr(), one.ctypes.data, 16)
+    t = r.table.copy()
+    t[0, 3] = -1  # tokens 192 .. 255
+    window = 400 - 255 - rows // 2  # the later half of the rows does not see them
+    q = to_type(r.rng.standard_normal((rows, 2, 64)), "float32")
+    b = r.batch([rows])
+    got = paged.attend(r.pool, paged.KvBatch(dev(t), b.lens, b.starts, rows=rows, max_rows=rows, max_len=400), dev(q), window=window).numpy()
+    want = attention(q.astype(np.float64), r.k.values(0), r.v.values(0), 0.125, window, 0)
+    p = 400 - rows + np.arange(rows)
+    sees = p - window < 255
+    assert sees.any() and (~sees).any() and np.isnan(got[sees]).all()
+    np.testing.assert_allclose(got[~sees], want[~sees], rtol=0, atol=2e-5 * np.abs(want).max())
 
 
 @pytest.mark.gpu
@@ -732,7 +795,8 @@ def test_a_search_with_all_operators(hiplib):
 class Fake:
     """an array's outside, with no memory behind it: a call that gets past its checks would have nothing to launch on"""
 
-    def __init__(self, shape, dtype, stride=None, ptr=4096, dense=True):
+    def __init__(self, shape, dtype, stride=None, ptr=4096, dense=True, device="cuda:0"):
+        self.device = device
         self.shape, self.dtype, self._ptr, self._dense = shape, dtype, ptr, dense
         s, out = 1, []
         for n in reversed(shape):
@@ -780,7 +844,7 @@ def test_entries_refuse_bad_pools_and_batches(hiplib):
     refused(hiplib.kv_append_hip(None, C.byref(b), 0, 4096, 4096, 0, 128, 64, 128, 64, None), hiplib, "missing")
     p = c_pool()
     for kw, words in [(dict(table=0), "missing"), (dict(n_seqs=0), "65535 sequences"), (dict(n_seqs=70000), "65535"), (dict(max_pages=0), "page column"), (dict(n_rows=-1), "negative"),
-                      (dict(n_seqs=60000, max_pages=60000), "2^31")]:
+                      (dict(n_seqs=60000, max_pages=60000), "2^30")]:
         bb = c_batch(**kw)
         refused(hiplib.kv_append_hip(C.byref(p), C.byref(bb), 0, 4096, 4096, 0, 128, 64, 128, 64, None), hiplib, words)
         refused(hiplib.kv_attend_workspace_hip(C.byref(p), C.byref(bb), 0, 4, 0, 0), hiplib, words)
@@ -805,6 +869,9 @@ def test_entries_refuse_bad_arguments(hiplib):
     assert need > 0
     for ws, n in ((None, need), (4096, need - 1), (4104, need)):
         refused(hiplib.kv_attend_hip(P, C.byref(long), 0, 4096, 4096, 0, 4, 256, 64, 0.1, 0, 0, ws, n, None), hiplib, "workspace")
+    # two rows of 4 heads of 64 fp32 values: 2048 bytes
+    for kw in (dict(), dict(o=4096 + 2032), dict(o=4096 - 2032), dict(qr=512, o=4096 + 2048), dict(qr=-256, o=4096 - 2048)):
+        refused(att(**kw), hiplib, "overlaps")
     refused(hiplib.kv_read_hip(P, 0, 4096, 4096, 4096, 2, 4, -1, 4096, 4096, 0, None), hiplib, "negative")
     refused(hiplib.kv_read_hip(P, 0, 4096, 0, 4096, 2, 4, 1, 4096, 4096, 0, None), hiplib, "missing")
     refused(hiplib.kv_read_hip(P, 0, 4096, 4096, 4096, 2, 4, 1, 4098, 4096, 1, None), hiplib, "aligned")
@@ -851,6 +918,13 @@ def test_python_checks():
         paged.KvBatch(t, n, st, 2, 3, 10)
     with pytest.raises(ValueError, match="contiguous"):
         paged.KvBatch(Fake((2, 4), "int32", dense=False), n, st, 2, 1, 10)
+    far = Fake((2,), "int32", device="cuda:1")
+    with pytest.raises(ValueError, match="cuda:1"):
+        paged.KvBatch(t, far, st, 2, 1, 10)
+    with pytest.raises(ValueError, match="cuda:1"):
+        paged.KvPool.over(k, v, s, Fake((2, 10, 2, 4), "float32", device="cuda:1"))
+    with pytest.raises(ValueError, match="at most"):
+        paged.KvBatch(t, n, st, 2, 1, 1 << 32)
     pool = paged.KvPool.__new__(paged.KvPool)
     pool.n_layers, pool.n_pages, pool.n_kv_heads, pool.head_dim = 2, 10, 2, 64
     b = paged.KvBatch(t, n, st, 2, 1, 10)
@@ -859,6 +933,13 @@ def test_python_checks():
                 Fake((2, 2, 64), "float16", stride=(130, 64, 1)), Fake((2, 2, 64), "float32")):
         with pytest.raises(ValueError):
             paged.append(pool, b, row, bad)
+    for kw in (dict(window=1 << 32), dict(sinks=1 << 31), dict(window=-1), dict(layer=2), dict(layer=(1 << 32) + 1), dict(layer=-1)):
+        with pytest.raises(ValueError, match="window|layer"):
+            paged.attend(pool, b, row, **kw)
+    with pytest.raises(ValueError, match="layer"):
+        paged.append(pool, b, row, row, layer=1 << 32)
+    with pytest.raises(ValueError, match="tokens"):
+        paged.read(pool, t, n, n, 1 << 32)
     with pytest.raises(ValueError, match="out"):
         paged.attend(pool, b, row, out=Fake((2, 2, 64), "float32"))
     with pytest.raises(ValueError, match="beams"):
