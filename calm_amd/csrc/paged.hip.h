@@ -417,11 +417,15 @@ __global__ __launch_bounds__(64) void k_kv_read(KvReadArgs a) {
 // j < sinks.  out = sum_j P_j V_j / sum_j P_j with P_j = 2^(x_j - m), x_j = (q . K_j) scale log2(e), m the running maximum.
 // Both products run on the matrix cores, transposed: S^T = K q^T puts a query row into a lane's column, so maximum, sum and rescaling
 // of a row are its lane's own (plus the other lanes of the same column), and the weights are already the operand layout that
-// O^T = V^T P^T wants.  Numerics: codes are exact binary16; q is one binary16 after its row is scaled by a power of two to at most 1
-// (fp16 and bf16 rows lose nothing above 2^-14 of their largest element), fp32 rows as the sum of two (22 bits); scores are fp32, times
-// the block's K scale; P_j times the block's V scale over the largest one met (E) is one binary16 for fp16 / bf16 outputs -- 2^-12 relative,
-// a third or less of the output's own rounding, since weights average -- and the sum of two for fp32; sums in fp32.  A weight below
-// 2^-14 of the largest (V scale included) keeps an absolute 2^-25 of it.
+// O^T = V^T P^T wants.  Numerics.  Codes are exact, as bytes and as binary16.  q is cut in two ways:
+//   k_kv_decode  signed digits of base 254 relative to the row's largest magnitude, d0 + d1 / 254 (+ d2 / 254^2 for fp32 rows): the scores are sums of
+//                byte products in whole numbers, exact; what is left out of q is 1.6e-5 (fp32: 6e-8) of its row's largest.  For 16-bit rows that is
+//                a 30th of what fp16 rows were rounded by near their largest element and comes up to it for elements below a 60th of that.
+//   k_kv_chunk   one binary16 after the row is scaled by a power of two to at most 1 (fp16 and bf16 rows lose nothing above 2^-14 of their largest
+//                element), fp32 rows as the sum of two (22 bits); scores are fp32 sums.
+// Scores are then fp32, times the block's K scale; P_j times the block's V scale over the largest one met (E) is one binary16 for fp16 / bf16
+// outputs -- 2^-12 relative, a third or less of the output's own rounding, since weights average -- and the sum of two for fp32; sums in
+// fp32.  A weight below 2^-14 of the largest (V scale included) keeps an absolute 2^-25 of it.
 
 struct KvAttnArgs {
 	KvLayer p;
@@ -429,7 +433,7 @@ struct KvAttnArgs {
 	const void* q;
 	void* out; // [row][head][D]
 	long q_row, q_head;
-	float* part; // [row x head][split][D + 2]: partial sums, then the maximum and the sum of weights
+	float* part; // [row x head][split][D + 4]: partial sums, then the maximum and the sum of weights
 	int n_heads, group, window, sinks, chunk, n_splits;
 	float scale; // scale * log2(e)
 };
@@ -495,9 +499,15 @@ __device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t 
 }
 
 // Few rows (one token of a sequence, or a few): the cache's bytes bound it.  A workgroup takes one sequence, one kv head, 16 rows (token x head
-// of the group) and a range of pages, dealt to its NW waves a page at a time; a wave holds a page's codes in registers as
-// the matrix operands they are, loads the next page's K behind the first product and its V behind the second, so 8 - 16 KiB per wave
-// are in flight throughout.  The waves' sums meet in LDS; ranges of one row meet in k_kv_merge.
+// of the group) and a range of pages, dealt to its NW waves a page at a time; a wave holds a page's codes in registers as the matrix
+// operands they are (no conversion: that is what whole-number scores are for), asks for the next
+// page's K behind the first product and for its V behind the second, so 8 - 16 KiB per wave are in flight throughout.  (Two sets of registers,
+// a whole page ahead: slower.)  The waves' sums meet
+// in LDS; ranges of one row meet in k_kv_merge.  Eight waves for heads up to 128: four, with twice the workgroups, lose 5 - 10 % to the
+// waits at both ends of a workgroup (64 sequences of 91 - 8191, heads of 64: 39.6 -> 36.2 us).
+// Measured, one row a sequence: 24 x 13.9 - 16.4k tokens, 8 kv heads of 128: 136 us, 746 MB = 5.5 TB/s; 8 x 4093: 18.2 us + 4.0 for the join, 67 MB = 3.0;
+// 64 x 91 - 8191, 4 of 64: 36 us, 137 MB = 3.8 (the longest sequences' chain of pages is what remains); five rows on the last 1024 and 64
+// first tokens of 6 - 9k: 13.7 us, 35 MB = 2.5.
 // grid = (splits, kv heads x tiles, seqs)
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnArgs a) {
@@ -892,12 +902,20 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 // Many rows (a prompt chunk): the matrix cores bound it.  A workgroup takes 128 rows (32 per wave) of one sequence and kv head and walks
 // the pages they see; a page's codes become binary16 ONCE per workgroup on their way into LDS (two buffers: the next page's loads are in
 // flight while a page is computed), laid out so that every operand is one 16-byte read of consecutive lanes.
+// Measured: 2049 rows of 32 heads (8 kv heads of 128) on 4099 tokens 166 - 174 us = 600 TFLOP/s; five ragged chunks of up to 1021 rows of 32 heads
+// (4 kv heads of 64) behind a window of 2048 73 us.  A page costs a wave 32 matrix instructions of 32 cycles (heads of 128) and 280 vector ones
+// of 4 (exponentials 8), and a matrix instruction keeps the vector unit for 16 of its cycles: the vector unit is what bounds it, two
+// workgroups to a CU reach 70 % of that, and the heaviest tiles (65 pages, 49 on average) end last.  Tried and slower: PV of a page with QK of
+// the next in one phase, the other phase's waves beside it behind barriers (eight waves of 256 rows: 199 us; four waves: 181), products of
+// neighbouring pages interleaved within a wave (257 us), light tiles behind heavy ones on a CU (187).
 // grid = row tiles x seqs x splits x kv heads
 template <int D>
 struct KvChunk {
 	static constexpr int KROW = 65;                // 16-byte units between two (k-step, half) columns of K: 64 tokens and one of padding
 	static constexpr int KU = D / 8 * KROW, VU = 8 * D; // units of a page's K and V
-	static constexpr size_t LDS = (size_t)2 * (KU + VU) * 16;
+	// two workgroups to a CU, never three: where there are no more than two for each, three on one CU leave others idle (five ragged chunks of up to
+	// 1021 rows, heads of 64: 90 instead of 75 us)
+	static constexpr size_t LDS = (size_t)2 * (KU + VU) * 16 < 56 * 1024 ? 56 * 1024 : (size_t)2 * (KU + VU) * 16;
 };
 
 // n operands' LDS reads, KV_AHEAD of them ahead, each feeding m matrix instructions
@@ -951,13 +969,15 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	const bool live = rr < nrows;
 	const int t = (live ? rr : nrows - 1) / a.group, hd = h * a.group + (live ? rr : nrows - 1) % a.group;
 	const int pos = len - n + t;
-	const size_t row = (size_t)(row0 + t) * a.n_heads + hd;
+	const auto row_of = [&](int r) {
+		return (size_t)(row0 + r / a.group) * a.n_heads + h * a.group + r % a.group;
+	};
 	const int wl = r0 + 32 * wave + 31 < nrows - 1 ? r0 + 32 * wave + 31 : nrows - 1;
 	const bool any = r0 + 32 * wave < nrows;
 	const int w_min = len - n + (any ? r0 + 32 * wave : 0) / a.group, w_max = any ? len - n + wl / a.group : -1;
 	if (i0 >= i1 && split > 0) {
 		if (!direct && live && hh == 0) {
-			float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
+			float* const p = a.part + (row_of(rr) * a.n_splits + split) * (D + 4) + D;
 			p[0] = -__builtin_inff(), p[1] = 0.f;
 		}
 		return;
@@ -996,7 +1016,8 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			}
 		}
 	}
-	float m = -__builtin_inff(), l = 0.f, E = 1.1754944e-38f;
+	float m = -__builtin_inff(), l = 0.f;
+	int Eb = 0x00800000; // the largest V scale met, by its bits
 	kv_f32x16 o[ND], zero;
 #pragma unroll
 	for (int e = 0; e < 16; ++e) {
@@ -1076,9 +1097,13 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	for (int i = i0; i < i1; ++i) {
 		const int buf = (i - i0) & 1;
 		const bool more = i + 1 < i1;
-		const bool bad = pid < 0;
-		const float none = __builtin_nanf("");
-		const kv_f32x4 ksc = bad ? (kv_f32x4){none, none, none, none} : ksc_n, vsc = bad ? (kv_f32x4){0.f, 0.f, 0.f, 0.f} : vsc_n;
+		// the page's scales, one of everything for the wave: their bits, in scalar registers
+		int kb[4], vb[4];
+#pragma unroll
+		for (int b = 0; b < 4; ++b) {
+			const float x = ksc_n[b], y = vsc_n[b];
+			kb[b] = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)), vb[b] = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, y));
+		}
 		int next = -1;
 		if (more) {
 			if (i + 1 >= ids0 + 64) {
@@ -1112,94 +1137,75 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			KV_FEED(2 * KS, HL ? 2 : 1);
 			__builtin_amdgcn_sched_barrier(0);
 			__builtin_amdgcn_s_setprio(0);
-			float Enew = E, least = 3e38f;
-			unsigned odd = 0;
+			kv_f16x8 pf[4], pl[HL ? 4 : 1];
+			// V's scales are powers of two: a weight takes its block's, over the largest met (E, 2^shift), into its exponent, and the sum of weights
+			// takes it out again a block at a time; all of that is whole numbers in scalar registers, beside the vector instructions.  A block
+			// that no row sees says nothing; one with the scale NaN, or of a missing page, is NaN through K, for the rows that see it.
+			int shift[4], En = Eb;
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
 				const int jb = j0 + 16 * b;
-				const bool seen = whole || (jb <= w_max && (a.window <= 0 || jb + 15 > w_min - a.window || jb < a.sinks));
-				const float vb = fabsf(vsc[b]), kb = ksc[b], vb0 = vsc[b];
-				Enew = fmaxf(Enew, seen ? vb : 0.f);
-				least = fminf(least, vb);
-				odd |= (__builtin_bit_cast(unsigned, vb0) & 0x807fffffu) | (__builtin_bit_cast(unsigned, kb) & 0x80000000u); // V: not a positive power of two, or NaN
+				const bool seen = whole || ((jb <= w_max) & ((a.window <= 0) | (jb + 15 > w_min - a.window) | (jb < a.sinks)));
+				const bool number = (unsigned)vb[b] < 0x7f800000u;
+				kb[b] = pid >= 0 && number ? kb[b] : 0x7fc00000;
+				vb[b] = pid >= 0 && number && seen ? vb[b] : 0;
+				En = max(En, vb[b]);
 			}
-			const float rE = __builtin_amdgcn_rcpf(Enew);
-			float og = E * rE;
-			E = Enew;
-			odd |= __builtin_bit_cast(unsigned, E) & 0x807fffffu;
-			// token 32 (b / 2) + 8 (e / 4) + 4 hh + e % 4 of the page is element e % 16 of tile b / 2; block b holds elements 8 (b % 2) ..
-			kv_f16x8 pf[4], pl[HL ? 4 : 1];
-			if (whole && odd == 0 && least * 65536.f >= E) {
-				// Every row sees every token, and the V scales are powers of two within 2^-16 of E: the weight's V scale goes into its
-				// exponent, and the sum of weights takes it out again a block at a time -- 96 instructions of 300 less.
-				float top = m;
+#pragma unroll
+			for (int b = 0; b < 4; ++b) {
+				shift[b] = max((vb[b] - En) >> 23, -64); // (below 2^-64 of E a V is nothing beside it, weighted or not)
+			}
+			float f[4];
+#pragma unroll
+			for (int b = 0; b < 4; ++b) {
+				const int k = kb[b];
+				f[b] = __builtin_bit_cast(float, k) * qf; // (not negative)
+			}
+			if (!whole) {
 #pragma unroll
 				for (int b = 0; b < 4; ++b) {
-					float t = sc[b >> 1][8 * (b & 1)];
-#pragma unroll
-					for (int e = 1; e < 8; ++e) {
-						t = fmaxf(t, sc[b >> 1][8 * (b & 1) + e]);
-					}
-					top = fmaxf(top, t * (ksc[b] * qf)); // (the factor is not negative)
-				}
-				top = kv_max32(top);
-				// the reference stays unless a score passes it by 2^8: weights up to 2^8 are no less exact, and the sums are seldom rescaled
-				const float ref = top > m + 8.f ? top : m; // (finite: every row sees the page)
-				const float alpha = kv_exp2(m - ref); // (m = -inf: 0)
-				m = ref;
-				l *= alpha;
-				og *= alpha;
-#pragma unroll
-				for (int b = 0; b < 4; ++b) {
-					const float f = ksc[b] * qf, fv = vsc[b] * rE;
-					const float shift = (float)((int)(__builtin_bit_cast(unsigned, fv) >> 23) - 127) - ref;
-					float sum = 0.f;
-#pragma unroll
-					for (int e = 0; e < 8; ++e) {
-						const float y = kv_exp2(__builtin_fmaf(sc[b >> 1][8 * (b & 1) + e], f, shift));
-						sum += y;
-						pf[b][e] = (_Float16)y;
-						if constexpr (HL) {
-							pl[b][e] = (_Float16)(y - (float)pf[b][e]);
-						}
-					}
-					l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(fv), l);
-				}
-			} else {
-				float top = m;
-#pragma unroll
-				for (int b = 0; b < 4; ++b) {
-					const float f = ksc[b] * qf;
 #pragma unroll
 					for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; ++e) {
 						const int j = j0 + 32 * (b >> 1) + 8 * (e >> 2) + 4 * hh + (e & 3);
-						const bool seen = j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
-						const float x = seen ? sc[b >> 1][e] * f : -__builtin_inff();
-						sc[b >> 1][e] = x;
-						top = fmaxf(top, x);
+						const bool seen = (j <= pos) & ((a.window <= 0) | (j > pos - a.window) | (j < a.sinks));
+						sc[b >> 1][e] = seen ? sc[b >> 1][e] * f[b] : -__builtin_inff();
+					}
+					f[b] = 1.f;
+				}
+			}
+			float top = m;
+#pragma unroll
+			for (int b = 0; b < 4; ++b) {
+				float t = -__builtin_inff();
+#pragma unroll
+				for (int e = 0; e < 8; ++e) {
+					t = fmaxf(t, sc[b >> 1][8 * (b & 1) + e]);
+				}
+				top = fmaxf(top, t * f[b]);
+			}
+			top = kv_max32(top);
+			// the reference stays unless a score passes it by 2^8: weights up to 2^8 are no less exact, and the sums are seldom rescaled
+			const float m0 = m;
+			m = top > m + 8.f ? top : m;
+			const float ref = m == -__builtin_inff() ? 0.f : m; // (no token seen yet)
+			const float alpha = kv_exp2(m0 - ref); // (m0 = -inf: 0)
+			const float og = alpha * __builtin_bit_cast(float, max(0x3f800000 + (Eb - En), 0));
+			Eb = En;
+			l *= alpha;
+#pragma unroll
+			for (int b = 0; b < 4; ++b) {
+				const float from = (float)shift[b] - ref;
+				float sum = 0.f;
+#pragma unroll
+				for (int e = 0; e < 8; ++e) {
+					const float y = kv_exp2(__builtin_fmaf(sc[b >> 1][8 * (b & 1) + e], f[b], from));
+					sum += y;
+					pf[b][e] = (_Float16)y;
+					if constexpr (HL) {
+						pl[b][e] = (_Float16)(y - (float)pf[b][e]);
 					}
 				}
-				top = kv_max32(top);
-				const float ref = top == -__builtin_inff() ? 0.f : top;
-				const float alpha = kv_exp2(m - ref);
-				m = top;
-				l *= alpha;
-				og *= alpha;
-#pragma unroll
-				for (int b = 0; b < 4; ++b) {
-					const float fv = vsc[b] * rE;
-#pragma unroll
-					for (int e = 0; e < 8; ++e) {
-						const float x = sc[b >> 1][8 * (b & 1) + e];
-						const float w = kv_exp2(x - ref);
-						l += w;
-						const float y = x == -__builtin_inff() ? 0.f : w * fv; // (a NaN scale must not reach a row that does not see the token)
-						pf[b][e] = (_Float16)y;
-						if constexpr (HL) {
-							pl[b][e] = (_Float16)(y - (float)pf[b][e]);
-						}
-					}
-				}
+				l = __builtin_fmaf(sum, kv_exp2i(-shift[b]), l);
 			}
 			if (__ballot(og != 1.f)) {
 #pragma unroll
@@ -1229,10 +1235,13 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 		pid = next;
 	}
 	l += __shfl_xor(l, 32);
-	if (!live) {
+	int again = rr; // (looked up anew: kept through the loop, the row would cost two registers)
+	asm volatile("" : "+v"(again));
+	if (again >= nrows) {
 		return;
 	}
-	const float f = direct ? (l == 0.f ? 0.f : E / l) : E;
+	const size_t row = row_of(again);
+	const float E = __builtin_bit_cast(float, Eb), f = direct ? (l == 0.f ? 0.f : E / l) : E;
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
 #pragma unroll

@@ -29,6 +29,7 @@ PAGE, BLOCK = 64, 16
 HEAD_DIMS = (64, 96, 128, 256)
 MAX_BEAMS = 32
 _TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_DTYPES = {}  # a name -> torch's dtype
 _NAMES = {}  # a dtype object -> its name (str(torch.float16) costs a microsecond)
 _SIZES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "int8": 1, "uint8": 1, "bool": 1}
 
@@ -168,8 +169,10 @@ def _call(guard, entry, *args) -> None:
 def _empty(like, shape, dtype: str):
     if isinstance(like, DeviceArray):
         return DeviceArray(shape, dtype)
-    torch = (_torch or _torch_calls())[0]
-    return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
+    kind = _DTYPES.get(dtype)
+    if kind is None:
+        kind = _DTYPES[dtype] = getattr((_torch or _torch_calls())[0], dtype)
+    return like.new_empty(shape, dtype=kind)
 
 
 def _need(cond, what: str) -> None:
@@ -198,20 +201,30 @@ def _array(x, name: str, dtypes, shape) -> None:
     """x is a dense array of one of `dtypes` and of `shape` (None: any size)"""
     if _name(x) not in dtypes:
         raise ValueError(f"{name}: {_name(x)} where {' or '.join(dtypes)} is wanted")
-    got = tuple(x.shape)
-    if len(got) != len(shape) or any(w is not None and w != n for n, w in zip(got, shape)):
+    got = x.shape
+    if got != shape and (len(got) != len(shape) or any(w is not None and w != n for n, w in zip(got, shape))):
+        got = tuple(got)
         raise ValueError(f"{name}: shape {got} where {tuple('any' if w is None else w for w in shape)} is wanted")
     if not x.is_contiguous():
         raise ValueError(f"{name} is not contiguous")
+
+
+def _sizes(table):
+    """rows and columns of a table"""
+    if len(table.shape) != 2:
+        raise ValueError(f"table: shape {tuple(table.shape)} where [rows][pages] is wanted")
+    _array(table, "table", ("int32",), table.shape)
+    n, mp = table.shape
+    return n, mp
 
 
 def _rows(x, name: str, rows: int, heads: Optional[int], dim: int):
     """x is [rows][heads][dim] with dense dims; its row and head strides"""
     if _name(x) not in _TYPES:
         raise ValueError(f"{name}: {_name(x)} where float32, float16 or bfloat16 is wanted")
-    shape = tuple(x.shape)
+    shape = x.shape
     if len(shape) != 3 or shape[0] < rows or shape[2] != dim or (heads is not None and shape[1] != heads):
-        raise ValueError(f"{name}: shape {shape} where ({rows}, {heads or 'heads'}, {dim}) is wanted")
+        raise ValueError(f"{name}: shape {tuple(shape)} where ({rows}, {heads or 'heads'}, {dim}) is wanted")
     r, h, d = x.stride()
     if d != 1:
         raise ValueError(f"{name}: the dims of a head are not contiguous")
@@ -241,7 +254,7 @@ class KvPool:
     @classmethod
     def over(cls, k, v, k_scale, v_scale) -> "KvPool":
         """a pool in arrays that the caller has: k int8 [layers][pages][heads][64][dim], v int8 [layers][pages][heads][4][dim][16] (byte
-        4 b + i of quad g: token 16 b + 4 g + i), scales float32 [layers][pages][heads][4]"""
+        4 b + i of quad g: token 16 b + 4 g + i), scales float32 [layers][pages][heads][4], positive powers of two or NaN"""
         self = cls.__new__(cls)
         self._set(k, v, k_scale, v_scale)
         return self
@@ -290,8 +303,7 @@ class KvBatch:
     max_len are the host's bounds (rows: what the packed row arrays hold; max_rows: of one sequence; max_len: tokens of a sequence)."""
 
     def __init__(self, table, lens, starts, rows: int, max_rows: int, max_len: int):
-        _array(table, "table", ("int32",), (None, None))
-        n, mp = (int(x) for x in table.shape)
+        n, mp = _sizes(table)
         _array(lens, "lens", ("int32",), (n,))
         _array(starts, "starts", ("int32",), (n + 1,))
         _together((table, lens, starts))
@@ -345,8 +357,7 @@ def attend(pool: KvPool, batch: KvBatch, q, layer: int = 0, window: int = 0, sin
 
 def read(pool: KvPool, table, lens, start, count: int, layer: int = 0, dtype: str = "float32"):
     """(K, V), [seqs][count][kv heads][dim]: the values of tokens start[s] .. start[s] + count - 1, zeros where sequence s has no such token"""
-    _array(table, "table", ("int32",), (None, None))
-    n, mp = (int(x) for x in table.shape)
+    n, mp = _sizes(table)
     _array(lens, "lens", ("int32",), (n,))
     _array(start, "start", ("int32",), (n,))
     _need(dtype in _TYPES, f"{dtype} where float32, float16 or bfloat16 is wanted")
@@ -359,9 +370,8 @@ def read(pool: KvPool, table, lens, start, count: int, layer: int = 0, dtype: st
 
 
 def _table(pool, table, refs):
-    _array(table, "table", ("int32",), (None, None))
     _array(refs, "refs", ("int32",), (pool.n_pages,))
-    return (int(x) for x in table.shape)
+    return _sizes(table)
 
 
 def reserve(pool: KvPool, table, refs, lens, lens_new) -> None:

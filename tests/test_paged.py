@@ -6,7 +6,10 @@ Tolerances, from the types alone.  u(t) = torch.finfo(t).eps / 2: fp32 2^-24, fp
   attention, max |out - ref| over max |V| of the row's visible values (an output is an average of them, so that is its scale):
       scores: q . K in fp32 over at most 256 dims, |error| <= 256 * 2^-24 * sum |q K|; with |scale * sum |q K|| <= S_MAX = 32 in these tests (checked
       below) a score is off by less than 32 * 256 * 2^-24 = 4.9e-4 at the very worst, sqrt(256) instead of 256 in practice; for fp32 rows q's
-      second half adds 2^-22 * 32.  A score error e changes a weight by a factor within 1 +- e.  2 e = 9.8e-4 bounds the output's error from scores
+      second half adds 2^-22 * 32.  (Few rows: q is held as base-254 digits, off by at most 0.5 / (127 * 254) = 1.55e-5 of the row's largest magnitude for 16-bit
+      rows, by 6e-8 for fp32 ones, and the products are exact.  D such errors, evenly spread, move a score by a standard deviation of
+      1.55e-5 / sqrt(3) * max|q| * |K| * scale; with max|q| <= 5 and |K| about sqrt(D) for normal rows and scale = D ** -0.5 that is 4.5e-5, four of them 1.8e-4,
+      inside the 4.9e-4 above; rows whose largest element is 8 times as large still meet 2^-9 by 2 * 1.4e-3 + averaging, and have u(t) besides.)  A score error e changes a weight by a factor within 1 +- e.  2 e = 9.8e-4 bounds the output's error from scores
       (numerator and denominator).  The weight's own rounding: 2^-12 for 16-bit outputs (to binary16), 2^-22 for fp32.  exp2, sums: n * 2^-24 with
       n <= 4100 tokens at the very worst 2.4e-4.  Bounds below: 2^-9 = 2e-3 + u(t) covers all of these for every type; the typical error is far below,
       so fp32 has to meet 2e-5 in the root mean square besides (sums of n random errors of 2^-24 .. 2^-22, weights of 16 .. 4100 tokens)."""
