@@ -355,10 +355,13 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 // grid = groups; one wave per row of the group at a time, then one wave for the group
 __global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
 	__shared__ double sm_t[BEAM_MAX * BEAM_MAX];
-	__shared__ int sm_i[BEAM_MAX * BEAM_MAX];
+	__shared__ int sm_i[BEAM_MAX * BEAM_MAX], sm_r[BEAM_MAX * BEAM_MAX];
 	__shared__ float sm_v[8][BEAM_MAX];
 	__shared__ int sm_j[8][BEAM_MAX];
 	const int lane = lane_id(), wave = wave_id(), W = a.beams, g = blockIdx.x;
+	for (int c = threadIdx.x; c < W * W; c += 512) {
+		sm_r[c] = 0;
+	}
 	for (int w = wave; w < W; w += 8) {
 		const int row = g * W + w;
 		const size_t part = (size_t)row * a.n_chunks;
@@ -449,30 +452,34 @@ __global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
 	}
 	__syncthreads();
 	// A row's list is in order, so a candidate's place in the group is its place in its own list plus, for every other row, how many of that row
-	// are better: found by halving.  Equal totals: the lower row first (its indices are lower), a row's own in its order.
-	for (int c = threadIdx.x; c < W * W; c += 512) {
-		const int w = c / W, k = c % W, at = sm_i[c];
-		if (at < 0) {
+	// are better: found by halving, a thread per candidate and other row (one per candidate: 11.8 instead of 7.8 us for 16 x 8 beams over 128256 tokens).
+	// Equal totals: the lower row first (its indices are lower), a row's own in its order.
+	for (int it = threadIdx.x; it < W * W * W; it += 512) {
+		const int c = it / W, u = it - c * W, w = c / W;
+		if (sm_i[c] < 0) {
 			continue;
 		}
 		const double t = sm_t[c];
-		int rank = k;
-		for (int u = 0; u < W && rank < W; ++u) {
-			if (u == w) {
-				continue;
-			}
-			int lo = 0, hi = W; // entries [0, lo) are better, [hi, W) are not (empty places, at the end, never are)
-			while (lo < hi) {
-				const int mid = (lo + hi) >> 1;
-				const double x = sm_t[u * W + mid];
-				const bool better = sm_i[u * W + mid] >= 0 && (x > t || (x == t && u < w));
-				lo = better ? mid + 1 : lo, hi = better ? hi : mid;
-			}
-			rank += lo;
+		int lo = 0, hi = W; // entries [0, lo) are better, [hi, W) are not (empty places, at the end, never are)
+		if (u == w) {
+			lo = hi = c - w * W;
 		}
-		if (rank < W) {
+		while (lo < hi) {
+			const int mid = (lo + hi) >> 1;
+			const double x = sm_t[u * W + mid];
+			const bool better = sm_i[u * W + mid] >= 0 && (x > t || (x == t && u < w));
+			lo = better ? mid + 1 : lo, hi = better ? hi : mid;
+		}
+		if (lo) {
+			atomicAdd(&sm_r[c], lo);
+		}
+	}
+	__syncthreads();
+	for (int c = threadIdx.x; c < W * W; c += 512) {
+		const int w = c / W, at = sm_i[c], rank = sm_r[c];
+		if (at >= 0 && rank < W) {
 			const int row = g * W + w, out = g * W + rank;
-			a.score_out[out] = (float)t;
+			a.score_out[out] = (float)sm_t[c];
 			a.parent[out] = w;
 			a.token[out] = at;
 			a.done_out[out] = (a.done && a.done[row]) || (a.eos >= 0 && at == a.eos) ? 1 : 0;

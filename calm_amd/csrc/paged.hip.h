@@ -1292,7 +1292,8 @@ __device__ __forceinline__ int kv_block_scan(int v, int* sm, int& total) {
 }
 
 // list[k] <- the k-th free page (refs == 0) in ascending order, k < want; returns how many there are (at most want).  refs written by this
-// workgroup before: barrier and fence are the caller's.
+// workgroup before: barrier and fence are the caller's.  LOCAL: refs is in LDS
+template <bool LOCAL>
 __device__ __forceinline__ int kv_free_pages(const int* refs, int n_pages, int want, int* list, int* sm) {
 	int have = 0;
 	for (int p0 = 0; p0 < n_pages && have < want; p0 += KV_BOOK * 8) {
@@ -1300,7 +1301,7 @@ __device__ __forceinline__ int kv_free_pages(const int* refs, int n_pages, int w
 		const int mine = p0 + (int)threadIdx.x * 8;
 #pragma unroll
 		for (int j = 0; j < 8; ++j) {
-			if (mine + j < n_pages && __hip_atomic_load(refs + mine + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) {
+			if (mine + j < n_pages && (LOCAL ? refs[mine + j] : __hip_atomic_load(refs + mine + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == 0) {
 				mask |= 1u << j;
 			}
 		}
@@ -1328,10 +1329,16 @@ struct KvForkArgs {
 };
 
 // (its time is round trips to memory, one behind another: parents and lengths are kept in LDS, and what does not depend on the new counts --
-// the shared part of the new table, who needs a page -- is done beside them: 13.2 -> 11.8 us for 48 rows of 19 pages)
+// the shared part of the new table, who needs a page -- is done beside them.  LOCAL: the counts are in LDS too, as many as fit, and go out
+// once: 11.8 -> 4.8 us for 48 rows of 19 pages.)
+constexpr int KV_FORK_LOCAL = 24576, KV_COMPACT_LOCAL = 12288; // pages whose bookkeeping LDS holds
+
+template <bool LOCAL>
 __global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
 	__shared__ int first[KV_MAX_ROWS], count[KV_MAX_ROWS], list[KV_MAX_ROWS], par[KV_MAX_ROWS], len[KV_MAX_ROWS], sm[KV_BOOK / 64];
+	extern __shared__ int kv_refs[];
 	const int tid = threadIdx.x, n = a.n_rows, mp = a.max_pages;
+	int* const refs = LOCAL ? kv_refs : a.refs_out;
 	for (int i = tid; i < n; i += KV_BOOK) {
 		const int p = a.parents[i], l = a.lens[i];
 		first[i] = n, count[i] = 0;
@@ -1341,7 +1348,7 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
 		}
 	}
 	for (int p = tid; p < a.n_pages; p += KV_BOOK) {
-		a.refs_out[p] = a.refs[p];
+		refs[p] = a.refs[p];
 	}
 	__syncthreads();
 	for (int i = tid; i < n; i += KV_BOOK) {
@@ -1350,7 +1357,9 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
 			atomicAdd(&count[par[i]], 1);
 		}
 	}
-	__threadfence();
+	if (!LOCAL) {
+		__threadfence();
+	}
 	__syncthreads();
 	for (int k = tid; k < n * mp; k += KV_BOOK) {
 		// counts: a full page of row r is listed by count[r] rows from now on, a page of its own by one of them at most
@@ -1365,7 +1374,7 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
 		a.table_out[k] = p;
 		if (old >= 0) {
 			if (old < a.n_pages) {
-				atomicAdd(&a.refs_out[old], d);
+				atomicAdd(&refs[old], d);
 			} else {
 				kv_flag(a.status, KV_BAD_PAGE);
 			}
@@ -1389,9 +1398,11 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
 		}
 		want += total;
 	}
-	__threadfence();
+	if (!LOCAL) {
+		__threadfence();
+	}
 	__syncthreads();
-	const int have = kv_free_pages(a.refs_out, a.n_pages, want, list, sm);
+	const int have = kv_free_pages<LOCAL>(refs, a.n_pages, want, list, sm);
 	if (have < want && tid == 0) {
 		kv_flag(a.status, KV_NO_PAGE);
 	}
@@ -1401,9 +1412,15 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_fork(KvForkArgs a) {
 		if (at >= 0 && at < have) {
 			to = list[at];
 			a.table_out[i * mp + len[par[i]] / KV_PAGE] = to;
-			a.refs_out[to] = 1;
+			refs[to] = 1;
 		}
 		a.copy[2 * i + 1] = to;
+	}
+	if constexpr (LOCAL) {
+		__syncthreads();
+		for (int p = tid; p < a.n_pages; p += KV_BOOK) {
+			a.refs_out[p] = refs[p];
+		}
 	}
 }
 
@@ -1439,7 +1456,7 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_reserve(KvReserveArgs a) {
 		// in portions of what `list` holds
 		for (int done = 0; done < total; done += KV_MAX_ROWS) {
 			const int want = total - done < KV_MAX_ROWS ? total - done : KV_MAX_ROWS;
-			const int have = kv_free_pages(a.refs, a.n_pages, want, list, sm);
+			const int have = kv_free_pages<false>(a.refs, a.n_pages, want, list, sm);
 			if (have < want && tid == 0) {
 				kv_flag(a.status, KV_NO_PAGE);
 			}
@@ -1488,15 +1505,27 @@ struct KvCompactArgs {
 	int n_rows, max_pages, n_pages;
 };
 
-// live pages at or beyond n_live (their number) move into the free ones below it, both in ascending order
+// live pages at or beyond n_live (their number) move into the free ones below it, both in ascending order.  LOCAL: counts and map are in LDS,
+// and the table's first entries are asked for at the start (12.5 -> 5.1 us for 900 pages)
+template <bool LOCAL>
 __global__ __launch_bounds__(KV_BOOK) void k_kv_compact(KvCompactArgs a) {
 	__shared__ int sm[KV_BOOK / 64];
-	const int tid = threadIdx.x, n = a.n_pages;
+	extern __shared__ int kv_book[]; // [pages] counts, [pages] map, [pages / 2] x {from, to}
+	const int tid = threadIdx.x, n = a.n_pages, cells = a.n_rows * a.max_pages;
+	int* const map = LOCAL ? kv_book + n : a.map;
+	int* const copy = LOCAL ? kv_book + 2 * n : a.copy;
+	const int early = LOCAL && tid < cells ? a.table[tid] : -1;
+	const auto refs = [&](int p) {
+		return LOCAL ? kv_book[p] : a.refs[p];
+	};
 	int live = 0;
 	for (int p0 = 0; p0 < n; p0 += KV_BOOK) {
-		const int p = p0 + tid;
+		const int p = p0 + tid, r = p < n ? a.refs[p] : 0;
+		if (LOCAL && p < n) {
+			kv_book[p] = r;
+		}
 		int total;
-		kv_block_scan(p < n && a.refs[p] > 0, sm, total);
+		kv_block_scan(r > 0, sm, total);
 		live += total;
 	}
 	if (tid == 0) {
@@ -1504,42 +1533,51 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_compact(KvCompactArgs a) {
 	}
 	int holes = 0, movers = 0;
 	for (int p0 = 0; p0 < n; p0 += KV_BOOK) {
-		const int p = p0 + tid, ref = p < n ? a.refs[p] : 0;
+		const int p = p0 + tid, ref = p < n ? refs(p) : 0; // (LOCAL: this thread's own)
 		int nh, nm;
 		const bool hole = p < live && ref <= 0, mover = p < n && p >= live && ref > 0;
 		const int h = holes + kv_block_scan(hole, sm, nh), m = movers + kv_block_scan(mover, sm, nm);
 		if (hole) {
-			a.copy[2 * h + 1] = p;
+			copy[2 * h + 1] = p;
 		}
 		if (mover) {
-			a.copy[2 * m] = p;
+			copy[2 * m] = p;
 		}
 		if (p < n) {
-			a.map[p] = p;
+			map[p] = p;
 			a.refs_out[p] = p < live ? ref : 0;
 		}
 		holes += nh, movers += nm;
 	}
-	__threadfence();
+	if (!LOCAL) {
+		__threadfence();
+	}
 	__syncthreads();
 	for (int i = tid; i < n / 2; i += KV_BOOK) {
+		int from = -1, to = -1;
 		if (i < movers) {
-			const int from = a.copy[2 * i], to = a.copy[2 * i + 1];
-			a.map[from] = to;
-			a.refs_out[to] = a.refs[from];
-		} else {
-			a.copy[2 * i + 1] = -1;
+			from = copy[2 * i], to = copy[2 * i + 1];
+			map[from] = to;
+			a.refs_out[to] = refs(from);
+		}
+		if (LOCAL) {
+			a.copy[2 * i] = from;
+		}
+		if (LOCAL || to < 0) {
+			a.copy[2 * i + 1] = to;
 		}
 	}
-	__threadfence();
+	if (!LOCAL) {
+		__threadfence();
+	}
 	__syncthreads();
-	for (int k = tid; k < a.n_rows * a.max_pages; k += KV_BOOK) {
-		const int p = a.table[k];
+	for (int k = tid; k < cells; k += KV_BOOK) {
+		const int p = LOCAL && k == tid ? early : a.table[k];
 		int q = p;
 		if (p >= n) {
 			kv_flag(a.status, KV_BAD_PAGE);
 		} else if (p >= 0) {
-			q = a.map[p];
+			q = map[p];
 		}
 		a.table_out[k] = q;
 	}

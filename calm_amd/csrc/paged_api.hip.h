@@ -369,7 +369,14 @@ extern "C" int kv_fork_hip(const struct KvPool* pool, const int* table, const in
 	KV_CHECK(table_out != table, "the new table is written beside the old one");
 	KV_CHECK(workspace && workspace_size >= (size_t)n_rows * 2 * sizeof(int) && kv_aligned(workspace, 4), "the workspace is missing or smaller than 8 bytes a row");
 	const KvForkArgs a = {table, lens, refs, parents, table_out, refs_out, (int*)workspace, pool->status, n_rows, max_pages, pool->n_pages};
-	hipLaunchKernelGGL(k_kv_fork, dim3(1), dim3(KV_BOOK), 0, (hipStream_t)stream, a);
+	if (pool->n_pages <= KV_FORK_LOCAL) {
+		if (kv_lds((const void*)k_kv_fork<true>, KV_FORK_LOCAL * sizeof(int), "kv_fork_hip")) {
+			return -1;
+		}
+		hipLaunchKernelGGL(k_kv_fork<true>, dim3(1), dim3(KV_BOOK), (size_t)pool->n_pages * sizeof(int), (hipStream_t)stream, a);
+	} else {
+		hipLaunchKernelGGL(k_kv_fork<false>, dim3(1), dim3(KV_BOOK), 0, (hipStream_t)stream, a);
+	}
 	const int rc = kv_launched("kv_fork_hip");
 	return rc ? rc : kv_copy_pages(pool, a.copy, n_rows, (hipStream_t)stream, "kv_fork_hip");
 }
@@ -383,7 +390,14 @@ extern "C" int kv_compact_hip(const struct KvPool* pool, const int* table, const
 	KV_CHECK(workspace && workspace_size >= (size_t)pool->n_pages * 2 * sizeof(int) && kv_aligned(workspace, 4), "the workspace is missing or smaller than 8 bytes a page");
 	int* const map = (int*)workspace;
 	const KvCompactArgs a = {table, refs, table_out, refs_out, n_live, map, map + pool->n_pages, pool->status, n_rows, max_pages, pool->n_pages};
-	hipLaunchKernelGGL(k_kv_compact, dim3(1), dim3(KV_BOOK), 0, (hipStream_t)stream, a);
+	if (pool->n_pages <= KV_COMPACT_LOCAL) {
+		if (kv_lds((const void*)k_kv_compact<true>, 3 * KV_COMPACT_LOCAL * sizeof(int), "kv_compact_hip")) {
+			return -1;
+		}
+		hipLaunchKernelGGL(k_kv_compact<true>, dim3(1), dim3(KV_BOOK), (size_t)pool->n_pages * 3 * sizeof(int), (hipStream_t)stream, a);
+	} else {
+		hipLaunchKernelGGL(k_kv_compact<false>, dim3(1), dim3(KV_BOOK), 0, (hipStream_t)stream, a);
+	}
 	const int rc = kv_launched("kv_compact_hip");
 	return rc || pool->n_pages < 2 ? rc : kv_copy_pages(pool, a.copy, pool->n_pages / 2, (hipStream_t)stream, "kv_compact_hip");
 }

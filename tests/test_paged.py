@@ -593,6 +593,49 @@ def test_pages_reserve_fork_trim(hiplib, rows, pages):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pages", [24576, 24577])
+def test_fork_in_a_large_pool(hiplib, pages):
+    """counts in LDS, and one page too many for that; most pages are in other hands, the free ones lie at the end"""
+    rng = np.random.default_rng(pages)
+    rows, mp = 30, 7
+    pool = paged.KvPool(1, pages, 1, 64)
+    book = Book(pages, rows, mp)
+    book.refs = [1] * (pages - 600) + [0] * 600
+    lens = [int(n) for n in rng.integers(0, 64 * mp + 1, rows)]
+    book.reserve([0] * rows, lens)
+    codes = rng.integers(-128, 128, (pages, 4096)).astype(np.int8)
+    pool.k._lib.copy_hip(pool.k.data_ptr(), codes.ctypes.data, codes.nbytes)
+    table, refs = dev(np.array(book.table, dtype=np.int32)), dev(np.array(book.refs, dtype=np.int32))
+    held = np.array(book.refs)
+    parents = [int(p) for p in rng.integers(0, rows, rows)]
+    table, refs = paged.fork(pool, table, ints(lens), refs, ints(parents))
+    for n in range(pages - 600):  # (the plain bookkeeping counts the table's rows alone)
+        held[n] = 1
+    held[pages - 600:] = 0
+    before = [list(r) for r in book.table]
+    first, want = {}, []
+    for i, p in enumerate(parents):
+        first.setdefault(p, i)
+    for i, p in enumerate(parents):
+        full = lens[p] // 64
+        book.table[i] = [x if first[p] == i or c < full else -1 for c, x in enumerate(before[p])]
+        if first[p] != i and lens[p] % 64:
+            want.append((i, full, before[p][full]))
+        for x in book.table[i]:
+            if x >= 0:
+                held[x] += 1
+    for i, c, src in want:
+        to = int(np.argmin(held))
+        held[to] = 1
+        book.table[i][c] = to
+        codes[to] = codes[src]
+    np.testing.assert_array_equal(table.numpy(), np.array(book.table))
+    np.testing.assert_array_equal(refs.numpy(), held)
+    np.testing.assert_array_equal(pool.k.numpy().reshape(pages, 4096), codes)
+    pool.check()
+
+
+@pytest.mark.gpu
 def test_pages_run_out(hiplib):
     """no free page: the entries stay -1, the pool says so, nothing else changes"""
     pool = paged.KvPool(1, 3, 1, 64)
@@ -613,7 +656,7 @@ def test_pages_run_out(hiplib):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("pages,live", [(1, 1), (2, 1), (7, 0), (7, 7), (64, 20), (2100, 1300)])
+@pytest.mark.parametrize("pages,live", [(1, 1), (2, 1), (7, 0), (7, 7), (64, 20), (2100, 1300), (12288, 9001), (12289, 9001)])
 def test_compact(hiplib, pages, live):
     rng = np.random.default_rng(pages)
     heads = 1 if pages > 100 else 3
