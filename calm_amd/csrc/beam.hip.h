@@ -17,7 +17,8 @@ namespace calm {
 constexpr int BEAM_MAX = 32;
 constexpr int BEAM_VPT = 32;              // values per thread
 constexpr int BEAM_CHUNK = 256 * BEAM_VPT; // values per workgroup
-constexpr int BEAM_HITS = 16;              // lanes of a wave that k_beam_rows looks through one by one
+constexpr int BEAM_HITS = 32;              // lanes of a wave that k_beam_rows looks through one by one
+constexpr int BEAM_LIST = 128;             // candidates that a wave of k_beam_rows keeps
 constexpr float BEAM_NONE = -__builtin_inff();
 
 struct BeamArgs {
@@ -100,6 +101,27 @@ __device__ inline void beam_sums(const BeamArgs& a, size_t part, const float* m,
 	a.sums[2 * part] = (double)M, a.sums[2 * part + 1] = s;
 }
 
+__device__ __forceinline__ unsigned beam_wave_max(unsigned v) { // over the wave's lanes, in every lane
+	const auto dpp = [](unsigned x, auto ctrl, auto row_mask) { return (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, decltype(ctrl)::value, decltype(row_mask)::value, 0xf, false); };
+	using F = std::integral_constant<int, 0xf>;
+	v = max(v, dpp(v, std::integral_constant<int, 0xb1>(), F()));
+	v = max(v, dpp(v, std::integral_constant<int, 0x4e>(), F()));
+	v = max(v, dpp(v, std::integral_constant<int, 0x141>(), F()));
+	v = max(v, dpp(v, std::integral_constant<int, 0x140>(), F()));
+	v = max(v, dpp(v, std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>()));
+	v = max(v, dpp(v, std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>()));
+	return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+// a value (no NaN) and its index as one number, larger for the better one: the value's bits in order, then the index turned round
+__device__ __forceinline__ unsigned long long beam_key(float v, int at) {
+	const unsigned b = __builtin_bit_cast(unsigned, v + 0.f); // (-0 is 0)
+	return ((unsigned long long)(b >> 31 ? ~b : b | 0x80000000u) << 32) | ~(unsigned)at;
+}
+__device__ __forceinline__ float beam_key_value(unsigned long long key) {
+	const unsigned b = (unsigned)(key >> 32);
+	return __builtin_bit_cast(float, b >> 31 ? b & 0x7fffffffu : ~b);
+}
+
 // grid = (chunks, rows)
 template <int DT>
 __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
@@ -107,8 +129,9 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	constexpr int NL = BEAM_VPT / VL;
 	__shared__ float sm_v[4 * BEAM_MAX];
 	__shared__ int sm_i[4 * BEAM_MAX];
-	__shared__ float sm_m[4], sm_c[256];
-	__shared__ int sm_ci[256], sm_n[4], sm_hl[4 * BEAM_HITS];
+	__shared__ float sm_m[4], sm_c[32];
+	__shared__ unsigned long long sm_k[4 * BEAM_LIST];
+	__shared__ int sm_n[4], sm_hl[4 * BEAM_HITS];
 	__shared__ __attribute__((aligned(16))) float sm_h[4 * BEAM_HITS][BEAM_VPT + 4];
 	__shared__ double sm_s[4];
 	const int lane = lane_id(), wave = wave_id(), chunk = blockIdx.x, row = blockIdx.y, W = a.beams;
@@ -136,24 +159,54 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	const int mis = (int)((((size_t)a.logits + row0 * ES) & 15) / ES);
 	float x[BEAM_VPT];
 	const int base = chunk * BEAM_CHUNK - mis;
+	u32x4 raw[NL];
+	const auto values = [&](int i) {
 #pragma unroll
-	for (int i = 0; i < NL; ++i) {
-		const int at = base + (i * 256 + (int)threadIdx.x) * VL;
-		if (at >= 0 && at + VL <= a.vocab) {
-			const u32x4 w = *(const u32x4*)((const char*)a.logits + (row0 + (size_t)at) * ES);
-#pragma unroll
-			for (int j = 0; j < 4; ++j) {
-				const unsigned one = w[j];
-				if constexpr (DT == KV_F32) {
-					x[i * VL + j] = __builtin_bit_cast(float, one);
-				} else {
-					kv_two<DT>(one, x[i * VL + 2 * j], x[i * VL + 2 * j + 1]);
-				}
+		for (int j = 0; j < 4; ++j) {
+			const unsigned one = raw[i][j];
+			if constexpr (DT == KV_F32) {
+				x[i * VL + j] = __builtin_bit_cast(float, one);
+			} else {
+				kv_two<DT>(one, x[i * VL + 2 * j], x[i * VL + 2 * j + 1]);
 			}
-		} else {
+		}
+	};
+	// (loads first, all of them, then what is made of them: a conversion beside its load is a wait for every one)
+	if (base >= 0 && base + BEAM_CHUNK <= a.vocab) {
 #pragma unroll
-			for (int j = 0; j < VL; ++j) {
-				x[i * VL + j] = at + j >= 0 && at + j < a.vocab ? beam_load<DT>(a.logits, row0 + at + j) : BEAM_NONE;
+		for (int i = 0; i < NL; ++i) {
+			raw[i] = *(const u32x4*)((const char*)a.logits + (row0 + (size_t)(base + (i * 256 + (int)threadIdx.x) * VL)) * ES);
+		}
+#pragma unroll
+		for (int i = 0; i < NL; ++i) {
+			values(i);
+		}
+	} else {
+#pragma unroll
+		for (int i = 0; i < NL; ++i) {
+			const int at = base + (i * 256 + (int)threadIdx.x) * VL;
+			if (at >= 0 && at + VL <= a.vocab) {
+				raw[i] = *(const u32x4*)((const char*)a.logits + (row0 + (size_t)at) * ES);
+			}
+		}
+#pragma unroll
+		for (int i = 0; i < NL; ++i) {
+			const int at = base + (i * 256 + (int)threadIdx.x) * VL;
+			if (at >= 0 && at + VL <= a.vocab) {
+				values(i);
+			} else {
+#pragma unroll
+				for (int j = 0; j < VL; ++j) {
+					x[i * VL + j] = BEAM_NONE;
+				}
+				if (at + VL > 0 && at < a.vocab) { // across an end of the row
+#pragma unroll
+					for (int j = 0; j < VL; ++j) {
+						const int k = at + j < 0 ? 0 : at + j < a.vocab ? at + j : a.vocab - 1;
+						const float one = beam_load<DT>(a.logits, row0 + k);
+						x[i * VL + j] = k == at + j ? one : BEAM_NONE;
+					}
+				}
 			}
 		}
 	}
@@ -177,8 +230,10 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	}
 	// The chunk's W best.  Its lanes are cut into groups, at least W of them; each group's largest value reaches the least of these, so at least W
 	// values of the chunk reach that bound.  What does (three times W on average, unless many are equal) goes to a list in LDS, a
-	// quarter a wave, where a candidate's place is the number of better ones.  Where a quarter would be longer than 64 -- equal values, the
-	// few values of a row's end -- rounds over all values find the best instead.  (One list with an atomic counter: 7 us more.)
+	// quarter a wave, as keys in order (beam_key), where a candidate's place is the number of larger ones.  Where a quarter would be longer than
+	// BEAM_LIST -- equal values, the few values of a row's end -- rounds over all values find the best instead.  (One list with an atomic
+	// counter: 7 us more for 16 x 8 beams over 128256.  Quarters of 64: one workgroup in 40 left for the rounds at 32 beams, and 4 x 32 over 32000
+	// took 112 instead of 20 us.)
 	float bound;
 	{
 		// (register moves across the lanes: through the LDS crossbar these few steps took as long as the logits)
@@ -207,7 +262,6 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 		const float least = -wave_max_dpp((lane & 7) < 64 / size && lane < 32 ? -sm_c[lane] : -__builtin_inff());
 		bound = least;
 	}
-	__syncthreads(); // (sm_c is the list from here on)
 	const auto place = [&](int i) { // the row's index of this lane's value i
 		return base + ((i / VL) * 256 + (int)threadIdx.x) * VL + i % VL;
 	};
@@ -217,8 +271,8 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 		const unsigned long long who = __ballot(in);
 		if (who) {
 			const int k = mine_n + __builtin_popcountll(who & ((1ull << lane) - 1));
-			if (in && k < 64) {
-				sm_c[wave * 64 + k] = v, sm_ci[wave * 64 + k] = at;
+			if (in && k < BEAM_LIST) {
+				sm_k[wave * BEAM_LIST + k] = beam_key(v, at);
 			}
 			mine_n += __builtin_popcountll(who);
 		}
@@ -259,22 +313,21 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	}
 	__syncthreads();
 	const int n0 = sm_n[0], n1 = sm_n[1], n2 = sm_n[2], n3 = sm_n[3], n = n0 + n1 + n2 + n3;
-	if (n0 <= 64 && n1 <= 64 && n2 <= 64 && n3 <= 64) {
+	if (n0 <= BEAM_LIST && n1 <= BEAM_LIST && n2 <= BEAM_LIST && n3 <= BEAM_LIST) {
 		const int t = threadIdx.x;
-		if (lane < mine_n) {
-			const float v = sm_c[t];
-			const int at = sm_ci[t];
+		for (int c = lane; c < mine_n; c += 64) {
+			const unsigned long long key = sm_k[wave * BEAM_LIST + c];
 			int rank = 0;
 #pragma unroll
 			for (int w = 0; w < 4; ++w) {
 				const int nw = w == 0 ? n0 : w == 1 ? n1 : w == 2 ? n2 : n3;
 #pragma unroll 4
 				for (int k = 0; k < nw; ++k) {
-					rank += beam_better(sm_c[w * 64 + k], sm_ci[w * 64 + k], v, at) ? 1 : 0;
+					rank += sm_k[w * BEAM_LIST + k] > key ? 1 : 0;
 				}
 			}
 			if (rank < W) {
-				a.val[part * W + rank] = v, a.idx[part * W + rank] = at;
+				a.val[part * W + rank] = beam_key_value(key), a.idx[part * W + rank] = (int)~(unsigned)key;
 			}
 		}
 		if (t >= n && t < W) { // fewer than W values in all
@@ -353,16 +406,16 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 }
 
 // grid = groups; one wave per row of the group at a time, then one wave for the group
-__global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
+__global__ __launch_bounds__(1024) void k_beam_pick(BeamArgs a) {
 	__shared__ double sm_t[BEAM_MAX * BEAM_MAX];
-	__shared__ int sm_i[BEAM_MAX * BEAM_MAX], sm_r[BEAM_MAX * BEAM_MAX];
-	__shared__ float sm_v[8][BEAM_MAX];
-	__shared__ int sm_j[8][BEAM_MAX];
-	const int lane = lane_id(), wave = wave_id(), W = a.beams, g = blockIdx.x;
-	for (int c = threadIdx.x; c < W * W; c += 512) {
+	__shared__ int sm_i[BEAM_MAX * BEAM_MAX], sm_r[16 * 16];
+	__shared__ float sm_v[16][BEAM_MAX];
+	__shared__ int sm_j[16][BEAM_MAX];
+	const int lane = lane_id(), wave = wave_id(), W = a.beams, g = blockIdx.x, threads = blockDim.x;
+	for (int c = threadIdx.x; c < 256; c += threads) {
 		sm_r[c] = 0;
 	}
-	for (int w = wave; w < W; w += 8) {
+	for (int w = wave; w < W; w += threads / 64) {
 		const int row = g * W + w;
 		const size_t part = (size_t)row * a.n_chunks;
 		const int nc = a.n_chunks * W;
@@ -374,6 +427,13 @@ __global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
 			at_n = ok ? a.idx[part * W + c + lane] : -1;
 		};
 		fetch(0);
+		// (at least W candidates reach the least of the chunks' values at place `deep`)
+		float bound = -BEAM_NONE;
+		const int deep = (W + a.n_chunks - 1) / a.n_chunks - 1;
+		for (int c = lane; c < a.n_chunks; c += 64) {
+			bound = fminf(bound, a.val[(part + c) * W + deep]);
+		}
+		bound = -wave_max_dpp(-bound);
 		// log of the sum over the chunks, by the same order of additions for every row
 		float top = BEAM_NONE; // (the maxima are fp32 numbers)
 		for (int c = lane; c < a.n_chunks; c += 64) {
@@ -404,15 +464,7 @@ __global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
 			// only what beats the last of the best so far matters
 			const float wv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bv), W - 1));
 			const int wi = __builtin_amdgcn_readlane(bi, W - 1);
-			bool in = at >= 0 && (wi < 0 || beam_better(v, at, wv, wi));
-			if (wi < 0) { // nothing to beat yet: the portion's W-th largest value
-				float left = in ? v : BEAM_NONE, low = BEAM_NONE;
-				for (int k = 0; k < W; ++k) {
-					low = wave_max_dpp(left);
-					left = lane == __builtin_ctzll(__ballot(left == low)) ? BEAM_NONE : left;
-				}
-				in = in && v >= low;
-			}
+			const bool in = at >= 0 && v >= bound && (wi < 0 || beam_better(v, at, wv, wi));
 			const unsigned long long who = __ballot(in);
 			if (!who) {
 				continue;
@@ -451,38 +503,63 @@ __global__ __launch_bounds__(512) void k_beam_pick(BeamArgs a) {
 		}
 	}
 	__syncthreads();
-	// A row's list is in order, so a candidate's place in the group is its place in its own list plus, for every other row, how many of that row
-	// are better: found by halving, a thread per candidate and other row (one per candidate: 11.8 instead of 7.8 us for 16 x 8 beams over 128256 tokens).
-	// Equal totals: the lower row first (its indices are lower), a row's own in its order.
-	for (int it = threadIdx.x; it < W * W * W; it += 512) {
-		const int c = it / W, u = it - c * W, w = c / W;
-		if (sm_i[c] < 0) {
-			continue;
+	// The rows' lists are in order.  Up to 16 rows: a candidate's place in the group is its place in its own list plus, for every other row, how many
+	// of that row are better, found by halving, a thread per candidate and other row.  More: one wave, a row a lane, takes the best of their
+	// heads W times.  Equal totals: the lower row first (its indices are lower), a row's own in its order.  Measured, the one and the other, this whole
+	// kernel: 16 x 8 rows of 16 chunks 5.8 / 7.7 us, 5 x 16 rows of 4 14.5 / 16.3, 4 x 32 rows of 4 158 / 40.
+	if (W <= 16) {
+		for (int it = threadIdx.x; it < W * W * W; it += threads) {
+			const int c = it / W, u = it - c * W, w = c / W;
+			if (sm_i[c] < 0) {
+				continue;
+			}
+			const double t = sm_t[c];
+			int lo = 0, hi = W; // entries [0, lo) are better, [hi, W) are not (empty places, at the end, never are)
+			if (u == w) {
+				lo = hi = c - w * W;
+			}
+			while (lo < hi) {
+				const int mid = (lo + hi) >> 1;
+				const double x = sm_t[u * W + mid];
+				const bool better = sm_i[u * W + mid] >= 0 && (x > t || (x == t && u < w));
+				lo = better ? mid + 1 : lo, hi = better ? hi : mid;
+			}
+			if (lo) {
+				atomicAdd(&sm_r[c], lo);
+			}
 		}
-		const double t = sm_t[c];
-		int lo = 0, hi = W; // entries [0, lo) are better, [hi, W) are not (empty places, at the end, never are)
-		if (u == w) {
-			lo = hi = c - w * W;
+		__syncthreads();
+		for (int c = threadIdx.x; c < W * W; c += threads) {
+			const int w = c / W, at = sm_i[c], rank = sm_r[c];
+			if (at >= 0 && rank < W) {
+				const int row = g * W + w, out = g * W + rank;
+				a.score_out[out] = (float)sm_t[c];
+				a.parent[out] = w;
+				a.token[out] = at;
+				a.done_out[out] = (a.done && a.done[row]) || (a.eos >= 0 && at == a.eos) ? 1 : 0;
+			}
 		}
-		while (lo < hi) {
-			const int mid = (lo + hi) >> 1;
-			const double x = sm_t[u * W + mid];
-			const bool better = sm_i[u * W + mid] >= 0 && (x > t || (x == t && u < w));
-			lo = better ? mid + 1 : lo, hi = better ? hi : mid;
-		}
-		if (lo) {
-			atomicAdd(&sm_r[c], lo);
-		}
+		return;
 	}
-	__syncthreads();
-	for (int c = threadIdx.x; c < W * W; c += 512) {
-		const int w = c / W, at = sm_i[c], rank = sm_r[c];
-		if (at >= 0 && rank < W) {
-			const int row = g * W + w, out = g * W + rank;
-			a.score_out[out] = (float)sm_t[c];
-			a.parent[out] = w;
+	if (wave != 0) {
+		return;
+	}
+	int k = 0, at = lane < W ? sm_i[lane * W] : -1;
+	double t = lane < W ? sm_t[lane * W] : 0.;
+	for (int r = 0; r < W; ++r) {
+		const unsigned long long b = __builtin_bit_cast(unsigned long long, t + 0.), key = at < 0 ? 0ull : b >> 63 ? ~b : b | 1ull << 63;
+		const unsigned hi = (unsigned)(key >> 32), lo = (unsigned)key;
+		const unsigned top = beam_wave_max(hi), low = beam_wave_max(hi == top ? lo : 0u);
+		const unsigned long long who = __ballot(at >= 0 && hi == top && lo == low);
+		if (who && lane == __builtin_ctzll(who)) {
+			const int row = g * W + lane, out = g * W + r;
+			a.score_out[out] = (float)t;
+			a.parent[out] = lane;
 			a.token[out] = at;
 			a.done_out[out] = (a.done && a.done[row]) || (a.eos >= 0 && at == a.eos) ? 1 : 0;
+			++k;
+			at = k < W ? sm_i[lane * W + k] : -1;
+			t = k < W ? sm_t[lane * W + k] : 0.;
 		}
 	}
 }

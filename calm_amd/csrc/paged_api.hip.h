@@ -439,6 +439,6 @@ extern "C" int beam_select_hip(const void* logits, int type, long row, int group
 	} else {
 		hipLaunchKernelGGL(k_beam_rows<KV_BF16>, grid, dim3(256), 0, st, a);
 	}
-	hipLaunchKernelGGL(k_beam_pick, dim3(groups), dim3(512), 0, st, a);
+	hipLaunchKernelGGL(k_beam_pick, dim3(groups), dim3(64 * (beams < 16 ? beams : 16)), 0, st, a);
 	return kv_launched("beam_select_hip");
 }
