@@ -500,14 +500,13 @@ __device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t 
 
 // Few rows (one token of a sequence, or a few): the cache's bytes bound it.  A workgroup takes one sequence, one kv head, 16 rows (token x head
 // of the group) and a range of pages, dealt to its NW waves a page at a time; a wave holds a page's codes in registers as the matrix
-// operands they are (no conversion: that is what whole-number scores are for), asks for the next
-// page's K behind the first product and for its V behind the second, so 8 - 16 KiB per wave are in flight throughout.  (Two sets of registers,
-// a whole page ahead: slower.)  The waves' sums meet
-// in LDS; ranges of one row meet in k_kv_merge.  Eight waves for heads up to 128: four, with twice the workgroups, lose 5 - 10 % to the
+// operands they are (no conversion: that is what whole-number scores are for), asks for the next page's K behind the first product and for its
+// V behind the second, so 8 - 16 KiB per wave are in flight throughout.  (Two sets of registers, a whole page ahead: slower.)  The waves' sums
+// meet in LDS; ranges of one row meet in k_kv_merge.  Eight waves for heads up to 128: four, with twice the workgroups, lose 5 - 10 % to the
 // waits at both ends of a workgroup (64 sequences of 91 - 8191, heads of 64: 39.6 -> 36.2 us).
 // Measured, one row a sequence: 24 x 13.9 - 16.4k tokens, 8 kv heads of 128: 136 us, 746 MB = 5.5 TB/s; 8 x 4093: 18.2 us + 4.0 for the join, 67 MB = 3.0;
-// 64 x 91 - 8191, 4 of 64: 36 us, 137 MB = 3.8 (the longest sequences' chain of pages is what remains); five rows on the last 1024 and 64
-// first tokens of 6 - 9k: 13.7 us, 35 MB = 2.5.
+// 64 x 91 - 8191, 4 of 64: 36 us, 137 MB = 3.8 (the longest sequences' chain of pages is what remains); up to five rows of 16 x 6 - 9k under a window of
+// 1024: 13.7 us, 35 MB = 2.5.
 // grid = (splits, kv heads x tiles, seqs)
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnArgs a) {
