@@ -122,6 +122,7 @@ __device__ __forceinline__ float beam_key_value(unsigned long long key) {
 	return __builtin_bit_cast(float, b >> 31 ? b & 0x7fffffffu : ~b);
 }
 
+// Measured: 128 rows of 128256 fp32 logits 16.8 us = 3.9 TB/s, 80 rows of 32000 at 16 beams 10 us, 4 rows of 32000 5.
 // grid = (chunks, rows)
 template <int DT>
 __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	}
 }
 
-// grid = groups; one wave per row of the group at a time, then one wave for the group
+// grid = groups; a wave per row of the group (16 at a time), then the group's join
 __global__ __launch_bounds__(1024) void k_beam_pick(BeamArgs a) {
 	__shared__ double sm_t[BEAM_MAX * BEAM_MAX];
 	__shared__ int sm_i[BEAM_MAX * BEAM_MAX], sm_r[16 * 16];

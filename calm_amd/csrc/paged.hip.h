@@ -184,7 +184,7 @@ __device__ __forceinline__ void kv_rows_of(const KvRows& r, int s, int& row0, in
 // magnitude of the block's new values, the scale, codes out.  Bytes bound it (a token's rows once in, a quarter or half of them out); a lane
 // takes four tokens x four dims, so K goes out as a dword per token and V as a dword per dim without crossing lanes.  Where all four blocks
 // get new tokens (a prompt's pages) V's dwords meet in LDS and go out as whole lines: four bytes every sixteen cost 5 of 48 us for the
-// 15k tokens of six prompts, 8 heads of 128.
+// 15k tokens of six prompts, 8 heads of 128.  Measured: those 26.6 us, 86 MB = 3.2 TB/s (fp16 in), one fp32 token of 48 sequences 6.1 us (two round trips).
 // grid = (pages touched at most, kv heads)
 template <int D, int DT>
 __global__ __launch_bounds__(256, DT == KV_F32 || D > 128 ? 1 : D == 96 ? 7 : 8) void k_kv_append(KvAppendArgs a) {
@@ -353,7 +353,8 @@ struct KvReadArgs {
 	int n_seqs, max_pages, count;
 };
 
-// values of positions start[s] .. start[s] + count - 1 of every sequence, zeros outside [0, lens[s]); a wave per (sequence, cache block, kv head)
+// values of positions start[s] .. start[s] + count - 1 of every sequence, zeros outside [0, lens[s]); a wave per (sequence, cache block, kv head):
+// bytes bound it.  Measured: 203 MB (six sequences of up to 4.1k tokens, fp32 out) 47.5 us = 4.3 TB/s; the last tokens of 48 sequences 7.9 us
 // grid = (blocks, kv heads, seqs)
 template <int D, int DT>
 __global__ __launch_bounds__(64) void k_kv_read(KvReadArgs a) {
@@ -850,7 +851,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 	}
 }
 
-// the ranges of a row put together; a wave per row, the ranges' maxima across its lanes (n_splits <= 64)
+// the ranges of a row put together; a wave per row, the ranges' maxima across its lanes (n_splits <= 64).  Measured: 256 rows of 128 in four
+// ranges 3.9 us, the launch and two round trips
 template <int D, int DT>
 __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 	const int lane = lane_id();
@@ -1590,6 +1592,7 @@ struct KvCopyArgs {
 	int scales;         // floats of a page's scales of one layer
 };
 
+// the bytes of the pages that move.  Measured: 315 MB (150 pages, 8 layers of 8 heads of 128) 66 us = 4.8 TB/s, 76 MB 17.8 us = 4.3
 // grid = (copies at most, pieces of a page, layers): piece = 16 KiB of K and of V
 constexpr int KV_PIECE = 16384;
 __global__ __launch_bounds__(256) void k_kv_copy(KvCopyArgs a) {
