@@ -505,7 +505,7 @@ __device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t 
 // V behind the second, so 8 - 16 KiB per wave are in flight throughout.  (Two sets of registers, a whole page ahead: slower.)  The waves' sums
 // meet in LDS; ranges of one row meet in k_kv_merge.  Eight waves for heads up to 128: four, with twice the workgroups, lose 5 - 10 % to the
 // waits at both ends of a workgroup (64 sequences of 91 - 8191, heads of 64: 39.6 -> 36.2 us).
-// Measured, one row a sequence: 24 x 13.9 - 16.4k tokens, 8 kv heads of 128: 136 us, 746 MB = 5.5 TB/s; 8 x 4093: 18.2 us + 4.0 for the join, 67 MB = 3.0;
+// Measured, one row a sequence: 24 x 13.9 - 16.4k tokens, 8 kv heads of 128: 136 us, 746 MB = 5.5 TB/s; 8 x 4093 (fp32): 17.8 us + 3.9 for the join, 67 MB = 3.1;
 // 64 x 91 - 8191, 4 of 64: 36 us, 137 MB = 3.8 (the longest sequences' chain of pages is what remains); up to five rows of 16 x 6 - 9k under a window of
 // 1024: 13.7 us, 35 MB = 2.5.
 // grid = (splits, kv heads x tiles, seqs)
@@ -595,6 +595,19 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 		vsc = *(const kv_f32x4*)(a.p.vs + page * 4);
 	};
+	// fp32 rows are asked for ahead of the codes -- loads come back in order, and the three digits are made while the codes are on their way -- 16-bit
+	// rows behind them (8 fp32 rows on 4093 tokens 17.8 instead of 19.0 us; up to five 16-bit rows under a window 14.0 instead of 13.7)
+	KvQuad<DT> qw[D / 16];
+	const size_t at = (row / a.n_heads) * (size_t)a.q_row + (row % a.n_heads) * (size_t)a.q_head + g * (D / 4);
+	const auto load_q = [&]() {
+#pragma unroll
+		for (int i = 0; i < D / 16; ++i) {
+			qw[i].load(a.q, at + 4 * i);
+		}
+	};
+	if constexpr (HL) {
+		load_q();
+	}
 	int pid = -1;
 	if (i0 + wave < i1) {
 		fetch_ids(i0 + wave);
@@ -603,16 +616,18 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		load_v(pid);
 	}
 	__builtin_amdgcn_sched_barrier(0); // (the loads stay ahead of what follows)
+	if constexpr (!HL) {
+		load_q();
+	}
 	// q as NQ signed digits of eight bits, row / 2^e = (d0 + d1 / 254 + d2 / 254^2) / 127: lane (col, g) holds dims g D / 4 .. of its row
 	constexpr int NQ = HL ? 3 : 2;
 	unsigned qd[NQ][KW];
 	float x[D / 4];
-	const size_t at = (row / a.n_heads) * (size_t)a.q_row + (row % a.n_heads) * (size_t)a.q_head + g * (D / 4);
 	unsigned top = 0;
 #pragma unroll
 	for (int i = 0; i < D / 16; ++i) {
 		float y[4];
-		kv_load4<DT>(a.q, at + 4 * i, y);
+		qw[i].get(y);
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
 			x[4 * i + j] = y[j];
