@@ -861,7 +861,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		kv_put<D, DT>(a, direct, at, split, d, y);
 		if (d == 0 && a.n_splits > 1) {
 			float* const pm = a.part + (at * a.n_splits + split) * (D + 4) + D;
-			pm[0] = direct ? __builtin_inff() : M, pm[1] = L; // +inf: the row is written already
+			pm[0] = M, pm[1] = direct ? -1.f : L; // (no sum of weights is negative: the row is written already)
 		}
 	}
 }
@@ -881,7 +881,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 	if (lane < a.n_splits) {
 		m = p[(size_t)lane * (D + 4) + D], l = p[(size_t)lane * (D + 4) + D + 1];
 	}
-	if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, m), 0) == 0x7f800000) {
+	if (__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), 0)) < 0.f) {
 		return; // one range: written by its workgroup
 	}
 	const bool empty = m == -__builtin_inff() && l == 0.f;
@@ -1268,7 +1268,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	}
 	if (hh == 0 && a.n_splits > 1) {
 		float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
-		p[0] = direct ? __builtin_inff() : m, p[1] = l;
+		p[0] = m, p[1] = direct ? -1.f : l; // (as above)
 	}
 }
 
