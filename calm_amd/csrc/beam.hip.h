@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 				tok = i == 0 ? a.eos : (i - 1 < a.eos ? i - 1 : i);
 			}
 			a.idx[part * W + i] = tok < a.vocab ? tok : -1;
-			a.val[part * W + i] = i == 0 ? 0.f : BEAM_NONE;
+			a.val[part * W + i] = chunk == 0 && i == 0 ? 0.f : BEAM_NONE; // (k_beam_pick's bound takes values without a look at their tokens)
 		}
 		if (threadIdx.x == 0) {
 			a.sums[2 * part] = chunk == 0 ? 0. : (double)BEAM_NONE;

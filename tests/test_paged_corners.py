@@ -30,3 +30,20 @@ def test_rows_whose_scores_overflow_are_nan(hiplib, rows, tokens):
     paged.attend(r.pool, r.batch([rows]), dev(q), out=out)
     assert np.isnan(out.numpy()).all()
     r.pool.check()
+
+
+# ---- selection ------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beams,vocab", [(2, 9000), (8, 128256), (1, 20000), (32, 9000)])
+def test_select_a_finished_beam_beside_dead_ones(hiplib, beams, vocab):
+    """as many chunks of the vocabulary as beams, or more: behind the finished beam's end token come its other tokens, at -inf, the lowest first"""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((2 * beams, vocab))
+    scores = np.full((2, beams), -np.inf)
+    done = np.zeros((2, beams))
+    scores[0, 0], done[0, 0] = -3.0, 1
+    scores[1, -1], done[1, -1] = -2.0, 1
+    for eos in (0, 1, vocab - 1):
+        check_select(x, scores, done, eos)
