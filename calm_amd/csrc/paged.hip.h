@@ -455,15 +455,6 @@ struct KvSpan {
 	}
 };
 
-template <int DT, int N>
-__device__ __forceinline__ float kv_row_top(const float (&x)[N]) {
-	float m = 0.f;
-#pragma unroll
-	for (int i = 0; i < N; ++i) {
-		m = fmaxf(m, fabsf(x[i]));
-	}
-	return m;
-}
 // maximum with the lane 32 (16) away: a swap of register halves, no trip through the LDS crossbar
 __device__ __forceinline__ float kv_max32(float v) {
 	const unsigned b = __builtin_bit_cast(unsigned, v);
@@ -853,7 +844,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 		const int t = (r0 + rr) / a.group;
 		const size_t at = (size_t)(row0 + t) * a.n_heads + h * a.group + (r0 + rr) % a.group;
-		const float f = direct ? (L == 0.f ? 0.f : EM / L) : EM; // (no token seen: zeros)
+		// (no token seen: zeros.  Tokens seen, and every score beyond fp32 below: NaN; k_kv_merge knows by a sum of -0)
+		const bool blind = L == 0.f && len - n + t < 0;
+		const float f = direct ? (L == 0.f ? (blind ? 0.f : __builtin_nanf("")) : EM / L) : EM;
 #pragma unroll
 		for (int e = 0; e < 4; ++e) {
 			y[e] *= f;
@@ -861,7 +854,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		kv_put<D, DT>(a, direct, at, split, d, y);
 		if (d == 0 && a.n_splits > 1) {
 			float* const pm = a.part + (at * a.n_splits + split) * (D + 4) + D;
-			pm[0] = M, pm[1] = direct ? -1.f : L; // (no sum of weights is negative: the row is written already)
+			pm[0] = M, pm[1] = direct ? -1.f : L == 0.f && !blind ? -0.f : L; // (no sum of weights is negative: the row is written already)
 		}
 	}
 }
@@ -881,7 +874,8 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 	if (lane < a.n_splits) {
 		m = p[(size_t)lane * (D + 4) + D], l = p[(size_t)lane * (D + 4) + D + 1];
 	}
-	if (__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), 0)) < 0.f) {
+	const int l0 = __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), 0); // (the first range's)
+	if (__builtin_bit_cast(float, l0) < 0.f) {
 		return; // one range: written by its workgroup
 	}
 	const bool empty = m == -__builtin_inff() && l == 0.f;
@@ -906,7 +900,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 		}
 	}
 	if (d < D) {
-		const float f = L == 0.f ? 0.f : 1.f / L;
+		const float f = L == 0.f ? (l0 < 0 ? __builtin_nanf("") : 0.f) : 1.f / L; // (-0: tokens seen, no score in range)
 #pragma unroll
 		for (int e = 0; e < 4; ++e) {
 			y[e] *= f;
@@ -1003,17 +997,22 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	{
 		const size_t at = (size_t)(row0 + t) * (size_t)a.q_row + (size_t)hd * (size_t)a.q_head + hh * 8;
 		// (the row is read twice: its largest magnitude first -- half a row of fp32 in registers beside everything else would not fit)
-		float top = 0.f;
+		float top = 0.f, odd = 0.f; // odd: NaN once an infinity or a NaN came by (fmaxf passes over a NaN)
 #pragma unroll 4
 		for (int i = 0; i < 2 * KS; ++i) {
 			float y[4];
 			kv_load4<DT>(a.q, at + 16 * (i >> 1) + 4 * (i & 1), y);
-			top = fmaxf(top, kv_row_top<DT>(y));
+#pragma unroll
+			for (int c = 0; c < 4; ++c) {
+				top = fmaxf(top, fabsf(y[c]));
+				odd = __builtin_fmaf(y[c], 0.f, odd);
+			}
 		}
 		top = kv_max32(top);
+		odd += __shfl_xor(odd, 32);
 		const int e = kv_row_exp(top);
 		const float inv = kv_exp2i(-e);
-		qf = kv_exp2i(e) * fabsf(a.scale);
+		qf = kv_exp2i(e) * fabsf(a.scale) + odd; // (a row with an infinity or a NaN is NaN)
 		const float sign = a.scale < 0.f ? -inv : inv;
 #pragma unroll
 		for (int i = 0; i < KS; ++i) {
@@ -1257,7 +1256,8 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 		return;
 	}
 	const size_t row = row_of(again);
-	const float E = __builtin_bit_cast(float, Eb), f = direct ? (l == 0.f ? 0.f : E / l) : E;
+	const bool blind = l == 0.f && len - n + again / a.group < 0;
+	const float E = __builtin_bit_cast(float, Eb), f = direct ? (l == 0.f ? (blind ? 0.f : __builtin_nanf("")) : E / l) : E;
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
 #pragma unroll
@@ -1268,7 +1268,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	}
 	if (hh == 0 && a.n_splits > 1) {
 		float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
-		p[0] = m, p[1] = direct ? -1.f : l; // (as above)
+		p[0] = m, p[1] = direct ? -1.f : l == 0.f && !blind ? -0.f : l; // (as above)
 	}
 }
 

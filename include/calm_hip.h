@@ -261,8 +261,8 @@ int kv_read_hip(const struct KvPool* pool, int layer, const int* table, const in
                 void* stream);
 
 /* Attention of the batch's query rows: a row at position p (its sequence's lens - rows + its place) sees tokens j <= p, with a window > 0
- * only j > p - window or j < sinks; out = softmax(scale * q . K) . V over them, zeros where it sees none.  n_heads query heads, a multiple
- * of the kv heads (head h reads kv head h / (n_heads / n_kv_heads)).  q strided like the rows above, out dense [n_rows][n_heads][head_dim]
+ * only j > p - window or j < sinks; out = softmax(scale * q . K) . V over them, zeros where it sees none; NaN for a row with an infinity
+ * or a NaN, and for one with a score beyond fp32's range above or all of them below.  n_heads query heads, a multiple of the kv heads (head h reads kv head h / (n_heads / n_kv_heads)).  q strided like the rows above, out dense [n_rows][n_heads][head_dim]
  * of q's type, not overlapping q.  Table entries of pages that no row sees may be -1.  workspace: kv_attend_workspace_hip() bytes for the same arguments
  * (0: none), written and read within the call. */
 long long kv_attend_workspace_hip(const struct KvPool* pool, const struct KvBatch* batch, int type, int n_heads, int window, int sinks);

@@ -32,6 +32,45 @@ def test_rows_whose_scores_overflow_are_nan(hiplib, rows, tokens):
     r.pool.check()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 45])
+@pytest.mark.parametrize("tokens", [90, 4100])
+def test_a_row_with_an_infinity_is_nan(hiplib, dtype, rows, tokens):
+    """whatever its sign and the keys' signs; the other rows are what they are without it"""
+    r = Rig(1, tokens, 1, 64, np.random.default_rng(32))
+    k = r.rng.standard_normal((tokens, 1, 64))
+    k[:, :, 5] = np.abs(k[:, :, 5]) + 0.5  # (-inf times these: a row whose scores are all -inf)
+    r.add([tokens], "float32", k=to_type(k, "float32"))
+    q = to_type(r.rng.standard_normal((rows, 4, 64)), dtype)
+    clean = paged.attend(r.pool, r.batch([rows]), dev(q, dtype)).numpy()
+    bad = np.array(q)
+    for h, x in ((1, np.inf), (2, -np.inf), (3, np.nan)):
+        bad[rows // 2, h, 5] = to_type(np.full(1, x), dtype)[0]
+    out = marked(rows, 4, 64, dtype)
+    paged.attend(r.pool, r.batch([rows]), dev(bad, dtype), out=out)
+    got = from_type(out.numpy(), dtype)
+    assert np.isnan(got[rows // 2, 1:]).all()
+    keep = np.ones((rows, 4), dtype=bool)
+    keep[rows // 2, 1:] = False
+    np.testing.assert_array_equal(got[keep], from_type(clean, dtype)[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 45])
+@pytest.mark.parametrize("tokens", [90, 4100])
+def test_a_row_whose_scores_are_all_beyond_range_below_is_nan(hiplib, rows, tokens):
+    """it sees tokens, so zeros -- the answer of a row that sees none -- would pass for a result"""
+    r = Rig(2, tokens, 1, 64, np.random.default_rng(33))
+    k = to_type((np.abs(r.rng.standard_normal((tokens, 1, 64))) + 0.1) * 1e20, "float32")
+    r.add([tokens, 0], "float32", k=k)
+    q = to_type((np.abs(r.rng.standard_normal((2 * rows, 2, 64))) + 0.1) * -1e20, "float32")
+    out = marked(2 * rows, 2, 64)
+    paged.attend(r.pool, r.batch([rows, rows]), dev(q), out=out)
+    got = out.numpy()
+    assert np.isnan(got[:rows]).all() and not got[rows:].any()
+
+
 # ---- selection ------------------------------------------------------------------------------------------------------------------------
 
 
