@@ -519,7 +519,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		return;
 	}
 	const int rl = r0 + 15 < nrows - 1 ? r0 + 15 : nrows - 1;
-	const int p_min = len - n + r0 / a.group, p_max = len - n + rl / a.group;
+	const int p_first = len - n + r0 / a.group, p_max = len - n + rl / a.group;
+	const int p_min = p_first < 0 ? 0 : p_first; // (rows before position 0 see nothing; their distance to a window's end may pass 32 bits)
 	const KvSpan sp(p_min, p_max, a.window, a.sinks);
 	// ranges of a.chunk pages; the last takes what a sequence longer than the host's bound has beyond them
 	const bool direct = sp.np <= a.chunk || a.n_splits == 1;
@@ -527,7 +528,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 	const int rr = r0 + col;
 	const bool live = rr < nrows;
 	const int t = (live ? rr : r0) / a.group, hd = h * a.group + (live ? rr : r0) % a.group;
-	const int pos = len - n + t;
+	const int pos = len - n + t, past = (pos < 0 ? 0 : pos) - a.window; // (the last position before the window)
 	const size_t row = (size_t)(row0 + t) * a.n_heads + hd;
 	if (i0 >= i1 && split > 0) {
 		if (!direct && wave == 0 && g == 0) { // a range without pages: marked empty for k_kv_merge
@@ -729,7 +730,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
 					const int j = j0 + 16 * t + 4 * g + e;
-					const bool seen = j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+					const bool seen = j <= pos && (a.window <= 0 || j > past || j < a.sinks);
 					sc[t][e] = seen ? sc[t][e] * (kscale[t] * qf) : -__builtin_inff();
 					top = fmaxf(top, sc[t][e]);
 				}
@@ -969,7 +970,8 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 		return;
 	}
 	const int rl = r0 + 127 < nrows - 1 ? r0 + 127 : nrows - 1;
-	const int p_min = len - n + r0 / a.group, p_max = len - n + rl / a.group;
+	const int p_first = len - n + r0 / a.group, p_max = len - n + rl / a.group;
+	const int p_min = p_first < 0 ? 0 : p_first; // (rows before position 0 see nothing; their distance to a window's end may pass 32 bits)
 	const KvSpan sp(p_min, p_max, a.window, a.sinks);
 	// ranges of a.chunk pages; the last takes what a sequence longer than the host's bound has beyond them
 	const bool direct = sp.np <= a.chunk || a.n_splits == 1;
@@ -978,13 +980,13 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	const int rr = r0 + 32 * wave + col;
 	const bool live = rr < nrows;
 	const int t = (live ? rr : nrows - 1) / a.group, hd = h * a.group + (live ? rr : nrows - 1) % a.group;
-	const int pos = len - n + t;
+	const int pos = len - n + t, past = (pos < 0 ? 0 : pos) - a.window; // (the last position before the window)
 	const auto row_of = [&](int r) {
 		return (size_t)(row0 + r / a.group) * a.n_heads + h * a.group + r % a.group;
 	};
 	const int wl = r0 + 32 * wave + 31 < nrows - 1 ? r0 + 32 * wave + 31 : nrows - 1;
 	const bool any = r0 + 32 * wave < nrows;
-	const int w_min = len - n + (any ? r0 + 32 * wave : 0) / a.group, w_max = any ? len - n + wl / a.group : -1;
+	const int w_first = len - n + (any ? r0 + 32 * wave : 0) / a.group, w_min = w_first < 0 ? 0 : w_first, w_max = any ? len - n + wl / a.group : -1;
 	if (i0 >= i1 && split > 0) {
 		if (!direct && live && hh == 0) {
 			float* const p = a.part + (row_of(rr) * a.n_splits + split) * (D + 4) + D;
@@ -1182,7 +1184,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 #pragma unroll
 					for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; ++e) {
 						const int j = j0 + 32 * (b >> 1) + 8 * (e >> 2) + 4 * hh + (e & 3);
-						const bool seen = (j <= pos) & ((a.window <= 0) | (j > pos - a.window) | (j < a.sinks));
+						const bool seen = (j <= pos) & ((a.window <= 0) | (j > past) | (j < a.sinks));
 						sc[b >> 1][e] = seen ? sc[b >> 1][e] * f[b] : -__builtin_inff();
 					}
 					f[b] = 1.f;

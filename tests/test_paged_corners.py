@@ -71,6 +71,22 @@ def test_a_row_whose_scores_are_all_beyond_range_below_is_nan(hiplib, rows, toke
     assert np.isnan(got[:rows]).all() and not got[rows:].any()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30])
+@pytest.mark.parametrize("rows", [12, 50])
+def test_the_widest_windows_beside_rows_before_position_0(hiplib, rows, window):
+    """a sequence of fewer tokens than rows, under a window that ends beyond 32 bits before its first rows: the rows at positions see what they see without a window"""
+    r = Rig(2, 100, 2, 64, np.random.default_rng(36))
+    r.add([rows - 7, 90], "float32")
+    q = dev(to_type(r.rng.standard_normal((2 * rows, 4, 64)), "float32"))
+    want = paged.attend(r.pool, r.batch([rows, rows]), q).numpy()
+    got = paged.attend(r.pool, r.batch([rows, rows]), q, window=window).numpy()
+    np.testing.assert_array_equal(got, want)
+    got = paged.attend(r.pool, r.batch([rows, rows]), q, window=window, sinks=2 ** 31 - 1).numpy()
+    np.testing.assert_array_equal(got, want)
+    assert not got[:7].any() and got[7:].any(axis=(1, 2)).all()
+
+
 # ---- selection ------------------------------------------------------------------------------------------------------------------------
 
 
