@@ -424,9 +424,9 @@ __global__ __launch_bounds__(64) void k_kv_read(KvReadArgs a) {
 //                a 30th of what fp16 rows were rounded by near their largest element and comes up to it for elements below a 60th of that.
 //   k_kv_chunk   one binary16 after the row is scaled by a power of two to at most 1 (fp16 and bf16 rows lose nothing above 2^-14 of their largest
 //                element), fp32 rows as the sum of two (22 bits); scores are fp32 sums.
-// Scores are then fp32, times the block's K scale; P_j times the block's V scale over the largest one met (E) is one binary16 for fp16 / bf16
-// outputs -- 2^-12 relative, a third or less of the output's own rounding, since weights average -- and the sum of two for fp32; sums in
-// fp32.  A weight below 2^-14 of the largest (V scale included) keeps an absolute 2^-25 of it.
+// Scores are then fp32, times the block's K scale.  A weight goes into the second product with its block's V scale, relative to the largest such
+// that the ROW met (KvRefs), as one binary16 for fp16 / bf16 outputs -- off by at most 2^-11, half a step, each its own way, and outputs are
+// averages of them -- and as the sum of two for fp32 (2^-22); sums are fp32.  Below 2^-20 of the largest a weight keeps an absolute 2^-31 of it.
 
 struct KvAttnArgs {
 	KvLayer p;
@@ -434,7 +434,7 @@ struct KvAttnArgs {
 	const void* q;
 	void* out; // [row][head][D]
 	long q_row, q_head;
-	float* part; // [row x head][split][D + 4]: partial sums, then the maximum and the sum of weights
+	float* part; // [row x head][split][D + 4]: partial sums, then reference, sum of weights and reference of the sums (KvRefs)
 	int n_heads, group, window, sinks, chunk, n_splits;
 	float scale; // scale * log2(e)
 };
@@ -479,7 +479,36 @@ __device__ __forceinline__ int kv_row_exp(float top) {
 	return e > 126 ? 126 : e;
 }
 
-// the result of a row, or its part of a split: `o` (a quad of dims) times f
+// Two references a row, whole numbers both: m follows x_j, mv follows x_j + v_j (v_j: the exponent field of V's scale), each over the tokens that
+// the row itself sees.  Sums of weights are relative to 2^m; what goes into the product with V's codes is y_j = 2^(x_j + v_j - mv + KV_LIFT), so
+// nothing that a row does not see, or gives no weight, takes bits from it, however large its V.  A block's share of the sum of weights is
+// that of its y, times 2^k, k = mv - KV_LIFT - m - v.  k is held between -126 and KV_REACH: above, V is 2^-53 of what the row's output is made of and
+// takes part as if it were no smaller; below, the weight is 2^-118 of the largest and nothing in 32 bits.  A reference stays unless it is passed by 2^8:
+// weights up to 2^8 are no less exact, and sums are seldom rescaled.  y <= 2^15 is inside binary16; KV_LIFT moves its subnormals away.
+constexpr float KV_LIFT = 7.f, KV_REACH = 60.f;
+struct KvRefs {
+	float m, mv, rm, rv, gap, m0, mv0;
+	bool moved;
+	__device__ __forceinline__ KvRefs(float m0_, float mv0_, float top, float topv) : m0(m0_), mv0(mv0_) {
+		m = top > m0 + 8.f ? ceilf(top) : m0;
+		mv = topv > mv0 + 8.f ? ceilf(topv) : mv0;
+		rm = m == -__builtin_inff() ? 0.f : m, rv = mv == -__builtin_inff() ? 0.f : mv; // (no token seen yet)
+		gap = rv - KV_LIFT - rm;
+		moved = m != m0 || mv != mv0;
+	}
+	__device__ __forceinline__ float of_l() const { // what rescales the sums (m0 = -inf: 0)
+		return kv_exp2(m0 - rm);
+	}
+	__device__ __forceinline__ float of_o() const {
+		return kv_exp2(mv0 - rv);
+	}
+};
+// sum of y_j V_j over the sum of weights, with V's scale back in
+__device__ __forceinline__ float kv_result(float y, float rm, float rv) {
+	return __builtin_amdgcn_ldexpf(y, (int)(rv - 127.f - KV_LIFT - rm));
+}
+
+// the result of a row, or its part of a split: a quad of dims
 template <int D, int DT>
 __device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t row, int split, int d, const float (&o)[4]) {
 	if (direct) {
@@ -534,7 +563,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		if (!direct && wave == 0 && g == 0) { // a range without pages: marked empty for k_kv_merge
 			if (live) {
 				float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
-				p[0] = -__builtin_inff(), p[1] = 0.f;
+				p[0] = -__builtin_inff(), p[1] = 0.f, p[2] = -__builtin_inff();
 			}
 		}
 		return;
@@ -658,12 +687,11 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 	}
 	kv_f32x4 o[ND];
-	float m = -__builtin_inff(), l = 0.f;
+	float m = -__builtin_inff(), mv = -__builtin_inff(), l = 0.f;
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
 		o[d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
 	}
-	float E = 1.1754944e-38f; // the largest V scale met
 	for (int i = i0 + wave; i < i1; i += NW) {
 		const int pg = sp.page(i), j0 = pg * KV_PAGE;
 		const bool bad = pid < 0;
@@ -705,89 +733,67 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 				sc[t][e] = y;
 			}
 		}
-		// (a missing page: NaN through K; its V scale must not become the reference of rows that do not see it)
-		const float none = __builtin_nanf("");
-		const kv_f32x4 kscale = bad ? (kv_f32x4){none, none, none, none} : ksc, vscale = bad ? (kv_f32x4){0.f, 0.f, 0.f, 0.f} : vsc;
+		// a missing page, and a block whose V scale is no number, are NaN through K, for the rows that see them
+		float kscale[4], lv[4];
+#pragma unroll
+		for (int t = 0; t < 4; ++t) {
+			const float one = vsc[t];
+			kscale[t] = bad ? __builtin_nanf("") : __builtin_fmaf(one, 0.f, ksc[t]);
+			lv[t] = (float)((__builtin_bit_cast(unsigned, one) >> 23) & 0xffu);
+		}
 		if (more) {
 			load_k(next);
 		}
 		// every token of the page seen by every row of the tile?
 		const bool whole = j0 + KV_PAGE - 1 <= p_min && (a.window <= 0 || j0 > p_max - a.window || j0 + KV_PAGE <= a.sinks);
-		float Enew = E;
+		float top = -__builtin_inff(), topv = -__builtin_inff();
 #pragma unroll
 		for (int t = 0; t < 4; ++t) {
-			const int jb = j0 + 16 * t;
-			const bool seen = whole || (jb <= p_max && (a.window <= 0 || jb + 15 > p_min - a.window || jb < a.sinks));
-			Enew = fmaxf(Enew, seen ? fabsf(vscale[t]) : 0.f);
-		}
-		const float rE = __builtin_amdgcn_rcpf(Enew), grow = E * rE;
-		E = Enew;
-		kv_f16x8 pf[2], pl[HL ? 2 : 1];
-		float top = -__builtin_inff();
-		if (!whole) {
-#pragma unroll
-			for (int t = 0; t < 4; ++t) {
+			const float f = kscale[t] * qf;
+			float x = -__builtin_inff();
+			if (!whole) {
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
 					const int j = j0 + 16 * t + 4 * g + e;
 					const bool seen = j <= pos && (a.window <= 0 || j > past || j < a.sinks);
-					sc[t][e] = seen ? sc[t][e] * (kscale[t] * qf) : -__builtin_inff();
-					top = fmaxf(top, sc[t][e]);
+					sc[t][e] = seen ? sc[t][e] * f : -__builtin_inff();
+					x = fmaxf(x, sc[t][e]);
 				}
-			}
-		} else {
-#pragma unroll
-			for (int t = 0; t < 4; ++t) {
-				const float f = kscale[t] * qf;
+				kscale[t] = 1.f;
+			} else {
 				const float hi = fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])) * f;
 				const float lo = fminf(fminf(sc[t][0], sc[t][1]), fminf(sc[t][2], sc[t][3])) * f;
-				top = fmaxf(top, fmaxf(hi, lo)); // (a negative factor turns them round)
+				x = fmaxf(hi, lo); // (a negative factor turns them round)
+				kscale[t] = f;
 			}
+			top = fmaxf(top, x), topv = fmaxf(topv, x + lv[t]);
 		}
-		top = kv_max32(kv_max16(top));
-		// the reference stays unless a score passes it by 2^8 (weights up to 2^8 are no less exact): sums are seldom rescaled
-		const float ref = top > m + 8.f || m == -__builtin_inff() ? fmaxf(top, m) : m;
-		const float zero_ref = ref == -__builtin_inff() ? 0.f : ref;
-		const float alpha = kv_exp2(m - zero_ref); // (m = -inf: 0)
-		m = ref;
-		const float og = alpha * grow;
-		if (__ballot(og != 1.f)) {
-			l *= alpha;
+		top = kv_max32(kv_max16(top)), topv = kv_max32(kv_max16(topv));
+		const KvRefs ref(m, mv, top, topv);
+		if (__ballot(ref.moved)) {
+			l *= ref.of_l();
+			const float by = ref.of_o();
 #pragma unroll
 			for (int d = 0; d < ND; ++d) {
-				o[d] *= og;
+				o[d] *= by;
 			}
 		}
-		if (!whole) {
+		m = ref.m, mv = ref.mv;
+		kv_f16x8 pf[2], pl[HL ? 2 : 1];
 #pragma unroll
-			for (int t = 0; t < 4; ++t) {
-				const float f = vscale[t] * rE;
+		for (int t = 0; t < 4; ++t) {
+			const float k = __builtin_amdgcn_fmed3f(ref.gap - lv[t], -126.f, KV_REACH), from = -(ref.rm + k);
+			float sum = 0.f;
 #pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					const float w = kv_exp2(sc[t][e] - zero_ref);
-					l += w;
-					const float y = sc[t][e] == -__builtin_inff() ? 0.f : w * f; // (a NaN scale must not reach a row that does not see the token)
-					pf[t >> 1][4 * (t & 1) + e] = (_Float16)y;
-					if constexpr (HL) {
-						pl[t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[t >> 1][4 * (t & 1) + e]);
-					}
+			for (int e = 0; e < 4; ++e) {
+				const float y = kv_exp2(__builtin_fmaf(sc[t][e], kscale[t], from));
+				sum += y;
+				pf[t >> 1][4 * (t & 1) + e] = (_Float16)y;
+				if constexpr (HL) {
+					pl[t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[t >> 1][4 * (t & 1) + e]);
 				}
 			}
-		} else {
-#pragma unroll
-			for (int t = 0; t < 4; ++t) {
-				const float f = kscale[t] * qf, fv = vscale[t] * rE;
-#pragma unroll
-				for (int e = 0; e < 4; ++e) {
-					const float w = kv_exp2(__builtin_fmaf(sc[t][e], f, -zero_ref));
-					l += w;
-					const float y = w * fv;
-					pf[t >> 1][4 * (t & 1) + e] = (_Float16)y;
-					if constexpr (HL) {
-						pl[t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[t >> 1][4 * (t & 1) + e]);
-					}
-				}
-			}
+			l = __builtin_fmaf(sum, kv_exp2(k), l);
 		}
 #pragma unroll
 		for (int d = 0; d < ND; ++d) {
@@ -815,7 +821,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		*(kv_f32x4*)(p + 16 * d + 4 * g) = o[d];
 	}
 	if (g == 0) {
-		p[D] = m, p[D + 1] = l, p[D + 2] = E;
+		p[D] = m, p[D + 1] = l, p[D + 2] = mv;
 	}
 	__syncthreads();
 	// a thread per (row, quad of dims)
@@ -826,36 +832,38 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 		const float* const p = kv_lds + rr * (D + 4);
 		constexpr int W = 16 * (D + 4);
-		float M = -__builtin_inff(), EM = 0.f;
+		float M = -__builtin_inff(), MV = M;
 #pragma unroll
 		for (int w = 0; w < NW; ++w) {
-			M = fmaxf(M, p[w * W + D]), EM = fmaxf(EM, p[w * W + D + 2]);
+			M = fmaxf(M, p[w * W + D]), MV = fmaxf(MV, p[w * W + D + 2]);
 		}
-		const float ref = M == -__builtin_inff() ? 0.f : M;
+		const float rm = M == -__builtin_inff() ? 0.f : M, rv = MV == -__builtin_inff() ? 0.f : MV;
 		float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 		for (int w = 0; w < NW; ++w) {
-			const float f = kv_exp2(p[w * W + D] - ref), fe = f * (p[w * W + D + 2] / EM);
-			L += f * p[w * W + D + 1];
+			const float fo = kv_exp2(p[w * W + D + 2] - rv);
+			L += kv_exp2(p[w * W + D] - rm) * p[w * W + D + 1];
 			const kv_f32x4 x = *(const kv_f32x4*)(p + w * W + d);
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
-				y[e] += fe * x[e];
+				y[e] += fo * x[e];
 			}
 		}
 		const int t = (r0 + rr) / a.group;
 		const size_t at = (size_t)(row0 + t) * a.n_heads + h * a.group + (r0 + rr) % a.group;
 		// (no token seen: zeros.  Tokens seen, and every score beyond fp32 below: NaN; k_kv_merge knows by a sum of -0)
 		const bool blind = L == 0.f && len - n + t < 0;
-		const float f = direct ? (L == 0.f ? (blind ? 0.f : __builtin_nanf("")) : EM / L) : EM;
+		if (direct) {
+			const float f = L == 0.f ? (blind ? 0.f : __builtin_nanf("")) : 1.f / L;
 #pragma unroll
-		for (int e = 0; e < 4; ++e) {
-			y[e] *= f;
+			for (int e = 0; e < 4; ++e) {
+				y[e] = kv_result(y[e] * f, rm, rv);
+			}
 		}
 		kv_put<D, DT>(a, direct, at, split, d, y);
 		if (d == 0 && a.n_splits > 1) {
 			float* const pm = a.part + (at * a.n_splits + split) * (D + 4) + D;
-			pm[0] = M, pm[1] = direct ? -1.f : L == 0.f && !blind ? -0.f : L; // (no sum of weights is negative: the row is written already)
+			pm[0] = M, pm[1] = direct ? -1.f : L == 0.f && !blind ? -0.f : L, pm[2] = MV; // (no sum of weights is negative: the row is written already)
 		}
 	}
 }
@@ -871,18 +879,18 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 		return; // rows behind the last sequence stay as they are
 	}
 	const float* const p = a.part + row * a.n_splits * (D + 4);
-	float m = -__builtin_inff(), l = 0.f;
+	float m = -__builtin_inff(), mv = m, l = 0.f;
 	if (lane < a.n_splits) {
-		m = p[(size_t)lane * (D + 4) + D], l = p[(size_t)lane * (D + 4) + D + 1];
+		m = p[(size_t)lane * (D + 4) + D], l = p[(size_t)lane * (D + 4) + D + 1], mv = p[(size_t)lane * (D + 4) + D + 2];
 	}
 	const int l0 = __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), 0); // (the first range's)
 	if (__builtin_bit_cast(float, l0) < 0.f) {
 		return; // one range: written by its workgroup
 	}
 	const bool empty = m == -__builtin_inff() && l == 0.f;
-	const float M = wave_max_dpp(m);
-	const float w = kv_exp2(m - (M == -__builtin_inff() ? 0.f : M));
-	const float L = wave_sum(empty ? 0.f : w * l);
+	const float M = wave_max_dpp(m), MV = wave_max_dpp(mv);
+	const float rm = M == -__builtin_inff() ? 0.f : M, rv = MV == -__builtin_inff() ? 0.f : MV;
+	const float L = wave_sum(empty ? 0.f : kv_exp2(m - rm) * l), w = kv_exp2(mv - rv);
 	const unsigned long long some = __ballot(!empty);
 	constexpr int N = (D + 255) / 256;
 	const int d = lane * 4;
@@ -904,7 +912,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 		const float f = L == 0.f ? (l0 < 0 ? __builtin_nanf("") : 0.f) : 1.f / L; // (-0: tokens seen, no score in range)
 #pragma unroll
 		for (int e = 0; e < 4; ++e) {
-			y[e] *= f;
+			y[e] = kv_result(y[e] * f, rm, rv);
 		}
 		kv_store4<DT>(a.out, row * D + d, y);
 	}
@@ -990,7 +998,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	if (i0 >= i1 && split > 0) {
 		if (!direct && live && hh == 0) {
 			float* const p = a.part + (row_of(rr) * a.n_splits + split) * (D + 4) + D;
-			p[0] = -__builtin_inff(), p[1] = 0.f;
+			p[0] = -__builtin_inff(), p[1] = 0.f, p[2] = -__builtin_inff();
 		}
 		return;
 	}
@@ -1033,8 +1041,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			}
 		}
 	}
-	float m = -__builtin_inff(), l = 0.f;
-	int Eb = 0x00800000; // the largest V scale met, by its bits
+	float m = -__builtin_inff(), mv = -__builtin_inff(), l = 0.f;
 	kv_f32x16 o[ND], zero;
 #pragma unroll
 	for (int e = 0; e < 16; ++e) {
@@ -1155,22 +1162,13 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			__builtin_amdgcn_sched_barrier(0);
 			__builtin_amdgcn_s_setprio(0);
 			kv_f16x8 pf[4], pl[HL ? 4 : 1];
-			// V's scales are powers of two: a weight takes its block's, over the largest met (E, 2^shift), into its exponent, and the sum of weights
-			// takes it out again a block at a time; all of that is whole numbers in scalar registers, beside the vector instructions.  A block
-			// that no row sees says nothing; one with the scale NaN, or of a missing page, is NaN through K, for the rows that see it.
-			int shift[4], En = Eb;
+			// (a block whose V scale is no number, and a missing page, are NaN through K, for the rows that see them)
+			int lv[4]; // exponents of V's scales
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
-				const int jb = j0 + 16 * b;
-				const bool seen = whole || ((jb <= w_max) & ((a.window <= 0) | (jb + 15 > w_min - a.window) | (jb < a.sinks)));
-				const bool number = (unsigned)vb[b] < 0x7f800000u;
-				kb[b] = pid >= 0 && number ? kb[b] : 0x7fc00000;
-				vb[b] = pid >= 0 && number && seen ? vb[b] : 0;
-				En = max(En, vb[b]);
-			}
-#pragma unroll
-			for (int b = 0; b < 4; ++b) {
-				shift[b] = max((vb[b] - En) >> 23, -64); // (below 2^-64 of E a V is nothing beside it, weighted or not)
+				const bool number = pid >= 0 && (unsigned)vb[b] < 0x7f800000u;
+				kb[b] = number ? kb[b] : 0x7fc00000;
+				lv[b] = number ? vb[b] >> 23 : 0;
 			}
 			float f[4];
 #pragma unroll
@@ -1190,7 +1188,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 					f[b] = 1.f;
 				}
 			}
-			float top = m;
+			float top = m, topv = mv;
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
 				float t = -__builtin_inff();
@@ -1198,20 +1196,19 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 				for (int e = 0; e < 8; ++e) {
 					t = fmaxf(t, sc[b >> 1][8 * (b & 1) + e]);
 				}
-				top = fmaxf(top, t * f[b]);
+				t *= f[b];
+				top = fmaxf(top, t), topv = fmaxf(topv, t + (float)lv[b]);
 			}
-			top = kv_max32(top);
-			// the reference stays unless a score passes it by 2^8: weights up to 2^8 are no less exact, and the sums are seldom rescaled
-			const float m0 = m;
-			m = top > m + 8.f ? top : m;
-			const float ref = m == -__builtin_inff() ? 0.f : m; // (no token seen yet)
-			const float alpha = kv_exp2(m0 - ref); // (m0 = -inf: 0)
-			const float og = alpha * __builtin_bit_cast(float, max(0x3f800000 + (Eb - En), 0));
-			Eb = En;
-			l *= alpha;
+			top = kv_max32(top), topv = kv_max32(topv);
+			const KvRefs ref(m, mv, top, topv);
+			m = ref.m, mv = ref.mv;
+			l *= ref.of_l();
+			const float by = ref.of_o();
+			const int gap = (int)ref.gap;
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
-				const float from = (float)shift[b] - ref;
+				const int k = min(max(gap - lv[b], -126), (int)KV_REACH);
+				const float from = -(ref.rm + (float)k);
 				float sum = 0.f;
 #pragma unroll
 				for (int e = 0; e < 8; ++e) {
@@ -1222,12 +1219,12 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 						pl[b][e] = (_Float16)(y - (float)pf[b][e]);
 					}
 				}
-				l = __builtin_fmaf(sum, kv_exp2i(-shift[b]), l);
+				l = __builtin_fmaf(sum, kv_exp2i(k), l);
 			}
-			if (__ballot(og != 1.f)) {
+			if (__ballot(ref.moved)) {
 #pragma unroll
 				for (int d = 0; d < ND; ++d) {
-					o[d] *= og;
+					o[d] *= by;
 				}
 			}
 			__builtin_amdgcn_sched_barrier(0);
@@ -1259,18 +1256,23 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	}
 	const size_t row = row_of(again);
 	const bool blind = l == 0.f && len - n + again / a.group < 0;
-	const float E = __builtin_bit_cast(float, Eb), f = direct ? (l == 0.f ? (blind ? 0.f : __builtin_nanf("")) : E / l) : E;
+	const float rm = m == -__builtin_inff() ? 0.f : m, rv = mv == -__builtin_inff() ? 0.f : mv;
+	const float f = l == 0.f ? (blind ? 0.f : __builtin_nanf("")) : 1.f / l;
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
 #pragma unroll
 		for (int q = 0; q < 4; ++q) {
-			const float y[4] = {o[d][4 * q] * f, o[d][4 * q + 1] * f, o[d][4 * q + 2] * f, o[d][4 * q + 3] * f};
+			float y[4];
+#pragma unroll
+			for (int e = 0; e < 4; ++e) {
+				y[e] = direct ? kv_result(o[d][4 * q + e] * f, rm, rv) : o[d][4 * q + e];
+			}
 			kv_put<D, DT>(a, direct, row, split, 32 * d + 8 * q + 4 * hh, y);
 		}
 	}
 	if (hh == 0 && a.n_splits > 1) {
 		float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
-		p[0] = m, p[1] = direct ? -1.f : l == 0.f && !blind ? -0.f : l; // (as above)
+		p[0] = m, p[1] = direct ? -1.f : l == 0.f && !blind ? -0.f : l, p[2] = mv; // (as above)
 	}
 }
 

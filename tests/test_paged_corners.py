@@ -87,6 +87,85 @@ def test_the_widest_windows_beside_rows_before_position_0(hiplib, rows, window):
     assert not got[:7].any() and got[7:].any(axis=(1, 2)).all()
 
 
+# ---- V's scales -----------------------------------------------------------------------------------------------------------------------
+
+
+def weighted_size(q, k, v, scale, window, sinks):
+    """sum_j p_j max_d |V_j|: what an output is made of, [rows, heads]"""
+    return attention(q, k, np.broadcast_to(np.abs(v).max(axis=2, keepdims=True), v.shape), scale, window, sinks)[..., 0]
+
+
+def weighted_blocks(q, k, cache, scale, window, sinks):
+    """sum_j p_j 127 s_j, s_j the scale of the token's block: what the same output could be made of, by the codes' range.  A row's reference is the largest
+    p_j s_j it sees, whichever codes those tokens hold (small ones beside a large one are held in its steps already): with two binary16 halves up to
+    2^15 and the largest at 2^6 or more, a term is off by 2^-31 of the reference times its code, n of them by n 2^-31 of this size: 3e-7 for 600."""
+    s = np.repeat(np.stack([cache.scale[0, b] for b in range(-(-len(k) // 16))]), 16, axis=0)[:len(k)]
+    return attention(q, k, np.broadcast_to(127 * s[:, :, None], k.shape), scale, window, sinks)[..., 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,tokens", [(14, 408), (50, 408), (14, 4104), (50, 4104)])
+@pytest.mark.parametrize("ratio", [12, 20, 60])
+def test_large_values_that_a_row_does_not_weigh_cost_it_nothing(hiplib, dtype, rows, tokens, ratio):
+    """V blocks 2^ratio larger: among the last tokens, which the earlier rows do not see, and one in the middle that every row sees and gives a weight of next
+    to nothing.  The error is held against what the row's own output is made of, by the bounds of tests/test_paged.py."""
+    dim, rng = 64, np.random.default_rng(ratio + rows)
+    r = Rig(1, tokens, 1, dim, rng)
+    u = rng.standard_normal(dim)
+    k = rng.standard_normal((tokens, 1, dim))
+    v = rng.standard_normal((tokens, 1, dim))
+    far = slice(160, 176)
+    k[far] = u * (-40 * dim ** 0.5 / (u @ u) * (1 + 0.02 * rng.standard_normal((16, 1, 1))))  # scores near -40
+    if ratio == 60:
+        k[far] *= 2  # ... of -80: e^-80 2^60 is nothing either
+    v[far] *= 2.0 ** ratio
+    last = (tokens - 1) // 16 * 16  # (the last block: later rows of a tile alone see it)
+    v[last:] *= 2.0 ** ratio
+    r.add([tokens], "float32", k=to_type(k, "float32"), v=to_type(v, "float32"))
+    q = to_type(u + 0.05 * rng.standard_normal((rows, 2, dim)), dtype)
+    got = from_type(paged.attend(r.pool, r.batch([rows]), dev(q, dtype)).numpy(), dtype)
+    x, kv, vv = from_type(q, dtype), r.k.values(0), r.v.values(0)
+    want = attention(x, kv, vv, dim ** -0.5, 0, 0)
+    size = weighted_size(x, kv, vv, dim ** -0.5, 0, 0)
+    before = tokens - rows + np.arange(rows) < last
+    assert before.any() and not before.all()
+    if dtype == "float16":  # (a result beyond the type's range is an infinity)
+        over = np.abs(want) >= 65520
+        np.testing.assert_array_equal(got[over], np.sign(want[over]) * np.inf)
+        got[over] = want[over]
+    err = np.abs(got - want) / size[..., None]
+    assert err.max() <= 2.0 ** -9 + U[dtype], (err.max(), np.unravel_index(err.argmax(), err.shape))
+    if dtype == "float32":
+        assert ((err ** 2).mean(axis=(1, 2)) ** 0.5).max() <= 2e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 50])
+def test_zeros_and_the_smallest_and_largest_scales(hiplib, rows):
+    """blocks of zeros (the least scale there is), of 1e-36 and of 1e30 in one sequence, weighted alike or not"""
+    rng = np.random.default_rng(35)
+    r = Rig(1, 600, 1, 64, rng)
+    v = rng.standard_normal((600, 1, 64))
+    v[:100], v[200:300], v[400:450] = 0, v[200:300] * 1e-36, v[400:450] * 1e30
+    r.add([600], "float32", v=to_type(v, "float32"))
+    q = to_type(rng.standard_normal((rows, 2, 64)), "float32")
+    for window in (0, 100, 170):
+        got = paged.attend(r.pool, r.batch([rows]), dev(q), window=window).numpy().astype(np.float64)
+        want = attention(q.astype(np.float64), r.k.values(0), r.v.values(0), 0.125, window, 0)
+        size = weighted_blocks(q.astype(np.float64), r.k.values(0), r.v, 0.125, window, 0)
+        err = np.abs(got - want) / size[..., None]
+        assert err.max() <= 2.0 ** -9 + U["float32"] and (err ** 2).mean() ** 0.5 <= 2e-5, (window, err.max())
+    # nothing but zeros, and nothing but the smallest
+    for lo, hi in ((0, 100), (200, 300)):
+        one = Rig(1, 100, 1, 64, rng)
+        one.add([100], "float32", v=to_type(v[lo:hi], "float32"))
+        got = paged.attend(one.pool, one.batch([rows]), dev(q)).numpy().astype(np.float64)
+        want = attention(q.astype(np.float64), one.k.values(0), one.v.values(0), 0.125, 0, 0)
+        err = np.abs(got - want) / max(np.abs(v[lo:hi]).max(), 1e-37)
+        assert err.max() <= 2.0 ** -9 and (err ** 2).mean() ** 0.5 <= 2e-5
+
+
 # ---- selection ------------------------------------------------------------------------------------------------------------------------
 
 
