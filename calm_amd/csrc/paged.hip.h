@@ -419,9 +419,9 @@ __global__ __launch_bounds__(64) void k_kv_read(KvReadArgs a) {
 // Both products run on the matrix cores, transposed: S^T = K q^T puts a query row into a lane's column, so maximum, sum and rescaling
 // of a row are its lane's own (plus the other lanes of the same column), and the weights are already the operand layout that
 // O^T = V^T P^T wants.  Numerics.  Codes are exact, as bytes and as binary16.  q is cut in two ways:
-//   k_kv_decode  signed digits of base 254 relative to the row's largest magnitude, d0 + d1 / 254 (+ d2 / 254^2 for fp32 rows): the scores are sums of
-//                byte products in whole numbers, exact; what is left out of q is 1.6e-5 (fp32: 6e-8) of its row's largest.  For 16-bit rows that is
-//                a 30th of what fp16 rows were rounded by near their largest element and comes up to it for elements below a 60th of that.
+//   k_kv_decode  three signed digits of base 254 relative to the row's largest magnitude, d0 + d1 / 254 + d2 / 254^2: the scores are sums of byte
+//                products in whole numbers, exact; what is left out of q is 6e-8 of its row's largest.  (Two digits for 16-bit rows, 1.6e-5, are
+//                2 - 4 % faster on 64 sequences with heads of 64 -- 37.5 instead of 39 us -- and cost a row with an outlier channel more than its type does.)
 //   k_kv_chunk   one binary16 after the row is scaled by a power of two to at most 1 (fp16 and bf16 rows lose nothing above 2^-14 of their largest
 //                element), fp32 rows as the sum of two (22 bits); scores are fp32 sums.
 // Scores are then fp32, times the block's K scale.  A weight goes into the second product with its block's V scale, relative to the largest such
@@ -640,8 +640,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 	if constexpr (!HL) {
 		load_q();
 	}
-	// q as NQ signed digits of eight bits, row / 2^e = (d0 + d1 / 254 + d2 / 254^2) / 127: lane (col, g) holds dims g D / 4 .. of its row
-	constexpr int NQ = HL ? 3 : 2;
+	// q as three signed digits of eight bits, row / 2^e = (d0 + d1 / 254 + d2 / 254^2) / 127: lane (col, g) holds dims g D / 4 .. of its row
+	constexpr int NQ = 3;
 	unsigned qd[NQ][KW];
 	float x[D / 4];
 	unsigned top = 0;
@@ -726,11 +726,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 			}
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
-				float y = __builtin_fmaf((float)acc[1][e], 1.f / 254.f, (float)acc[0][e]);
-				if constexpr (HL) {
-					y = __builtin_fmaf((float)acc[2][e], 1.f / (254.f * 254.f), y);
-				}
-				sc[t][e] = y;
+				// (|sums| < 2^23: the lower two in one whole number below 2^31)
+				sc[t][e] = __builtin_fmaf((float)(__mul24(acc[1][e], 254) + acc[2][e]), 1.f / (254.f * 254.f), (float)acc[0][e]);
 			}
 		}
 		// a missing page, and a block whose V scale is no number, are NaN through K, for the rows that see them

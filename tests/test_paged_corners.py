@@ -71,6 +71,29 @@ def test_a_row_whose_scores_are_all_beyond_range_below_is_nan(hiplib, rows, toke
     assert np.isnan(got[:rows]).all() and not got[rows:].any()
 
 
+# ---- queries with one large element -----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("rows", [1, 45])
+def test_an_outlier_in_a_row_costs_the_others_nothing(hiplib, dtype, dim, rows):
+    """one element of q 4000 times the others, where K is zero: the scores are those of the other elements.  What a row leaves out of them is 6e-8 (2^-24) of its
+    largest element and 2^-25 in chunks, so a score is off by sqrt(dim) * 2^-24 * 4000 * max|K| * dim ** -0.5 < 1e-3 at the very worst and a weight by twice that
+    share: inside the 2^-9 of tests/test_paged.py, which stands for this."""
+    r = Rig(1, 300, 1, dim, np.random.default_rng(dim))
+    k = r.rng.standard_normal((300, 1, dim))
+    k[:, :, 3] = 0
+    r.add([300], "float32", k=to_type(k, "float32"))
+    q = r.rng.standard_normal((rows, 2, dim))
+    q[:, :, 3] = 4000 * np.sign(q[:, :, 3])
+    q = to_type(q, dtype)
+    got = from_type(paged.attend(r.pool, r.batch([rows]), dev(q, dtype)).numpy(), dtype)
+    want = attention(from_type(q, dtype), r.k.values(0), r.v.values(0), dim ** -0.5, 0, 0)
+    assert np.abs(got - want).max() <= (2.0 ** -9 + U[dtype]) * np.abs(r.v.values(0)).max()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30])
 @pytest.mark.parametrize("rows", [12, 50])
