@@ -185,7 +185,7 @@ __device__ __forceinline__ void kv_rows_of(const KvRows& r, int s, int& row0, in
 // takes four tokens x four dims, so K goes out as a dword per token and V as a dword per dim without crossing lanes.  Where all four blocks
 // get new tokens (a prompt's pages) V's dwords meet in LDS and go out as whole lines: four bytes every sixteen cost 5 of 48 us for the
 // 15k tokens of six prompts, 8 heads of 128.  Measured: those 26.6 us, 86 MB = 3.2 TB/s (fp16 in), one fp32 token of 48 sequences 6.1 us (two round trips).
-// grid = (pages touched at most, kv heads)
+// grid = (pages touched at most, + 1, kv heads)
 template <int D, int DT>
 __global__ __launch_bounds__(256, DT == KV_F32 || D > 128 ? 1 : D == 96 ? 7 : 8) void k_kv_append(KvAppendArgs a) {
 	constexpr int NI = (D + 63) / 64; // items (quad of tokens, four dims) per lane: 4 x D / 4 over 64 lanes
@@ -193,11 +193,16 @@ __global__ __launch_bounds__(256, DT == KV_F32 || D > 128 ? 1 : D == 96 ? 7 : 8)
 	const int lane = lane_id(), blk = wave_id(), h = blockIdx.y;
 	int s, at;
 	const KvRows& r = a.r;
+	if (blockIdx.x == gridDim.x - 1) { // one workgroup more than there can be pages: it looks every sequence's bounds over
+		for (int i = threadIdx.x; h == 0 && i < r.n_seqs; i += 256) {
+			if (!kv_rows_fit(r, i)) {
+				kv_flag(a.p.status, KV_BAD_BATCH);
+			}
+		}
+		return;
+	}
 	const auto pages = [&](int i) {
 		int row0, n, len;
-		if (blockIdx.x == 0 && h == 0 && blk == 0 && !kv_rows_fit(r, i)) {
-			kv_flag(a.p.status, KV_BAD_BATCH);
-		}
 		kv_rows_of(r, i, row0, n, len);
 		n = n < len ? n : len;
 		return n > 0 ? (len - 1) / KV_PAGE - (len - n) / KV_PAGE + 1 : 0;

@@ -234,7 +234,7 @@ extern "C" int kv_append_hip(const struct KvPool* pool, const struct KvBatch* ba
 	const long long most = (long long)batch->n_rows / KV_PAGE + 2ll * batch->n_seqs;
 	const unsigned pages = (unsigned)(most < batch->n_rows ? most : batch->n_rows);
 	return kv_dispatch(pool->head_dim, type, [&](auto D, auto T) {
-		hipLaunchKernelGGL((k_kv_append<decltype(D)::value, decltype(T)::value>), dim3(pages, pool->n_kv_heads), dim3(256), 0, (hipStream_t)stream, a);
+		hipLaunchKernelGGL((k_kv_append<decltype(D)::value, decltype(T)::value>), dim3(pages + 1, pool->n_kv_heads), dim3(256), 0, (hipStream_t)stream, a);
 		return kv_launched("kv_append_hip");
 	});
 }

@@ -189,6 +189,29 @@ def test_zeros_and_the_smallest_and_largest_scales(hiplib, rows):
         assert err.max() <= 2.0 ** -9 and (err ** 2).mean() ** 0.5 <= 2e-5
 
 
+# ---- batches that do not add up -------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,bad", [(70, 69), (70, 66), (64, 63), (200, 130)])
+def test_append_reports_starts_of_any_sequence(hiplib, seqs, bad):
+    """one token each for `seqs` sequences, one of them with starts outside its rows: it is not stored, and the pool says so"""
+    r = Rig(seqs, 3, 1, 64, np.random.default_rng(seqs))
+    starts = list(range(seqs + 1))
+    if bad == seqs - 1:
+        starts[-1] = seqs + 5
+    else:
+        starts[bad + 1] = starts[bad] - 3  # (the sequence behind it begins inside other rows: still within its bounds)
+    x = dev(np.ones((seqs, 1, 64), dtype=np.float32))
+    b = paged.KvBatch(r.dtable, ints([5] * seqs), ints(starts), rows=seqs, max_rows=seqs, max_len=5)
+    paged.append(r.pool, b, x, x)
+    with pytest.raises(RuntimeError, match="max_rows"):
+        r.pool.check()
+    good = paged.KvBatch(r.dtable, ints([1] * seqs), ints(list(range(seqs + 1))), rows=seqs, max_rows=1, max_len=1)
+    paged.append(r.pool, good, x, x)
+    r.pool.check()
+
+
 # ---- selection ------------------------------------------------------------------------------------------------------------------------
 
 
