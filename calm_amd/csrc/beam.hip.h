@@ -9,7 +9,9 @@
 // become one.  k_beam_pick: one workgroup per group joins the chunks' sums and lists into every row's W best, then the rows into the group's.
 //
 // The sum decides the order of continuations of DIFFERENT beams, where 32 bits lose what matters: sums and totals are 64 bits wide from a
-// lane's 32 values on; the exponentials are 32 (their errors, 2^-23 each, are not alike and average over the row).
+// lane's 32 values on.  The exponentials are 32 bits (2^-23 each; their errors are not alike and average over the row): all totals of a beam are off by
+// one amount, below 2^-22 and 1e-8 as a rule, and candidates of two beams that are nearer to each other than that may come in either order.
+// Equal rows get equal sums (a value's place in them follows from its index alone), so equal totals stay equal.
 #pragma once
 
 namespace calm {
@@ -154,12 +156,13 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 		return;
 	}
 	const size_t row0 = (size_t)row * (size_t)a.row;
-	// 16-byte loads whatever the row's alignment: the row begins `mis` values behind a 16-byte boundary, and value i of the row is
-	// value i + mis from there; loads that are not wholly inside the row go value by value
+	// 16-byte loads, wherever the row begins (the memory unit takes them at any address): which thread holds which value must not follow the row's
+	// alignment, or the sums of equal rows are added up in different orders and equal totals part.  Loads that are not wholly inside the row go
+	// value by value
 	constexpr int ES = DT == KV_F32 ? 4 : 2;
-	const int mis = (int)((((size_t)a.logits + row0 * ES) & 15) / ES);
+	typedef u32x4 any_u32x4 __attribute__((aligned(2)));
 	float x[BEAM_VPT];
-	const int base = chunk * BEAM_CHUNK - mis;
+	const int base = chunk * BEAM_CHUNK;
 	u32x4 raw[NL];
 	const auto values = [&](int i) {
 #pragma unroll
@@ -173,10 +176,10 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 		}
 	};
 	// (loads first, all of them, then what is made of them: a conversion beside its load is a wait for every one)
-	if (base >= 0 && base + BEAM_CHUNK <= a.vocab) {
+	if (base + BEAM_CHUNK <= a.vocab) {
 #pragma unroll
 		for (int i = 0; i < NL; ++i) {
-			raw[i] = *(const u32x4*)((const char*)a.logits + (row0 + (size_t)(base + (i * 256 + (int)threadIdx.x) * VL)) * ES);
+			raw[i] = *(const any_u32x4*)((const char*)a.logits + (row0 + (size_t)(base + (i * 256 + (int)threadIdx.x) * VL)) * ES);
 		}
 #pragma unroll
 		for (int i = 0; i < NL; ++i) {
@@ -186,24 +189,24 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 #pragma unroll
 		for (int i = 0; i < NL; ++i) {
 			const int at = base + (i * 256 + (int)threadIdx.x) * VL;
-			if (at >= 0 && at + VL <= a.vocab) {
-				raw[i] = *(const u32x4*)((const char*)a.logits + (row0 + (size_t)at) * ES);
+			if (at + VL <= a.vocab) {
+				raw[i] = *(const any_u32x4*)((const char*)a.logits + (row0 + (size_t)at) * ES);
 			}
 		}
 #pragma unroll
 		for (int i = 0; i < NL; ++i) {
 			const int at = base + (i * 256 + (int)threadIdx.x) * VL;
-			if (at >= 0 && at + VL <= a.vocab) {
+			if (at + VL <= a.vocab) {
 				values(i);
 			} else {
 #pragma unroll
 				for (int j = 0; j < VL; ++j) {
 					x[i * VL + j] = BEAM_NONE;
 				}
-				if (at + VL > 0 && at < a.vocab) { // across an end of the row
+				if (at < a.vocab) { // across the row's end
 #pragma unroll
 					for (int j = 0; j < VL; ++j) {
-						const int k = at + j < 0 ? 0 : at + j < a.vocab ? at + j : a.vocab - 1;
+						const int k = at + j < a.vocab ? at + j : a.vocab - 1;
 						const float one = beam_load<DT>(a.logits, row0 + k);
 						x[i * VL + j] = k == at + j ? one : BEAM_NONE;
 					}
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
 	const auto place = [&](int i) { // the row's index of this lane's value i
 		return base + ((i / VL) * 256 + (int)threadIdx.x) * VL + i % VL;
 	};
-	const auto inside = [&](int at) { return at >= 0 && at < a.vocab; };
+	const auto inside = [&](int at) { return at < a.vocab; };
 	int mine_n = 0; // of the wave's own quarter of the list
 	const auto add = [&](bool in, float v, int at) {
 		const unsigned long long who = __ballot(in);

@@ -403,18 +403,19 @@ extern "C" int kv_compact_hip(const struct KvPool* pool, const int* table, const
 }
 
 static int beam_chunks(int vocab) {
-	return (int)(((long long)vocab + 7 + BEAM_CHUNK - 1) / BEAM_CHUNK); // (a row begins up to 7 values behind a 16-byte boundary)
+	return (vocab + BEAM_CHUNK - 1) / BEAM_CHUNK;
 }
 
 extern "C" long long beam_workspace_hip(int groups, int beams, int vocab) {
-	KV_CHECK(groups >= 1 && beams >= 1 && beams <= BEAM_MAX && vocab >= 1 && (long long)groups * beams <= 65535, "1 to 32 beams, at least one token, at most 65535 rows");
+	KV_CHECK(groups >= 1 && beams >= 1 && beams <= BEAM_MAX && vocab >= 1 && vocab <= 1 << 30 && (long long)groups * beams <= 65535,
+	         "1 to 32 beams, 1 to 2^30 tokens, at most 65535 rows");
 	return (long long)groups * beams * beam_chunks(vocab) * (2ll * sizeof(double) + beams * (sizeof(float) + sizeof(int)));
 }
 
 extern "C" int beam_select_hip(const void* logits, int type, long row, int groups, int beams, int vocab, const float* scores, const unsigned char* done, int eos, float* scores_out,
                                int* parents, int* tokens, unsigned char* done_out, void* workspace, size_t workspace_size, void* stream) {
 	const long long need = beam_workspace_hip(groups, beams, vocab);
-	KV_CHECK(need > 0, "1 to 32 beams, at least one token, at most 65535 rows");
+	KV_CHECK(need > 0, "1 to 32 beams, 1 to 2^30 tokens, at most 65535 rows");
 	KV_CHECK(type >= KV_F32 && type <= KV_BF16, "types 0 (fp32), 1 (fp16), 2 (bf16)");
 	KV_CHECK(logits && scores && scores_out && parents && tokens && done_out, "a pointer is missing");
 	KV_CHECK(kv_aligned(logits, type == KV_F32 ? 4 : 2), "logits are not aligned to their type");

@@ -288,7 +288,8 @@ int kv_compact_hip(const struct KvPool* pool, const int* table, const int* refs,
 /* One selection step of a beam search over `groups` of `beams` (<= 32) hypotheses: the best `beams` of every group's beams x vocab
  * continuations by scores[g][w] + log softmax(logits[g * beams + w])[v], best first, equal ones by w, then v.  logits: row stride `row`
  * in elements.  A hypothesis with done[g][w] != 0 (done may be NULL) continues only with `eos`, its score unchanged; a continuation with
- * eos is done.  eos < 0: none (done is not read).  A beam whose score is -inf or whose log-sum-exp is not finite offers only -inf.
+ * eos is done.  eos < 0: none (done is not read).  (Sums are 64 bits of 32-bit exponentials: a beam's totals are off by one amount below 2^-22, 1e-8 as a
+ * rule; beams with equal logits and scores have equal totals.)  A beam whose score is -inf or whose log-sum-exp is not finite offers only -inf.
  * Outputs, [groups][beams] each, beside the inputs: scores, the beam that each continues (0 .. beams - 1), its token, done. */
 long long beam_workspace_hip(int groups, int beams, int vocab);
 int beam_select_hip(const void* logits, int type, long row, int groups, int beams, int vocab, const float* scores, const unsigned char* done, int eos, float* scores_out, int* parents,

@@ -227,3 +227,19 @@ def test_select_a_finished_beam_beside_dead_ones(hiplib, beams, vocab):
     scores[1, -1], done[1, -1] = -2.0, 1
     for eos in (0, 1, vocab - 1):
         check_select(x, scores, done, eos)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("beams,vocab", [(4, 20011), (3, 8193), (8, 32001), (16, 1001), (2, 128257)])
+def test_select_equal_beams_at_any_alignment(hiplib, dtype, beams, vocab):
+    """hypotheses with the same logits and the same score: their totals are equal, so the lowest beam's tokens come first, wherever a row begins"""
+    rng = np.random.default_rng(vocab)
+    x = np.repeat(rng.standard_normal((2, 1, vocab)) * 3, beams, axis=1).reshape(2 * beams, vocab)
+    check_select(x, np.zeros((2, beams)), None, -1, dtype)
+    check_select(x, np.full((2, beams), -1.5), None, -1, dtype, strided=3)
+
+
+def test_select_refuses_vocabularies_beyond_its_indexes(hiplib):
+    assert hiplib.beam_workspace_hip(1, 1, 1 << 30) > 0
+    assert hiplib.beam_workspace_hip(1, 1, (1 << 30) + 1) == -1 and b"2^30 tokens" in hiplib.calm_hip_error()
