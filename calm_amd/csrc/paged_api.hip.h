@@ -347,7 +347,9 @@ extern "C" int kv_reserve_hip(const struct KvPool* pool, int* table, int* refs, 
 	const char* fault = kv_table_fault(pool, table, lens, refs, n_rows, max_pages);
 	KV_CHECK(!fault, fault);
 	KV_CHECK(lens_new, "new lengths are missing");
-	const KvReserveArgs a = {table, refs, lens, lens_new, pool->status, n_rows, max_pages, pool->n_pages};
+	const size_t page = (size_t)pool->n_kv_heads * KV_PAGE * pool->head_dim;
+	const KvReserveArgs a = {table, refs, lens, lens_new, pool->status, n_rows, max_pages, pool->n_pages, pool->k, pool->v, pool->k_scale, pool->v_scale, page,
+	                         pool->n_kv_heads * 4, pool->n_layers};
 	hipLaunchKernelGGL(k_kv_reserve, dim3(1), dim3(KV_BOOK), 0, (hipStream_t)stream, a);
 	return kv_launched("kv_reserve_hip");
 }
@@ -356,7 +358,7 @@ extern "C" int kv_trim_hip(const struct KvPool* pool, int* table, int* refs, con
 	const char* fault = kv_table_fault(pool, table, lens, refs, n_rows, max_pages);
 	KV_CHECK(!fault, fault);
 	KV_CHECK(window >= 0 && sinks >= 0, "a negative window or count of first tokens");
-	const KvReserveArgs a = {table, refs, lens, nullptr, pool->status, n_rows, max_pages, pool->n_pages};
+	const KvReserveArgs a = {table, refs, lens, nullptr, pool->status, n_rows, max_pages, pool->n_pages, nullptr, nullptr, nullptr, nullptr, 0, 0, 0};
 	hipLaunchKernelGGL(k_kv_trim, dim3((unsigned)(((long long)n_rows * max_pages + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a, window, sinks);
 	return kv_launched("kv_trim_hip");
 }

@@ -248,7 +248,7 @@ const char* calm_hip_error(void);
 /* the backend's own stream on the current stage's device (init_hip is run if it was not): what forward_hip and the others are ordered on */
 void* calm_hip_stream(void);
 
-/* Quantises the batch's K and V rows into their pages (which the table must hold already: kv_reserve_hip): element (row, head, dim) of k
+/* Quantises the batch's K and V rows into their pages (which the table must hold, and no other row list: kv_reserve_hip sees to both): element (row, head, dim) of k
  * is at k[row * k_row + head * k_head + dim], strides in elements, multiples of 4.  A block's scale is the least power of two 2^e, e >=
  * -126, with max|x| <= 127 * 2^e over its tokens; a block that holds older tokens keeps the larger of its scale and the new rows', and
  * the older codes are rounded to it.  A block with an infinity or NaN is NaN from then on. */
@@ -269,9 +269,10 @@ long long kv_attend_workspace_hip(const struct KvPool* pool, const struct KvBatc
 int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* batch, int layer, const void* q, void* out, int type, int n_heads, long q_row, long q_head, float scale, int window,
                   int sinks, void* workspace, size_t workspace_size, void* stream);
 
-/* The upkeep of pages.  refs[p] = how many table rows list page p (int [n_pages], 0: free); a page that is not full belongs to one row.
+/* The upkeep of pages.  refs[p] = how many table rows list page p (int [n_pages], 0: free); a page that tokens go into belongs to one row.
  * Up to 2048 table rows, 2^30 entries and pages.  Free pages are taken lowest first, rows in order.
- *   reserve  entries of the pages that tokens lens[r] .. lens_new[r] - 1 of row r need (in place)
+ *   reserve  entries of the pages that tokens lens[r] .. lens_new[r] - 1 of row r need (in place).  Where row r was cut back into a page that other rows list,
+ *            too, that is a page of its own, which takes the old one's bytes in all layers, or -1 and status 2 if none is free
  *   trim     gives up pages behind lens[r] (0: all of them) and, with a window > 0, those that no later token sees (in place)
  *   fork     row r becomes a copy of row parents[r] (out of place: table_out, refs_out; refs_out may be refs): full pages are shared, a
  *            page that is not full stays with its row's first child and is copied, in all layers, for the others; rows without a

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from calm_amd import paged
-from test_paged import TYPES, U, Cache, Rig, attention, check_select, dev, from_type, ints, to_type
+from test_paged import TYPES, U, Book, Cache, Rig, attention, check_select, dev, from_type, ints, to_type
 
 
 # ---- scores and queries out of range --------------------------------------------------------------------------------------------------
@@ -210,6 +210,151 @@ def test_append_reports_starts_of_any_sequence(hiplib, seqs, bad):
     good = paged.KvBatch(r.dtable, ints([1] * seqs), ints(list(range(seqs + 1))), rows=seqs, max_rows=1, max_len=1)
     paged.append(r.pool, good, x, x)
     r.pool.check()
+
+
+# ---- pages that rows share ------------------------------------------------------------------------------------------------------------
+
+
+def fill(pool, rng):
+    """random bytes in every page; the host's copy"""
+    want = []
+    for x in (pool.k, pool.v, pool.k_scale, pool.v_scale):
+        junk = rng.integers(-128, 128, x.shape).astype(np.int8) if x.dtype == "int8" else rng.standard_normal(x.shape).astype(np.float32)
+        x._lib.copy_hip(x.data_ptr(), junk.ctypes.data, junk.nbytes)
+        want.append(junk)
+    return want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dim,layers", [(1, 64, 1), (3, 96, 2)])
+def test_a_row_cut_back_into_a_shared_page_gets_its_own(hiplib, heads, dim, layers):
+    """rows that share full pages are cut back into them (drafts given up behind a fork): before new tokens go in, reserve gives each writer a page of its own
+    with the old one's bytes; the rows that keep the page keep its bytes"""
+    rng = np.random.default_rng(heads)
+    pool = paged.KvPool(layers, 20, heads, dim)
+    want = fill(pool, rng)
+    # rows 0 .. 2 list pages 0, 1, 2 (192 tokens); row 3 lists 0, 1 and owns 3; row 4 owns 4
+    t0 = [[0, 1, 2, -1], [0, 1, 2, -1], [0, 1, 2, -1], [0, 1, 3, -1], [4, -1, -1, -1]]
+    r0 = [4, 4, 3, 1, 1] + [0] * 15
+    table, refs = dev(np.array(t0, dtype=np.int32)), dev(np.array(r0, dtype=np.int32))
+    # row 0 goes back to 100 tokens (inside page 1), row 1 to 128 (a border), row 2 keeps 192, row 3 goes back to 70, row 4 to 10
+    lens = [100, 128, 192, 70, 10]
+    paged.trim(pool, table, refs, ints(lens))
+    np.testing.assert_array_equal(refs.numpy(), [4, 4, 1, 0, 1] + [0] * 15)
+    new = [101, 130, 192, 70, 12]
+    paged.reserve(pool, table, refs, ints(lens), ints(new))
+    # pages in rows' order, the lowest free one each: row 0 a copy of page 1, row 1 a new page; row 3 adds no token and copies nothing, row 4 owns its page
+    np.testing.assert_array_equal(table.numpy(), [[0, 3, -1, -1], [0, 1, 5, -1], [0, 1, 2, -1], [0, 1, -1, -1], [4, -1, -1, -1]])
+    np.testing.assert_array_equal(refs.numpy(), [4, 3, 1, 1, 1, 1] + [0] * 14)
+    for x in want:
+        x[:, 3] = x[:, 1]
+    for got, x in zip((pool.k, pool.v, pool.k_scale, pool.v_scale), want):
+        np.testing.assert_array_equal(got.numpy(), x)
+    # every row that lists page 1 goes on inside it: each gets a copy, and the page itself is free
+    lens = [101, 100, 100, 100, 12]
+    paged.trim(pool, table, refs, ints(lens))
+    paged.reserve(pool, table, refs, ints(lens), ints([n + 1 for n in lens]))
+    t, n = table.numpy(), refs.numpy()
+    assert len({t[1, 1], t[2, 1], t[3, 1], t[0, 1], t[4, 0], 0}) == 6 and (t[:4, 0] == 0).all()
+    counts = np.bincount(t[t >= 0], minlength=20)
+    np.testing.assert_array_equal(n, counts)
+    for row in (1, 2, 3):
+        for x, got in zip(want, (pool.k, pool.v, pool.k_scale, pool.v_scale)):
+            np.testing.assert_array_equal(got.numpy()[:, t[row, 1]], x[:, 1])
+    pool.check()
+
+
+@pytest.mark.gpu
+def test_no_page_for_a_row_cut_back_into_a_shared_one(hiplib):
+    """no free page: the row loses the entry rather than write into the others' page, and the pool says so"""
+    pool = paged.KvPool(1, 2, 1, 64)
+    table, refs = dev(np.array([[0, 1], [0, 1]], dtype=np.int32)), dev(np.array([2, 2], dtype=np.int32))
+    paged.reserve(pool, table, refs, ints([100, 128]), ints([101, 128]))
+    np.testing.assert_array_equal(table.numpy(), [[0, -1], [0, 1]])
+    np.testing.assert_array_equal(refs.numpy(), [2, 1])
+    with pytest.raises(RuntimeError, match="no page was free"):
+        pool.check()
+
+
+@pytest.mark.gpu
+def test_drafts_given_up_behind_a_fork(hiplib):
+    """two rows of one prompt, full pages shared; one is cut back into them and goes on: the other's values stay"""
+    rng = np.random.default_rng(41)
+    pool = paged.KvPool(1, 12, 2, 64)
+    table, refs = dev(np.full((2, 4), -1, dtype=np.int32)), dev(np.zeros(12, dtype=np.int32))
+    k, v = Cache(2, 64), Cache(2, 64)
+
+    def add(lens, new, rows):
+        paged.reserve(pool, table, refs, ints(lens), ints(new))
+        starts = np.concatenate([[0], np.cumsum([b - a for a, b in zip(lens, new)])])
+        batch = paged.KvBatch(table, ints(new), ints(starts), rows=int(starts[-1]), max_rows=int(np.diff(starts).max()), max_len=max(new))
+        paged.append(pool, batch, dev(rows), dev(-rows))
+
+    rows = rng.standard_normal((128, 2, 64)).astype(np.float32)
+    add([0, 0], [128, 0], rows)
+    k.append(0, rows.astype(np.float64)), v.append(0, -rows.astype(np.float64))
+    table, refs = paged.fork(pool, table, ints([128, 0]), refs, ints([0, 0]))
+    paged.trim(pool, table, refs, ints([80, 128]))  # (80: a block's border, so that the first row's old blocks keep their scales)
+    add([80, 128], [90, 128], rng.standard_normal((10, 2, 64)).astype(np.float32) * 50)
+    gk, gv = paged.read(pool, table, ints([90, 128]), ints([0, 0]), 128)
+    for got, want in ((gk, k), (gv, v)):
+        np.testing.assert_array_equal(got.numpy()[1], want.values(0).astype(np.float32))
+        np.testing.assert_array_equal(got.numpy()[0, :80], want.values(0)[:80].astype(np.float32))
+        assert np.abs(got.numpy()[0, 80:90]).max() > 50
+    pool.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,pages", [(9, 80), (300, 1500), (1500, 4000)])
+def test_rounds_of_sharing_and_cutting_back(hiplib, rows, pages):
+    """fork, cut back to any length, go on: table, counts and bytes follow the plain bookkeeping, more rows than the workgroup has threads among them"""
+    rng = np.random.default_rng(rows)
+    mp = 4
+    pool = paged.KvPool(1, pages, 1, 64)
+    want = fill(pool, rng)
+    book = Book(pages, rows, mp)
+    table, refs = dev(np.array(book.table, dtype=np.int32)), dev(np.array(book.refs, dtype=np.int32))
+    lens = [0] * rows
+    for step in range(6):
+        new = [min(n + int(x), 64 * mp) for n, x in zip(lens, rng.integers(0, 60, rows))]
+        live = sum(x > 0 for x in book.refs)
+        if live + sum(-(-m // 64) - n // 64 for n, m in zip(lens, new)) > pages:
+            new = lens
+        paged.reserve(pool, table, refs, ints(lens), ints(new))
+        given, held = [], list(book.refs)
+        for row, a, b in zip(book.table, lens, new):
+            for c in range(a // 64, -(-b // 64) if b > a else a // 64):
+                if a % 64 and c == a // 64 and row[c] >= 0 and held[row[c]] > 1:
+                    given.append(row[c])
+                    row[c] = book.take()
+                    for x in want:
+                        x[:, row[c]] = x[:, given[-1]]
+                elif row[c] < 0:
+                    row[c] = book.take()
+        for p in given:
+            book.refs[p] -= 1
+        book.same(table.numpy(), refs.numpy())
+        lens = new
+        # most rows continue one of a few
+        parents = [int(p) for p in np.where(rng.random(rows) < 0.8, rng.integers(0, max(rows // 6, 1), rows), np.arange(rows))]
+        free = sum(x == 0 for x in book.refs)
+        if sum(lens[p] % 64 > 0 for p in parents) > free:
+            parents = list(range(rows))
+        table, refs = paged.fork(pool, table, ints(lens), refs, ints(parents))
+        for src, to in book.fork(lens, parents):
+            for x in want:
+                x[:, to] = x[:, src]
+        book.same(table.numpy(), refs.numpy())
+        lens = [lens[p] for p in parents]
+        lens = [int(rng.integers(0, n + 1)) if rng.random() < 0.4 else n for n in lens]
+        paged.trim(pool, table, refs, ints(lens))
+        book.trim(lens)
+        book.same(table.numpy(), refs.numpy())
+        live = [p for p in range(pages) if book.refs[p]]
+        for got, x in zip((pool.k, pool.v, pool.k_scale, pool.v_scale), want):
+            np.testing.assert_array_equal(got.numpy()[:, live], x[:, live])
+    pool.check()
+    assert max(book.refs) > 1
 
 
 # ---- selection ------------------------------------------------------------------------------------------------------------------------
