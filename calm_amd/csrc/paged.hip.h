@@ -1483,6 +1483,10 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_reserve(KvReserveArgs a) {
 			if (c0 < c1 && len % KV_PAGE) {
 				const int p = a.table[(size_t)i * mp + c0];
 				shared = p >= 0 && p < a.n_pages && a.refs[p] > 1 ? p : -1;
+				if (p < 0) { // the row's last tokens are lost: a new page would pass its bytes off as them
+					kv_flag(a.status, KV_BAD_PAGE);
+					++c0;
+				}
 			}
 		}
 		int need = shared >= 0;

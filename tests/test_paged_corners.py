@@ -357,6 +357,18 @@ def test_rounds_of_sharing_and_cutting_back(hiplib, rows, pages):
     assert max(book.refs) > 1
 
 
+@pytest.mark.gpu
+def test_reserve_does_not_make_up_a_page_that_is_lost(hiplib):
+    """a row whose last tokens' page is missing: the entry stays -1 (whatever a free page holds would be read as those tokens), the pages behind it are given"""
+    pool = paged.KvPool(1, 6, 1, 64)
+    table, refs = dev(np.array([[0, -1, -1], [1, -1, -1]], dtype=np.int32)), dev(np.array([1, 1, 0, 0, 0, 0], dtype=np.int32))
+    paged.reserve(pool, table, refs, ints([100, 64]), ints([130, 65]))
+    np.testing.assert_array_equal(table.numpy(), [[0, -1, 2], [1, 3, -1]])
+    np.testing.assert_array_equal(refs.numpy(), [1, 1, 1, 1, 0, 0])
+    with pytest.raises(RuntimeError, match="missing"):
+        pool.check()
+
+
 # ---- selection ------------------------------------------------------------------------------------------------------------------------
 
 
