@@ -153,7 +153,8 @@ extern "C" int decode_beam_hip(struct Transformer* t, int token, int pos, int n_
 			return -1;
 		}
 		const struct KvBatch prompt = {table[0], lens(1), starts0, W, mp, pos, pos, pos};
-		for (int l = 0; l < L; ++l) {
+		int bad = 0;
+		for (int l = 0; l < L && !bad; ++l) {
 			const char* const kc = (const char*)c->kc + (size_t)l * c->kv_layer_bytes;
 			const char* const vc = (const char*)c->vc + (size_t)l * c->kv_layer_bytes;
 			const void *k = kc, *v = vc;
@@ -167,16 +168,14 @@ extern "C" int decode_beam_hip(struct Transformer* t, int token, int pos, int n_
 				                   (unsigned short*)b->wide, pos, c->seq_len, D);
 				k = b->wide, v = b->wide + per, head = (long)pos * D;
 			}
-			if (kv_append_hip(&pool, &prompt, l, k, v, KV_F16, D, head, D, head, g_stream)) {
-				return -1;
-			}
+			bad = kv_append_hip(&pool, &prompt, l, k, v, KV_F16, D, head, D, head, g_stream);
 		}
 		if (c->kvbits == 8) {
 			HIP_CHECK(hipStreamSynchronize(g_stream));
 			HIP_CHECK(hipFree(b->wide));
 			b->wide = nullptr;
 		}
-		if (kv_fork_hip(&pool, table[0], lens(1), refs, b->par, W, mp, table[1], refs, b->work, b->work_bytes, g_stream)) {
+		if (bad || kv_fork_hip(&pool, table[0], lens(1), refs, b->par, W, mp, table[1], refs, b->work, b->work_bytes, g_stream)) {
 			return -1;
 		}
 		std::swap(table[0], table[1]);
