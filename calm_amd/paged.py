@@ -233,7 +233,19 @@ def _rows(x, name: str, rows: int, heads: Optional[int], dim: int):
     return r, h
 
 
-class KvPool:
+class _Fixed:
+    """attributes that are set once: the library has the arrays' addresses and the bounds from then on (`_c`)"""
+
+    def __setattr__(self, name, value):
+        if "_c" in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} is not changed behind its making: make another")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{type(self).__name__}.{name} is not taken away: make another")
+
+
+class KvPool(_Fixed):
     """pages of a cache, for every layer of a model"""
 
     def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, device=None):
@@ -276,17 +288,17 @@ class KvPool:
             import torch
 
             self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
-        self._c = _Pool(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.status.data_ptr(), layers, pages, heads, dim)
-        self._ref = C.byref(self._c)
+        c = _Pool(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.status.data_ptr(), layers, pages, heads, dim)
+        self._ref = C.byref(c)
+        self._c = c
 
     def check(self) -> None:
         """waits for the calls so far and raises RuntimeError if one of them found its pages or batch wanting"""
         if isinstance(self.status, DeviceArray):
             found = int(self.status.numpy()[0])
-            if found:
-                self._c.status = None
-                self.status = DeviceArray.of(np.zeros(1, dtype=np.int32))
-                self._c.status = self.status.data_ptr()
+            if found:  # (in place: a captured graph has the word's address)
+                none = np.zeros(1, dtype=np.int32)
+                self.status._lib.copy_hip(self.status.data_ptr(), none.ctypes.data, none.nbytes)
         else:
             found = int(self.status.item())
             if found:
@@ -297,10 +309,10 @@ class KvPool:
             raise RuntimeError("paged cache: " + "; ".join(w for bit, w in words if found & bit))
 
 
-class KvBatch:
+class KvBatch(_Fixed):
     """Which rows of a call belong to which sequence: rows starts[s] .. starts[s + 1] - 1 are the last tokens of sequence s, which has lens[s]
-    tokens with them.  The arrays are read when a call runs, so a program may change their values between calls; rows, max_rows and
-    max_len are the host's bounds (rows: what the packed row arrays hold; max_rows: of one sequence; max_len: tokens of a sequence)."""
+    tokens with them.  The arrays are read when a call runs, so a program may change their values between calls (other arrays -- the table of a
+    fork, say -- make another batch); rows, max_rows and max_len are the host's bounds (rows: what the packed row arrays hold; max_rows: of one sequence; max_len: tokens of a sequence)."""
 
     def __init__(self, table, lens, starts, rows: int, max_rows: int, max_len: int):
         n, mp = _sizes(table)
@@ -312,9 +324,10 @@ class KvBatch:
         _need(rows >= 0 and 0 <= max_rows <= rows and max_len >= 0, "rows, max_rows and max_len are not negative, max_rows is at most rows")
         self.table, self.lens, self.starts = table, lens, starts
         self.n_seqs, self.rows, self.max_rows, self.max_len = n, rows, max_rows, max_len
-        self._c = _Batch(table.data_ptr(), lens.data_ptr(), starts.data_ptr(), n, mp, rows, max_rows, max_len)
-        self._ref = C.byref(self._c)
         self._work = {}  # workspace sizes of attention
+        c = _Batch(table.data_ptr(), lens.data_ptr(), starts.data_ptr(), n, mp, rows, max_rows, max_len)
+        self._ref = C.byref(c)
+        self._c = c
 
 
 def append(pool: KvPool, batch: KvBatch, k, v, layer: int = 0) -> None:

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from calm_amd import paged
-from test_paged import TYPES, U, Book, Cache, Rig, attention, check_select, dev, from_type, ints, to_type
+from test_paged import TYPES, U, Book, Cache, Fake, Rig, attention, check_select, dev, from_type, ints, to_type
 
 
 # ---- scores and queries out of range --------------------------------------------------------------------------------------------------
@@ -400,3 +400,24 @@ def test_select_equal_beams_at_any_alignment(hiplib, dtype, beams, vocab):
 def test_select_refuses_vocabularies_beyond_its_indexes(hiplib):
     assert hiplib.beam_workspace_hip(1, 1, 1 << 30) > 0
     assert hiplib.beam_workspace_hip(1, 1, (1 << 30) + 1) == -1 and b"2^30 tokens" in hiplib.calm_hip_error()
+
+
+# ---- handles and streams --------------------------------------------------------------------------------------------------------------
+
+
+def test_handles_are_not_changed():
+    """a pool's and a batch's arrays and bounds went to the library when they were made: a change would be seen by the checks here and not by the kernels"""
+    k, v, s = Fake((2, 10, 2, 64, 64), "int8"), Fake((2, 10, 2, 4, 64, 16), "int8"), Fake((2, 10, 2, 4), "float32")
+    t, n, st = Fake((2, 4), "int32"), Fake((2,), "int32"), Fake((3,), "int32")
+    b = paged.KvBatch(t, n, st, 2, 1, 10)
+    for name, x in (("table", t), ("lens", n), ("starts", st), ("rows", 1), ("max_rows", 1), ("max_len", 5), ("n_seqs", 1)):
+        with pytest.raises(AttributeError, match="make another"):
+            setattr(b, name, x)
+    with pytest.raises(AttributeError, match="make another"):
+        del b.table
+    assert (b.table, b.rows) == (t, 2)
+    pool = paged.KvPool.__new__(paged.KvPool)
+    for name, x in (("k", k), ("v", v), ("k_scale", s), ("v_scale", s), ("n_layers", 2), ("_c", None)):  # (as its constructor does, without memory)
+        setattr(pool, name, x)
+    with pytest.raises(AttributeError, match="make another"):
+        pool.k = k
