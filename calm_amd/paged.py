@@ -293,16 +293,20 @@ class KvPool(_Fixed):
         self._c = c
 
     def check(self) -> None:
-        """waits for the calls so far and raises RuntimeError if one of them found its pages or batch wanting"""
+        """waits for the calls so far, on any stream, and raises RuntimeError if one of them found its pages or batch wanting"""
         if isinstance(self.status, DeviceArray):
             found = int(self.status.numpy()[0])
             if found:  # (in place: a captured graph has the word's address)
                 none = np.zeros(1, dtype=np.int32)
                 self.status._lib.copy_hip(self.status.data_ptr(), none.ctypes.data, none.nbytes)
         else:
+            import torch
+
+            torch.cuda.synchronize(self.status.device)  # (.item() waits for the current stream alone)
             found = int(self.status.item())
             if found:
                 self.status.zero_()
+                torch.cuda.synchronize(self.status.device)  # (before a call on another stream finds something new)
         words = [(1, "a page that was needed is missing from the table or outside the pool"), (2, "no page was free"),
                  (4, "a sequence has more new rows than max_rows, or row starts that do not fit the rows"), (8, "a parent outside the table")]
         if found:

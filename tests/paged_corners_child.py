@@ -1,0 +1,55 @@
+"""Corners of calm_amd/paged.py on torch tensors: run by tests/test_paged_corners.py in a process of its own (torch has to come before the library).
+
+Prints one line per check, then ALL OK."""
+import os
+import sys
+
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+
+from calm_amd import paged  # noqa: E402
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def refused(f, words, kind=ValueError):
+    try:
+        f()
+    except kind as e:
+        assert words in str(e), e
+    else:
+        raise AssertionError(words)
+
+
+pool = paged.KvPool(1, 8, 2, 64, device="cuda")
+table, lens = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4), ints([200, 130])
+paged.append(pool, paged.KvBatch(table, lens, ints([0, 200, 330]), rows=330, max_rows=200, max_len=200), *(torch.randn((330, 2, 64), device="cuda") for _ in range(2)))
+batch = paged.KvBatch(table, lens, ints([0, 1, 2]), rows=2, max_rows=1, max_len=200)
+q = torch.randn((2, 4, 64), device="cuda")
+want = paged.attend(pool, batch, q)
+pool.check()
+
+# check() waits for calls on every stream, not on the current one alone; what it found is cleared for good
+side = torch.cuda.Stream()
+big = torch.randn((8192, 8192), device="cuda")
+torch.cuda.synchronize()
+bad = paged.KvBatch(ints([[0, 1, 2, -1], [-1, -1, -1, -1]]), lens, ints([0, 1, 2]), rows=2, max_rows=1, max_len=200)
+torch.cuda.synchronize()
+for rep in range(3):
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            torch.mm(big, big)
+        paged.attend(pool, bad, q)
+    refused(pool.check, "missing", RuntimeError)
+    pool.check()
+with torch.cuda.stream(side):
+    paged.attend(pool, bad, q)
+refused(pool.check, "missing", RuntimeError)
+assert torch.equal(paged.attend(pool, batch, q), want)
+pool.check()
+print("check", flush=True)
+print("ALL OK")

@@ -3,10 +3,15 @@ cut back, equal rows at odd places, handles and streams.
 
 The plain restatements, the inputs' helpers and the tolerances' derivation are tests/test_paged.py's."""
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 from calm_amd import paged
+from conftest import ROOT
 from test_paged import TYPES, U, Book, Cache, Fake, Rig, attention, check_select, dev, from_type, ints, to_type
 
 
@@ -421,3 +426,10 @@ def test_handles_are_not_changed():
         setattr(pool, name, x)
     with pytest.raises(AttributeError, match="make another"):
         pool.k = k
+
+
+@pytest.mark.gpu
+def test_paged_operators_on_torch_tensors_corners():
+    """streams and gradients of torch tensors, in a process of its own: torch has to come before the library"""
+    r = subprocess.run([sys.executable, "-u", os.path.join(ROOT, "tests", "paged_corners_child.py")], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and r.stdout.rstrip().endswith("ALL OK"), r.stdout[-2000:] + r.stderr[-3000:]
