@@ -10,7 +10,7 @@ Arrays are torch tensors on the GPU -- the calls run on torch's current stream o
 library, for programs without torch), which run on the backend's own stream, the one forward_hip is ordered on.  All arrays of a call are
 of one kind and on one device.  Nothing here synchronises but `KvPool.check`, `DeviceArray.numpy` and the creation of DeviceArrays; with
 tensors every call can be captured into a graph.  A call that cannot be right raises ValueError before anything is launched.  There is no
-backward pass: tensors that require gradients are refused unless gradients are switched off.
+backward pass: tensors that require gradients are refused unless gradients are switched off, and tensors with forward-mode tangents always.
 
 torch has to be imported before the library is loaded in a process that uses both (host.require_torch_first).
 """
@@ -125,9 +125,10 @@ def _torch_calls():
     global _torch
     if _torch is None:
         import torch
+        import torch.autograd.forward_ad as forward
 
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle alone, without a Stream object around it
-        _torch = (torch, torch.Tensor, raw or (lambda i: torch.cuda.current_stream(i).cuda_stream), getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device))
+        _torch = (torch, torch.Tensor, raw or (lambda i: torch.cuda.current_stream(i).cuda_stream), getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device), forward)
     return _torch
 
 
@@ -139,11 +140,11 @@ def _on(arrays):
             if not isinstance(a, DeviceArray):
                 raise ValueError("tensors and DeviceArrays in one call")
         return _lib().calm_hip_stream(), None
-    torch, tensor, raw_stream, current = _torch or _torch_calls()
+    torch, tensor, raw_stream, current, forward = _torch or _torch_calls()
     dev = first.device
     if dev.type != "cuda":
         raise ValueError(f"arrays on {dev}: these operators run on the GPU only")
-    grads = torch.is_grad_enabled()
+    grads, tangents = torch.is_grad_enabled(), forward._current_level >= 0
     for a in arrays:
         if not isinstance(a, tensor):
             raise ValueError("tensors and DeviceArrays in one call")
@@ -151,6 +152,8 @@ def _on(arrays):
             raise ValueError(f"arrays on {dev} and on {a.device} in one call")
         if grads and a.requires_grad:
             raise ValueError("there is no backward pass: call under torch.no_grad()")
+        if tangents and forward.unpack_dual(a).tangent is not None:
+            raise ValueError("there is no derivative: a tensor has a forward-mode tangent")
     index = dev.index
     return raw_stream(index), None if index == current() else torch.cuda.device(dev)
 
@@ -183,9 +186,11 @@ def _need(cond, what: str) -> None:
 def _together(arrays) -> None:
     """arrays that are kept for later calls: of one kind, on one device"""
     first = arrays[0]
-    for a in arrays[1:]:
+    for a in arrays:
         if isinstance(a, DeviceArray) != isinstance(first, DeviceArray):
             raise ValueError("tensors and DeviceArrays in one call")
+        if getattr(a, "requires_grad", False):
+            raise ValueError("there is no backward pass, and the arrays of a pool or batch are written in place: detach() them")
         if getattr(a, "device", None) != getattr(first, "device", None):
             raise ValueError(f"arrays on {first.device} and on {a.device} in one call")
 
@@ -346,7 +351,8 @@ def append(pool: KvPool, batch: KvBatch, k, v, layer: int = 0) -> None:
 
 def attend(pool: KvPool, batch: KvBatch, q, layer: int = 0, window: int = 0, sinks: int = 0, scale: Optional[float] = None, out=None):
     """softmax(scale q . K) . V for query rows [rows][query heads][dim]: a row at position p sees tokens j <= p, with a window > 0 those of them
-    with j > p - window or j < sinks; zeros where it sees none.  scale: dim ** -0.5 if not given; out does not overlap q"""
+    with j > p - window or j < sinks; zeros where it sees none.  scale: dim ** -0.5 if not given; out does not overlap q.  Rows behind the last sequence's
+    are not written: of a result that was not given as `out` they are whatever its memory held"""
     dim = pool.head_dim
     _sees(layer, pool.n_layers, window, sinks)
     qr, qh = _rows(q, "q", batch.rows, None, dim)

@@ -52,4 +52,18 @@ refused(pool.check, "missing", RuntimeError)
 assert torch.equal(paged.attend(pool, batch, q), want)
 pool.check()
 print("check", flush=True)
+
+# no derivative is dropped silently: forward-mode tangents and arrays of a pool that require gradients are refused as reverse-mode ones are
+import torch.autograd.forward_ad as fwd  # noqa: E402
+
+with fwd.dual_level():
+    refused(lambda: paged.attend(pool, batch, fwd.make_dual(q, torch.ones_like(q))), "no derivative")
+    rows = torch.randn((2, 2, 64), device="cuda")
+    refused(lambda: paged.append(pool, batch, rows, fwd.make_dual(rows, rows)), "no derivative")
+    x = torch.randn((2, 50), device="cuda")
+    refused(lambda: paged.beam_select(fwd.make_dual(x, x), torch.zeros((1, 2), device="cuda")), "no derivative")
+    assert torch.equal(paged.attend(pool, batch, q), want)  # (tensors without tangents)
+assert torch.equal(paged.attend(pool, batch, q), want)
+refused(lambda: paged.KvPool.over(pool.k, pool.v, pool.k_scale.clone().requires_grad_(), pool.v_scale), "no backward")
+print("forward mode", flush=True)
 print("ALL OK")
