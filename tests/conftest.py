@@ -21,7 +21,8 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 GOLDEN = os.path.join(ROOT, "tests", "golden")
-REFERENCE = "/root/reference"
+# the reference's tree; a folder without its sources is none (tests that read them skip where it is not a folder)
+REFERENCE = "/root/reference" if os.path.exists("/root/reference/src/model.h") else "/root/reference/absent"
 
 GOLDEN_CASES = ["tiny_fp16", "tiny_fp8", "tiny_gf4", "moe_fp8", "ln_gelu_clip_fp16", "par_fp8", "bias_tied_gf4", "sink_fp16", "ragged_fp8",
                 "partial_rope_fp16", "dbrx_like_fp8", "mqa_hd96_fp16", "moe_gf4", "hd256_sink_fp8", "moe6_fp8", "moe12_ln_fp16",
@@ -63,7 +64,12 @@ def _gpu_count():
 
 def pytest_collection_modifyitems(config, items):
     """a gpu-marked test on a box without a GPU is a hard error only when -m gpu was asked for;
-    in a plain `pytest tests/` run on CPU it is skipped"""
+    in a plain `pytest tests/` run on CPU it is skipped.
+
+    Without the reference's own build (oracle/_ref) the full-depth DBRX test is held against the restatement, which takes another expert at a near-tie
+    (gate logits 1e-4 apart, where two orders of summation differ by 2e-4): it runs last then, so that a run that ends at a failure has run the others"""
+    if not os.path.exists(os.path.join(ROOT, "oracle", "_ref", "libcalm_ref.so")):
+        items.sort(key=lambda item: item.name == "test_dbrx_132b_fp8_full_depth")
     if _gpu_count() > 0:
         return
     asked = "gpu" in (config.getoption("-m") or "") and "not gpu" not in (config.getoption("-m") or "")
