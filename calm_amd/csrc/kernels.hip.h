@@ -261,14 +261,14 @@ __device__ __forceinline__ float fma_mix_hi(unsigned h2, float x, float acc) {
 }
 
 // acc += dot(16-byte lane-load `v`, its G activations), as a 2-wide accumulator (even/odd columns)
-// so that every multiply-add is a v_pk_fma_f32 on register pairs that are already adjacent: the
-// converted weight pair, the activation pair from ds_read_b128, the accumulator pair.
+// so that both columns of a multiply-add are register pairs that are already adjacent: the converted weight pair, the activation pair
+// from ds_read_b128, the accumulator pair.  (Two v_fma_f32 a pair: packed fp32 instructions are switched off, build.py.)
 // xp points at this lane's first float4 of the chunk in the swizzled LDS image; float4 #i of the
 // lane is at xp[i * ROW] (ROW = Fmt<DB>::ROW slots).
 // X(i): the lane's float4 #i of the chunk's activations -- from the LDS image (dot16) or from registers (run_rows_impl XR)
 template <int DB, class XF>
 __device__ __forceinline__ f32x2 dot16x(u32x4 v, XF X, f32x2 acc) {
-	// (fp16 / fp8: a second, call-local accumulator pair halves the length of the dependent v_pk_fma chain
+	// (fp16 / fp8: a second, call-local accumulator pair halves the length of the dependent fma chain
 	// -- PMC showed 30-40 % of wave cycles in issue stalls with one chain per row)
 	if constexpr (DB == 16) {
 		f32x2 acc_b = {0.f, 0.f};
