@@ -430,8 +430,11 @@ __global__ __launch_bounds__(64) void k_kv_read(KvReadArgs a) {
 //   k_kv_chunk   one binary16 after the row is scaled by a power of two to at most 1 (fp16 and bf16 rows lose nothing above 2^-14 of their largest
 //                element), fp32 rows as the sum of two (22 bits); scores are fp32 sums.
 // Scores are then fp32, times the block's K scale.  A weight goes into the second product with its block's V scale, relative to the largest such
-// that the ROW met (KvRefs), as one binary16 for fp16 / bf16 outputs -- off by at most 2^-11, half a step, each its own way, and outputs are
-// averages of them -- and as the sum of two for fp32 (2^-22); sums are fp32.  Below 2^-20 of the largest a weight keeps an absolute 2^-31 of it.
+// that the ROW met (KvRefs), as one binary16 for fp16 / bf16 outputs -- off by at most 2^-11, half a step -- and as the sum of two for fp32 (2^-22); sums
+// are fp32.  Below 2^-20 of the largest a weight keeps an absolute 2^-31 of it.  fp16 outputs, whose own rounding the weights' comes up to, take the
+// sum of the ROUNDED weights, so that they are averages of V's and a token that has all the weight is returned exactly: off by 2.6e-4 of their
+// root mean square, 2.9e-4 with the sum of the unrounded (2.07e-4 is the output's own; for bf16 it is 1.66e-3, and nothing is gained) -- unless a block's V scale
+// is so far below the reference (KV_NEAR) that its weights round to few bits or none, and the sum would lose what they weigh.
 
 struct KvAttnArgs {
 	KvLayer p;
@@ -488,18 +491,18 @@ __device__ __forceinline__ int kv_row_exp(float top) {
 // the row itself sees.  Sums of weights are relative to 2^m; what goes into the product with V's codes is y_j = 2^(x_j + v_j - mv + KV_LIFT), so
 // nothing that a row does not see, or gives no weight, takes bits from it, however large its V.  A block's share of the sum of weights is
 // that of its y, times 2^k, k = mv - KV_LIFT - m - v.  k is held between -126 and KV_REACH: above, V is 2^-53 of what the row's output is made of and
-// takes part as if it were no smaller; below, the weight is 2^-118 of the largest and nothing in 32 bits.  A reference stays unless it is passed by 2^8:
-// weights up to 2^8 are no less exact, and sums are seldom rescaled.  y <= 2^15 is inside binary16; KV_LIFT moves its subnormals away.
-constexpr float KV_LIFT = 7.f, KV_REACH = 60.f;
+// takes part as if it were no smaller; below, the weight is 2^-118 of the largest and nothing in 32 bits.  The references stay unless one is passed by
+// 2^8 (weights up to 2^8 are no less exact, and sums are seldom rescaled), and then both follow, so that k is what V's scales make it: -7 for equal
+// ones, and up to KV_NEAR where the rounded weights may stand for the weights (fp16).  y <= 2^15 is inside binary16; KV_LIFT moves its subnormals away.
+constexpr float KV_LIFT = 7.f, KV_REACH = 60.f, KV_NEAR = -2.f;
 struct KvRefs {
 	float m, mv, rm, rv, gap, m0, mv0;
 	bool moved;
 	__device__ __forceinline__ KvRefs(float m0_, float mv0_, float top, float topv) : m0(m0_), mv0(mv0_) {
-		m = top > m0 + 8.f ? ceilf(top) : m0;
-		mv = topv > mv0 + 8.f ? ceilf(topv) : mv0;
+		moved = top > m0 + 8.f || topv > mv0 + 8.f;
+		m = moved ? ceilf(top) : m0, mv = moved ? ceilf(topv) : mv0;
 		rm = m == -__builtin_inff() ? 0.f : m, rv = mv == -__builtin_inff() ? 0.f : mv; // (no token seen yet)
 		gap = rv - KV_LIFT - rm;
-		moved = m != m0 || mv != mv0;
 	}
 	__device__ __forceinline__ float of_l() const { // what rescales the sums (m0 = -inf: 0)
 		return kv_exp2(m0 - rm);
@@ -508,6 +511,11 @@ struct KvRefs {
 		return kv_exp2(mv0 - rv);
 	}
 };
+// acc + the two binary16 numbers of a word
+__device__ __forceinline__ float kv_add2(float acc, unsigned h2) {
+	const kv_f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+	return __builtin_amdgcn_fdot2(__builtin_bit_cast(kv_f16x2, h2), one, acc, false);
+}
 // sum of y_j V_j over the sum of weights, with V's scale back in
 __device__ __forceinline__ float kv_result(float y, float rm, float rv) {
 	return __builtin_amdgcn_ldexpf(y, (int)(rv - 127.f - KV_LIFT - rm));
@@ -649,7 +657,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 	constexpr int NQ = 3;
 	unsigned qd[NQ][KW];
 	float x[D / 4];
-	unsigned top = 0;
+	unsigned big = 0;
 #pragma unroll
 	for (int i = 0; i < D / 16; ++i) {
 		float y[4];
@@ -658,17 +666,17 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		for (int j = 0; j < 4; ++j) {
 			x[4 * i + j] = y[j];
 			const unsigned u = __builtin_bit_cast(unsigned, y[j]) & 0x7fffffffu;
-			top = top > u ? top : u;
+			big = big > u ? big : u;
 		}
 	}
-	const unsigned t1 = __shfl_xor(top, 16);
-	top = top > t1 ? top : t1;
-	const unsigned t2 = __shfl_xor(top, 32);
-	top = top > t2 ? top : t2;
-	const int e0 = kv_row_exp(__builtin_bit_cast(float, top)), e = e0 < -119 ? -119 : e0; // (2^119 * 127 is a number; smaller rows' scores are none)
+	const unsigned t1 = __shfl_xor(big, 16);
+	big = big > t1 ? big : t1;
+	const unsigned t2 = __shfl_xor(big, 32);
+	big = big > t2 ? big : t2;
+	const int e0 = kv_row_exp(__builtin_bit_cast(float, big)), e = e0 < -119 ? -119 : e0; // (2^119 * 127 is a number; smaller rows' scores are none)
 	const float inv = kv_exp2i(-e) * 127.f;
 	// (a row with an infinity or a NaN is NaN)
-	const float qf = top >= 0x7f800000u ? __builtin_nanf("") : kv_exp2i(e) * a.scale * (1.f / 127.f);
+	const float qf = big >= 0x7f800000u ? __builtin_nanf("") : kv_exp2i(e) * a.scale * (1.f / 127.f);
 #pragma unroll
 	for (int i = 0; i < KW; ++i) {
 		unsigned w[NQ];
@@ -678,7 +686,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 #pragma unroll
 		for (int j = 0; j < 4; ++j) {
-			float y = top >= 0x7f800000u ? 0.f : x[4 * i + j] * inv;
+			float y = big >= 0x7f800000u ? 0.f : x[4 * i + j] * inv;
 #pragma unroll
 			for (int n = 0; n < NQ; ++n) {
 				const float r = __builtin_rintf(y);
@@ -692,7 +700,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 	}
 	kv_f32x4 o[ND];
-	float m = -__builtin_inff(), mv = -__builtin_inff(), l = 0.f;
+	float m = -__builtin_inff(), mv = m, top = m, topv = m, l = 0.f; // (top, topv: the largest met, which the references trail)
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
 		o[d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
@@ -748,7 +756,6 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 		// every token of the page seen by every row of the tile?
 		const bool whole = j0 + KV_PAGE - 1 <= p_min && (a.window <= 0 || j0 > p_max - a.window || j0 + KV_PAGE <= a.sinks);
-		float top = -__builtin_inff(), topv = -__builtin_inff();
 #pragma unroll
 		for (int t = 0; t < 4; ++t) {
 			const float f = kscale[t] * qf;
@@ -782,20 +789,31 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 		m = ref.m, mv = ref.mv;
 		kv_f16x8 pf[2], pl[HL ? 2 : 1];
+		const auto weigh = [&](auto rounded) {
 #pragma unroll
-		for (int t = 0; t < 4; ++t) {
-			const float k = __builtin_amdgcn_fmed3f(ref.gap - lv[t], -126.f, KV_REACH), from = -(ref.rm + k);
-			float sum = 0.f;
+			for (int t = 0; t < 4; ++t) {
+				const float k = __builtin_amdgcn_fmed3f(ref.gap - lv[t], -126.f, KV_REACH), from = -(ref.rm + k);
+				float sum = 0.f;
 #pragma unroll
-			for (int e = 0; e < 4; ++e) {
-				const float y = kv_exp2(__builtin_fmaf(sc[t][e], kscale[t], from));
-				sum += y;
-				pf[t >> 1][4 * (t & 1) + e] = (_Float16)y;
-				if constexpr (HL) {
-					pl[t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[t >> 1][4 * (t & 1) + e]);
+				for (int e = 0; e < 4; ++e) {
+					const float y = kv_exp2(__builtin_fmaf(sc[t][e], kscale[t], from));
+					sum += rounded ? 0.f : y;
+					pf[t >> 1][4 * (t & 1) + e] = (_Float16)y;
+					if constexpr (HL) {
+						pl[t >> 1][4 * (t & 1) + e] = (_Float16)(y - (float)pf[t >> 1][4 * (t & 1) + e]);
+					}
 				}
+				if constexpr (rounded) {
+					const u32x4 w = __builtin_bit_cast(u32x4, pf[t >> 1]);
+					sum = kv_add2(kv_add2(0.f, w[2 * (t & 1)]), w[2 * (t & 1) + 1]);
+				}
+				l = __builtin_fmaf(sum, kv_exp2(k), l);
 			}
-			l = __builtin_fmaf(sum, kv_exp2(k), l);
+		};
+		if (DT == KV_F16 && !__ballot(ref.gap > fminf(fminf(lv[0], lv[1]), fminf(lv[2], lv[3])) + KV_NEAR)) {
+			weigh(std::integral_constant<bool, DT == KV_F16>());
+		} else {
+			weigh(std::false_type());
 		}
 #pragma unroll
 		for (int d = 0; d < ND; ++d) {
@@ -1043,7 +1061,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			}
 		}
 	}
-	float m = -__builtin_inff(), mv = -__builtin_inff(), l = 0.f;
+	float m = -__builtin_inff(), mv = m, top = m, topv = m, l = 0.f; // (top, topv: the largest met, which the references trail)
 	kv_f32x16 o[ND], zero;
 #pragma unroll
 	for (int e = 0; e < 16; ++e) {
@@ -1190,7 +1208,6 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 					f[b] = 1.f;
 				}
 			}
-			float top = m, topv = mv;
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
 				float t = -__builtin_inff();
@@ -1207,21 +1224,32 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			l *= ref.of_l();
 			const float by = ref.of_o();
 			const int gap = (int)ref.gap;
+			const auto weigh = [&](auto rounded) {
 #pragma unroll
-			for (int b = 0; b < 4; ++b) {
-				const int k = min(max(gap - lv[b], -126), (int)KV_REACH);
-				const float from = -(ref.rm + (float)k);
-				float sum = 0.f;
+				for (int b = 0; b < 4; ++b) {
+					const int k = min(max(gap - lv[b], -126), (int)KV_REACH);
+					const float from = -(ref.rm + (float)k);
+					float sum = 0.f;
 #pragma unroll
-				for (int e = 0; e < 8; ++e) {
-					const float y = kv_exp2(__builtin_fmaf(sc[b >> 1][8 * (b & 1) + e], f[b], from));
-					sum += y;
-					pf[b][e] = (_Float16)y;
-					if constexpr (HL) {
-						pl[b][e] = (_Float16)(y - (float)pf[b][e]);
+					for (int e = 0; e < 8; ++e) {
+						const float y = kv_exp2(__builtin_fmaf(sc[b >> 1][8 * (b & 1) + e], f[b], from));
+						sum += rounded ? 0.f : y;
+						pf[b][e] = (_Float16)y;
+						if constexpr (HL) {
+							pl[b][e] = (_Float16)(y - (float)pf[b][e]);
+						}
 					}
+					if constexpr (rounded) {
+						const u32x4 w = __builtin_bit_cast(u32x4, pf[b]);
+						sum = kv_add2(kv_add2(kv_add2(kv_add2(0.f, w[0]), w[1]), w[2]), w[3]);
+					}
+					l = __builtin_fmaf(sum, kv_exp2i(k), l);
 				}
-				l = __builtin_fmaf(sum, kv_exp2i(k), l);
+			};
+			if (DT == KV_F16 && !__ballot(gap > min(min(lv[0], lv[1]), min(lv[2], lv[3])) + (int)KV_NEAR)) {
+				weigh(std::integral_constant<bool, DT == KV_F16>());
+			} else {
+				weigh(std::false_type());
 			}
 			if (__ballot(ref.moved)) {
 #pragma unroll

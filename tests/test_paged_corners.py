@@ -100,6 +100,27 @@ def test_an_outlier_in_a_row_costs_the_others_nothing(hiplib, dtype, dim, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,tokens", [(1, 300), (45, 300), (1, 4100), (45, 4100)])
+def test_a_row_that_weighs_one_token_returns_its_value(hiplib, dtype, rows, tokens):
+    """one token's score 30 to 60 above all others (0): their weights, e^-30 in sum at most 4100 * 1e-13 = 4e-10, are nothing, so the output is that token's V -- exactly
+    for 16-bit rows, whose sum of weights is that of the weights as they go into the product (V, a code of 7 bits times a power of two, is a number of the type), and
+    to 2^-21 for fp32 ones: the weight as two halves (2^-22), the reciprocal, one product"""
+    r = Rig(1, tokens, 1, 64, np.random.default_rng(37))
+    k = np.zeros((tokens, 1, 64))
+    at = tokens // 3
+    k[at, 0] = np.where(r.rng.random(64) < 0.5, 1.0, -1.0)
+    r.add([tokens], "float32", k=to_type(k, "float32"))
+    q = k[at, 0] * (30 + 30 * r.rng.random((rows, 4, 1))) * 8 / 64  # q . K * 64 ** -0.5 = 30 .. 60
+    got = from_type(paged.attend(r.pool, r.batch([rows]), dev(to_type(q, dtype), dtype)).numpy(), dtype)
+    want = np.broadcast_to(r.v.values(0)[at, 0], got.shape)
+    if dtype == "float32":
+        np.testing.assert_allclose(got, want, rtol=2.0 ** -21, atol=1e-9 * np.abs(r.v.values(0)).max())
+    else:
+        np.testing.assert_allclose(got, want, rtol=0, atol=1e-7)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30])
 @pytest.mark.parametrize("rows", [12, 50])
 def test_the_widest_windows_beside_rows_before_position_0(hiplib, rows, window):
