@@ -756,6 +756,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 		// every token of the page seen by every row of the tile?
 		const bool whole = j0 + KV_PAGE - 1 <= p_min && (a.window <= 0 || j0 > p_max - a.window || j0 + KV_PAGE <= a.sinks);
+		float least = 255.f; // the smallest V scale that this lane's tokens have (behind the row's mask a scale may be anything)
 #pragma unroll
 		for (int t = 0; t < 4; ++t) {
 			const float f = kscale[t] * qf;
@@ -776,6 +777,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 				kscale[t] = f;
 			}
 			top = fmaxf(top, x), topv = fmaxf(topv, x + lv[t]);
+			least = fminf(least, x > -__builtin_inff() ? lv[t] : 255.f);
 		}
 		top = kv_max32(kv_max16(top)), topv = kv_max32(kv_max16(topv));
 		const KvRefs ref(m, mv, top, topv);
@@ -810,7 +812,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 				l = __builtin_fmaf(sum, kv_exp2(k), l);
 			}
 		};
-		if (DT == KV_F16 && !__ballot(ref.gap > fminf(fminf(lv[0], lv[1]), fminf(lv[2], lv[3])) + KV_NEAR)) {
+		if (DT == KV_F16 && !__ballot(ref.gap > least + KV_NEAR)) {
 			weigh(std::integral_constant<bool, DT == KV_F16>());
 		} else {
 			weigh(std::false_type());
@@ -1208,6 +1210,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 					f[b] = 1.f;
 				}
 			}
+			int least = 255; // (as in k_kv_decode)
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
 				float t = -__builtin_inff();
@@ -1217,6 +1220,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 				}
 				t *= f[b];
 				top = fmaxf(top, t), topv = fmaxf(topv, t + (float)lv[b]);
+				least = min(least, t > -__builtin_inff() ? lv[b] : 255);
 			}
 			top = kv_max32(top), topv = kv_max32(topv);
 			const KvRefs ref(m, mv, top, topv);
@@ -1246,7 +1250,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 					l = __builtin_fmaf(sum, kv_exp2i(k), l);
 				}
 			};
-			if (DT == KV_F16 && !__ballot(gap > min(min(lv[0], lv[1]), min(lv[2], lv[3])) + (int)KV_NEAR)) {
+			if (DT == KV_F16 && !__ballot(gap > least + (int)KV_NEAR)) {
 				weigh(std::integral_constant<bool, DT == KV_F16>());
 			} else {
 				weigh(std::false_type());

@@ -121,6 +121,27 @@ def test_a_row_that_weighs_one_token_returns_its_value(hiplib, dtype, rows, toke
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+def test_what_lies_behind_the_tokens_does_not_matter(hiplib, dtype, rows):
+    """the same bits whatever the pages hold behind a sequence's tokens, in rows and blocks of one tile that some rows do not see, and in pages of nobody"""
+    got = []
+    for junk in (0x00, 0x01, 0x3F, 0x7F, 0xFF):
+        r = Rig(2, 1000, 2, 64, np.random.default_rng(38))
+        for a in (r.pool.k, r.pool.v, r.pool.k_scale, r.pool.v_scale):
+            b = np.full(a.nbytes, junk, dtype=np.uint8)
+            a._lib.copy_hip(a.data_ptr(), b.ctypes.data, b.nbytes)
+        r.add([993, 70], "float32")
+        q = to_type(r.rng.standard_normal((2 * rows, 8, 64)), dtype)
+        b = r.batch([rows, rows])
+        got.append([paged.attend(r.pool, b, dev(q, dtype), window=w).numpy() for w in (0, 37)])
+        r.pool.check()
+    for x in got[1:]:
+        for a, b in zip(x, got[0]):
+            np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30])
 @pytest.mark.parametrize("rows", [12, 50])
 def test_the_widest_windows_beside_rows_before_position_0(hiplib, rows, window):
