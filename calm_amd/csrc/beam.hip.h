@@ -124,7 +124,7 @@ __device__ __forceinline__ float beam_key_value(unsigned long long key) {
 	return __builtin_bit_cast(float, b >> 31 ? b & 0x7fffffffu : ~b);
 }
 
-// Measured: 128 rows of 128256 fp32 logits 16.8 us = 3.9 TB/s, 80 rows of 32000 at 16 beams 10 us, 4 rows of 32000 5.
+// Measured: 128 rows of 128256 fp32 logits 16.8 us = 3.9 TB/s, 80 rows of 32000 at 16 beams 10.9 us, 128 at 32 beams 18.6, 4 rows of 32000 at 4 beams 5.4.
 // grid = (chunks, rows)
 template <int DT>
 __global__ __launch_bounds__(256) void k_beam_rows(BeamArgs a) {
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(1024) void k_beam_pick(BeamArgs a) {
 	// The rows' lists are in order.  Up to 16 rows: a candidate's place in the group is its place in its own list plus, for every other row, how many
 	// of that row are better, found by halving, a thread per candidate and other row.  More: one wave, a row a lane, takes the best of their
 	// heads W times.  Equal totals: the lower row first (its indices are lower), a row's own in its order.  Measured, the one and the other, this whole
-	// kernel: 16 x 8 rows of 16 chunks 5.8 / 7.7 us, 5 x 16 rows of 4 14.5 / 16.3, 4 x 32 rows of 4 158 / 40.
+	// kernel: 1 x 4 rows of 4 chunks 4.5 / 5.0 us, 16 x 8 rows of 16 9.7 / 11.4, 5 x 16 rows of 4 14.2 / 13.8, 4 x 32 rows of 4 157 / 37.
 	if (W <= 16) {
 		for (int it = threadIdx.x; it < W * W * W; it += threads) {
 			const int c = it / W, u = it - c * W, w = c / W;

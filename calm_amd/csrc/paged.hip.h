@@ -537,10 +537,10 @@ __device__ __forceinline__ void kv_put(const KvAttnArgs& a, bool direct, size_t 
 // operands they are (no conversion: that is what whole-number scores are for), asks for the next page's K behind the first product and for its
 // V behind the second, so 8 - 16 KiB per wave are in flight throughout.  (Two sets of registers, a whole page ahead: slower.)  The waves' sums
 // meet in LDS; ranges of one row meet in k_kv_merge.  Eight waves for heads up to 128: four, with twice the workgroups, lose 5 - 10 % to the
-// waits at both ends of a workgroup (64 sequences of 91 - 8191, heads of 64: 39.6 -> 36.2 us).
-// Measured, one row a sequence: 24 x 13.9 - 16.4k tokens, 8 kv heads of 128: 136 us, 746 MB = 5.5 TB/s; 8 x 4093 (fp32): 17.8 us + 3.9 for the join, 67 MB = 3.1;
-// 64 x 91 - 8191, 4 of 64: 36 us, 137 MB = 3.8 (the longest sequences' chain of pages is what remains); up to five rows of 16 x 6 - 9k under a window of
-// 1024: 13.7 us, 35 MB = 2.5.
+// waits at both ends of a workgroup (64 sequences of 91 - 8191, heads of 64, with two digits: 39.6 -> 36.2 us).
+// Measured, one row a sequence: 24 x 13.9 - 16.4k tokens, 8 kv heads of 128: 136 us, 746 MB = 5.5 TB/s; 8 x 4093 (fp32): 17.2 us + 3.9 for the join, 67 MB = 3.2;
+// 64 x 91 - 8191, 4 of 64: 39.6 us, 137 MB = 3.5 (the longest sequences' chain of pages is what remains); up to five rows of 16 x 6 - 9k under a window of
+// 1024: 14.1 us, 35 MB = 2.5.
 // grid = (splits, kv heads x tiles, seqs)
 template <int D, int DT, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnArgs a) {
@@ -940,13 +940,14 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 	}
 }
 
-// Many rows (a prompt chunk): the matrix cores bound it.  A workgroup takes 128 rows (32 per wave) of one sequence and kv head and walks
+// Many rows (a prompt chunk).  A workgroup takes 128 rows (32 per wave) of one sequence and kv head and walks
 // the pages they see; a page's codes become binary16 ONCE per workgroup on their way into LDS (two buffers: the next page's loads are in
 // flight while a page is computed), laid out so that every operand is one 16-byte read of consecutive lanes.
-// Measured: 2049 rows of 32 heads (8 kv heads of 128) on 4099 tokens 166 - 174 us = 600 TFLOP/s; five ragged chunks of up to 1021 rows of 32 heads
-// (4 kv heads of 64) behind a window of 2048 73 us.  A page costs a wave 32 matrix instructions of 32 cycles (heads of 128) and 280 vector ones
-// of 4 (exponentials 8), and a matrix instruction keeps the vector unit for 16 of its cycles: the vector unit is what bounds it, two
-// workgroups to a CU reach 70 % of that, and the heaviest tiles (65 pages, 49 on average) end last.  Tried and slower: PV of a page with QK of
+// Measured: 2049 rows of 32 heads (8 kv heads of 128) on 4099 tokens 162 - 172 us = 620 TFLOP/s; five ragged chunks of up to 1021 rows of 32 heads
+// (4 kv heads of 64) behind a window of 2048 75 us.  What bounds it is the chain of pages of the heaviest tiles (65, 49 on average; 2.5 us each): of the first
+// shape's 387k cycles the matrix unit is busy 100k and vector instructions issue 161k, with 1.32 of two possible waves on a SIMD on average -- light
+// tiles end early, nothing follows them -- and a wave issues 46 % of its time, waits to issue 30 and for memory, LDS and barriers 24.  (Under the
+// window: 200k cycles, 25k and 73k, 1.05 waves.)  Tried and slower: PV of a page with QK of
 // the next in one phase, the other phase's waves beside it behind barriers (eight waves of 256 rows: 199 us; four waves: 181), products of
 // neighbouring pages interleaved within a wave (257 us), light tiles behind heavy ones on a CU (187).
 // grid = row tiles x seqs x splits x kv heads
@@ -1491,34 +1492,83 @@ struct KvReserveArgs {
 };
 
 // pages for the tokens [lens[r], lens_new[r]) of every row: rows in order, a row's pages in order, the lowest free page each.  A row that was cut back
-// into a page which other rows list (refs > 1 where its tokens end inside the page) is about to write there: it gets a page of its own with the old
-// one's bytes, or, with no page free, loses the entry.  The pages so given up count as free from the next call on, so nothing is copied over before it
-// has been read.  This workgroup copies them itself: a list for other workgroups would take a workspace, and such rows are few.  Measured: a token for each of 48 rows
-// of 33 pages 2.6 us, 500 rows 2.7, with nothing to copy; k_kv_trim of the same rows 2.1 and 1.9.
+// lists pages that other rows list, too (refs > 1), and is about to write there: it gives them up for pages of its own.  The one that its tokens end in
+// takes the old one's bytes with it, or, with no page free, the row loses the entry; it counts as free from the next call on, so nothing is copied over before
+// it has been read.  This workgroup copies the bytes itself: a list for other workgroups would take a workspace, and such rows are few.  Who gives up
+// what is settled by the counts at the beginning, so it does not depend on the rows' order.  Measured: a token for each of 48 rows of 33 pages 3.0 us, 500
+// rows 3.4, with nothing to copy; k_kv_trim of the same rows 2.1 and 1.9.
 __global__ __launch_bounds__(KV_BOOK) void k_kv_reserve(KvReserveArgs a) {
-	__shared__ int list[KV_MAX_ROWS], from[KV_MAX_ROWS], into[KV_MAX_ROWS], sm[KV_BOOK / 64], n_own;
+	__shared__ int list[KV_MAX_ROWS], from[KV_MAX_ROWS], into[KV_MAX_ROWS], sm[KV_BOOK / 64], n_own, n_left;
 	const int tid = threadIdx.x, n = a.n_rows, mp = a.max_pages;
 	if (tid == 0) {
-		n_own = 0;
+		n_own = 0, n_left = 0;
 	}
-	// a row at a time per thread; a call adds few pages to a row (a prompt: its pages)
-	for (int i0 = 0; i0 < n; i0 += KV_BOOK) {
-		const int i = i0 + tid;
-		int c0 = 0, c1 = 0, shared = -1; // shared: the page that the row's tokens end in, if others list it
-		if (i < n) {
-			const int len = a.lens[i] < 0 ? 0 : a.lens[i], to = a.lens_new[i] < 0 ? 0 : a.lens_new[i];
-			c0 = len / KV_PAGE, c1 = to > len ? (to - 1) / KV_PAGE + 1 : c0;
-			if (c1 > mp) {
-				kv_flag(a.status, KV_NO_PAGE);
-				c1 = mp;
-			}
-			if (c0 < c1 && len % KV_PAGE) {
-				const int p = a.table[(size_t)i * mp + c0];
-				shared = p >= 0 && p < a.n_pages && a.refs[p] > 1 ? p : -1;
-				if (p < 0) { // the row's last tokens are lost: a new page would pass its bytes off as them
-					kv_flag(a.status, KV_BAD_PAGE);
-					++c0;
+	// entries [c0, c1) of row i are to be pages of its own; cut: the first of them holds tokens already
+	const auto range = [&](int i, int& c0, int& c1, bool& cut) {
+		const int len = a.lens[i] < 0 ? 0 : a.lens[i], to = a.lens_new[i] < 0 ? 0 : a.lens_new[i];
+		c0 = len / KV_PAGE, c1 = to > len ? (to - 1) / KV_PAGE + 1 : c0, cut = len % KV_PAGE;
+		c1 = c1 > mp ? mp : c1;
+		return to > len && (to - 1) / KV_PAGE >= mp;
+	};
+	__syncthreads();
+	for (int i = tid; i < n; i += KV_BOOK) {
+		int c0, c1;
+		bool cut;
+		if (range(i, c0, c1, cut)) {
+			kv_flag(a.status, KV_NO_PAGE);
+		}
+		list[i] = -1; // (until pages are looked for: the page that the row's tokens end in, if others list it)
+		for (int c = c0; c < c1; ++c) {
+			int* const entry = a.table + (size_t)i * mp + c;
+			const int p = *entry;
+			if (p >= 0 && p < a.n_pages && a.refs[p] > 1) {
+				if (c == c0 && cut) {
+					list[i] = p;
+				} else { // (below: after every row has looked at the counts)
+					*entry = -2 - p;
+					n_left = 1;
 				}
+			} else if (p < 0) {
+				*entry = -1;
+			}
+		}
+	}
+	__syncthreads();
+	int mine[KV_MAX_ROWS / KV_BOOK]; // list[] of this thread's rows
+#pragma unroll
+	for (int k = 0; k < KV_MAX_ROWS / KV_BOOK; ++k) {
+		mine[k] = k * KV_BOOK + tid < n ? list[k * KV_BOOK + tid] : -1;
+	}
+	if (n_left) {
+		for (int i = tid; i < n; i += KV_BOOK) {
+			int c0, c1;
+			bool cut;
+			range(i, c0, c1, cut);
+			for (int c = c0; c < c1; ++c) {
+				int* const entry = a.table + (size_t)i * mp + c;
+				if (*entry < -1) {
+					atomicSub(&a.refs[-2 - *entry], 1);
+					*entry = -1;
+				}
+			}
+		}
+		__threadfence();
+	}
+	__syncthreads();
+	// a row at a time per thread; a call adds few pages to a row (a prompt: its pages)
+#pragma unroll
+	for (int k = 0; k < KV_MAX_ROWS / KV_BOOK; ++k) {
+		if (k * KV_BOOK >= n) {
+			break;
+		}
+		const int i = k * KV_BOOK + tid;
+		int c0 = 0, c1 = 0, shared = mine[k];
+		if (i < n) {
+			bool cut;
+			range(i, c0, c1, cut);
+			if (c0 < c1 && cut && a.table[(size_t)i * mp + c0] < 0) { // the row's last tokens are lost: a new page would pass its bytes off as them
+				kv_flag(a.status, KV_BAD_PAGE);
+				++c0;
 			}
 		}
 		int need = shared >= 0;
@@ -1542,8 +1592,8 @@ __global__ __launch_bounds__(KV_BOOK) void k_kv_reserve(KvReserveArgs a) {
 						__hip_atomic_store(a.refs + p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 					}
 					if (shared >= 0) {
-						const int k = atomicAdd(&n_own, 1);
-						from[k] = shared, into[k] = p;
+						const int own = atomicAdd(&n_own, 1);
+						from[own] = shared, into[own] = p;
 						shared = -1;
 					}
 					*entry = p;

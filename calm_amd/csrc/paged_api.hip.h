@@ -163,8 +163,8 @@ KvCut kv_cut(const struct KvPool* p, const struct KvBatch* b, int n_heads, int t
 	}
 	// What a cut into n ranges costs, in steps of a workgroup (a page for each of its waves, about 2 us): workgroups run in rounds of one
 	// to a CU (their registers fill it), a round begins with look-ups and first loads (2 steps), and ranges are joined by a second launch.
-	// Measured, n = 1 / 2 / 4 / 8, in us: 8 sequences of 4093, 8 kv heads of 128 (64 workgroups uncut) 32.2 / 24.7 / 21.8 / 30.7; 64 of 91 - 8191, 4 kv
-	// heads of 64 (256) 36.3 / 43.2 / 50.2 / 63.5; 24 of 13.9 - 16.4k (192) 136 / 158 / 144 / 151; 16 under a window of 1024 (256) 13.7 / 27.3 / 27.8.
+	// Measured, n = 1 / 2 / 4 / 8, in us: 8 sequences of 4093, 8 kv heads of 128 (64 workgroups uncut) 30.3 / 23.2 / 20.5 / 28.5; 64 of 91 - 8191, 4 kv
+	// heads of 64 (256) 39.3 / 46.2 / 54.1 / 68.9; 24 of 13.9 - 16.4k (192) 136 / 157 / 144 / 151; 16 under a window of 1024 (256) 14.3 / 27.7 / 30.4 / 30.6.
 	const int nw = p->head_dim <= 128 ? 8 : 4;
 	c.nw = nw, c.tiles = (int)((rows + 15) / 16);
 	const long long wgs = base * c.tiles, seen = pages(16);

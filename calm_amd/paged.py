@@ -398,8 +398,8 @@ def _table(pool, table, refs):
 
 
 def reserve(pool: KvPool, table, refs, lens, lens_new) -> None:
-    """pages for tokens lens[r] .. lens_new[r] - 1 of every row of the table, in place; refs[p] counts the rows that list page p.  A row that was cut back into a
-    page of other rows' gets its own, with the old one's tokens"""
+    """pages for tokens lens[r] .. lens_new[r] - 1 of every row of the table, in place; refs[p] counts the rows that list page p.  These pages are the row's own
+    then: one that was cut back gives up pages that other rows list, too, for others, with the tokens that it keeps"""
     n, mp = _table(pool, table, refs)
     _array(lens, "lens", ("int32",), (n,))
     _array(lens_new, "lens_new", ("int32",), (n,))

@@ -271,9 +271,9 @@ int kv_attend_hip(const struct KvPool* pool, const struct KvBatch* batch, int la
 
 /* The upkeep of pages.  refs[p] = how many table rows list page p (int [n_pages], 0: free); a page that tokens go into belongs to one row.
  * Up to 2048 table rows, 2^30 entries and pages.  Free pages are taken lowest first, rows in order.
- *   reserve  entries of the pages that tokens lens[r] .. lens_new[r] - 1 of row r need (in place).  Where row r was cut back into a page that other rows list,
- *            too, that is a page of its own, which takes the old one's bytes in all layers, or -1 and status 2 if none is free.  A page that
- *            holds tokens already and is missing stays so: status 1
+ *   reserve  entries of the pages that tokens lens[r] .. lens_new[r] - 1 of row r need (in place).  They are the row's own from then on: where it was cut
+ *            back and lists pages that other rows list, too, it gives them up for others, the one its tokens end in with its bytes in all layers (-1 and
+ *            status 2 where none is free).  A page that holds tokens already and is missing stays so: status 1
  *   trim     gives up pages behind lens[r] (0: all of them) and, with a window > 0, those that no later token sees (in place)
  *   fork     row r becomes a copy of row parents[r] (out of place: table_out, refs_out; refs_out may be refs): full pages are shared, a
  *            page that is not full stays with its row's first child and is copied, in all layers, for the others; rows without a

@@ -416,6 +416,29 @@ def test_reserve_does_not_make_up_a_page_that_is_lost(hiplib):
         pool.check()
 
 
+@pytest.mark.gpu
+def test_every_page_that_a_row_goes_on_in_is_its_own(hiplib):
+    """a row that was cut back without giving its pages up: those behind its tokens are the others', too, and are not written"""
+    rng = np.random.default_rng(43)
+    pool = paged.KvPool(2, 12, 1, 64)
+    want = fill(pool, rng)
+    # three rows of four shared pages (256 tokens)
+    table, refs = dev(np.array([[0, 1, 2, 3, -1]] * 3, dtype=np.int32)), dev(np.array([3, 3, 3, 3] + [0] * 8, dtype=np.int32))
+    # row 0 goes on from 70 to 200 tokens, row 1 from 128 to 129, row 2 stays
+    paged.reserve(pool, table, refs, ints([70, 128, 256]), ints([200, 129, 256]))
+    np.testing.assert_array_equal(table.numpy(), [[0, 4, 5, 6, -1], [0, 1, 7, 3, -1], [0, 1, 2, 3, -1]])
+    np.testing.assert_array_equal(refs.numpy(), [3, 2, 1, 2, 1, 1, 1, 1, 0, 0, 0, 0])
+    for x in want:
+        x[:, 4] = x[:, 1]  # (tokens 64 .. 69 of row 0; nothing of the other pages is a token of it)
+    for got, x in zip((pool.k, pool.v, pool.k_scale, pool.v_scale), want):
+        np.testing.assert_array_equal(got.numpy(), x)
+    # the last two that list page 3 both go on in it: both give it up, and the lower row takes it as the lowest free page
+    paged.reserve(pool, table, refs, ints([192, 192, 192]), ints([192, 200, 193]))
+    np.testing.assert_array_equal(table.numpy(), [[0, 4, 5, 6, -1], [0, 1, 7, 3, -1], [0, 1, 2, 8, -1]])
+    np.testing.assert_array_equal(refs.numpy(), [3, 2, 1, 1, 1, 1, 1, 1, 1, 0, 0, 0])
+    pool.check()
+
+
 # ---- selection ------------------------------------------------------------------------------------------------------------------------
 
 
