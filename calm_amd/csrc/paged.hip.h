@@ -487,38 +487,60 @@ __device__ __forceinline__ int kv_row_exp(float top) {
 	return e > 126 ? 126 : e;
 }
 
-// Two references a row, whole numbers both: m follows x_j, mv follows x_j + v_j (v_j: the exponent field of V's scale), each over the tokens that
-// the row itself sees.  Sums of weights are relative to 2^m; what goes into the product with V's codes is y_j = 2^(x_j + v_j - mv + KV_LIFT), so
-// nothing that a row does not see, or gives no weight, takes bits from it, however large its V.  A block's share of the sum of weights is
-// that of its y, times 2^k, k = mv - KV_LIFT - m - v.  k is held between -126 and KV_REACH: above, V is 2^-53 of what the row's output is made of and
-// takes part as if it were no smaller; below, the weight is 2^-118 of the largest and nothing in 32 bits.  The references stay unless one is passed by
-// 2^8 (weights up to 2^8 are no less exact, and sums are seldom rescaled), and then both follow, so that k is what V's scales make it: -7 for equal
-// ones, and up to KV_NEAR where the rounded weights may stand for the weights (fp16).  y <= 2^15 is inside binary16; KV_LIFT moves its subnormals away.
+// A row's references, whole numbers both: m follows the scores x_j, m + g follows x_j + v_j (v_j: the exponent field of V's scale), each over the
+// tokens that the row itself sees.  Sums of weights are relative to 2^m; what goes into the product with V's codes is y_j = 2^(x_j + v_j - m - g + KV_LIFT),
+// so nothing that a row does not see, or gives no weight, takes bits from it, however large its V.  A block's share of the sum of weights is that of
+// its y, times 2^k, k = g - KV_LIFT - v.  k is KV_REACH at most: beyond, V is 2^-53 of what the row's output is made of and takes part as if it were no
+// smaller.  The references stay unless one is passed by 2^8 (weights up to 2^8 are no less exact, and sums are seldom rescaled), and then both follow, so
+// that k is what V's scales make it: -7 for equal ones, and up to KV_NEAR where the rounded weights may stand for the weights (fp16).  y <= 2^15 is inside
+// binary16; KV_LIFT moves its subnormals away.  Scores of 2^20 and more take their differences from m before anything small is added (kv_far_score).
 constexpr float KV_LIFT = 7.f, KV_REACH = 60.f, KV_NEAR = -2.f;
+// A row's tokens lie in several lanes.  Each keeps what it has met itself; the row's is put together (`join`: the maximum over its lanes) where a lane
+// asks for a move, so that a page that moves nothing takes no trip across the lanes and one branch.
+constexpr float KV_LOW = -3e38f, KV_NO_GAP = -1000.f; // no token seen yet
 struct KvRefs {
-	float m, mv, rm, rv, gap, m0, mv0;
-	bool moved;
-	__device__ __forceinline__ KvRefs(float m0_, float mv0_, float top, float topv) : m0(m0_), mv0(mv0_) {
-		moved = top > m0 + 8.f || topv > mv0 + 8.f;
-		m = moved ? ceilf(top) : m0, mv = moved ? ceilf(topv) : mv0;
-		rm = m == -__builtin_inff() ? 0.f : m, rv = mv == -__builtin_inff() ? 0.f : mv; // (no token seen yet)
-		gap = rv - KV_LIFT - rm;
+	float m = KV_LOW, g = KV_NO_GAP;                       // the references
+	float top = -__builtin_inff(), tv = -__builtin_inff(); // the largest x_j that the lane met, the largest x_j - m + v_j
+	bool far = false;                                      // (of the wave) a score's last place is near a weight's size
+	// the lane's largest score of a page, and its largest x_j - m + v_j
+	__device__ __forceinline__ bool asks(float x, float v) {
+		top = fmaxf(top, x);
+		return top > m + 8.f || v > g + 8.f;
 	}
-	__device__ __forceinline__ float of_l() const { // what rescales the sums (m0 = -inf: 0)
-		return kv_exp2(m0 - rm);
+	__device__ __forceinline__ float shift(bool to_top, float& l) {
+		const float to = to_top ? ceilf(top) : m, d = m - to;
+		m = to, g += d, l *= kv_exp2(d);
+		return d;
 	}
-	__device__ __forceinline__ float of_o() const {
-		return kv_exp2(mv0 - rv);
+	// the references after a page in which some row's asked for it -> what multiplies the products' sums.  again(m): the page's largest x_j - m + v_j
+	template <class J, class A>
+	__device__ __forceinline__ float follow(float& l, J join, A again) {
+		top = join(top);
+		bool rose = top > m + 8.f;
+		tv += shift(rose, l);
+		tv = join(fmaxf(tv, again(m)));
+		rose = rose || tv > g + 8.f;
+		tv += shift(rose, l);
+		const float gap = rose ? ceilf(tv) : g, by = kv_exp2(g - gap);
+		g = gap;
+		far = __ballot(m != KV_LOW && !(fabsf(m) < 1048576.f)) != 0;
+		return by;
 	}
 };
+// x - m with x the product as it was compared (not fused: in the last place of a large score there is room for more than a weight)
+__device__ __forceinline__ float kv_far_score(float sc, float f, float m) {
+#pragma clang fp contract(off)
+	const float x = sc * f;
+	return x - m;
+}
 // acc + the two binary16 numbers of a word
 __device__ __forceinline__ float kv_add2(float acc, unsigned h2) {
 	const kv_f16x2 one = {(_Float16)1.f, (_Float16)1.f};
 	return __builtin_amdgcn_fdot2(__builtin_bit_cast(kv_f16x2, h2), one, acc, false);
 }
-// sum of y_j V_j over the sum of weights, with V's scale back in
-__device__ __forceinline__ float kv_result(float y, float rm, float rv) {
-	return __builtin_amdgcn_ldexpf(y, (int)(rv - 127.f - KV_LIFT - rm));
+// sum of y_j V_j over the sum of weights, with V's scale back in (g: finite)
+__device__ __forceinline__ float kv_result(float y, float g) {
+	return __builtin_amdgcn_ldexpf(y, (int)(g - 127.f - KV_LIFT));
 }
 
 // the result of a row, or its part of a split: a quad of dims
@@ -576,7 +598,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		if (!direct && wave == 0 && g == 0) { // a range without pages: marked empty for k_kv_merge
 			if (live) {
 				float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
-				p[0] = -__builtin_inff(), p[1] = 0.f, p[2] = -__builtin_inff();
+				p[0] = KV_LOW, p[1] = 0.f, p[2] = KV_NO_GAP;
 			}
 		}
 		return;
@@ -700,7 +722,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 	}
 	kv_f32x4 o[ND];
-	float m = -__builtin_inff(), mv = m, top = m, topv = m, l = 0.f; // (top, topv: the largest met, which the references trail)
+	KvRefs ref;
+	float l = 0.f;
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
 		o[d] = (kv_f32x4){0.f, 0.f, 0.f, 0.f};
@@ -757,6 +780,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		// every token of the page seen by every row of the tile?
 		const bool whole = j0 + KV_PAGE - 1 <= p_min && (a.window <= 0 || j0 > p_max - a.window || j0 + KV_PAGE <= a.sinks);
 		float least = 255.f; // the smallest V scale that this lane's tokens have (behind the row's mask a scale may be anything)
+		float xb[4], top = -__builtin_inff();
 #pragma unroll
 		for (int t = 0; t < 4; ++t) {
 			const float f = kscale[t] * qf;
@@ -776,25 +800,42 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 				x = fmaxf(hi, lo); // (a negative factor turns them round)
 				kscale[t] = f;
 			}
-			top = fmaxf(top, x), topv = fmaxf(topv, x + lv[t]);
+			xb[t] = x;
+			top = fmaxf(top, x);
 			least = fminf(least, x > -__builtin_inff() ? lv[t] : 255.f);
 		}
-		top = kv_max32(kv_max16(top)), topv = kv_max32(kv_max16(topv));
-		const KvRefs ref(m, mv, top, topv);
-		if (__ballot(ref.moved)) {
-			l *= ref.of_l();
-			const float by = ref.of_o();
+		const auto join = [](float x) { return kv_max32(kv_max16(x)); };
+		const auto largest = [&](float m) {
+			return fmaxf(fmaxf((xb[0] - m) + lv[0], (xb[1] - m) + lv[1]), fmaxf((xb[2] - m) + lv[2], (xb[3] - m) + lv[3]));
+		};
+		const float tv = largest(ref.m);
+		bool far = false;
+		if (__ballot(ref.asks(top, tv)) || ref.far) {
+			const float by = ref.follow(l, join, largest);
 #pragma unroll
 			for (int d = 0; d < ND; ++d) {
 				o[d] *= by;
 			}
+			if (ref.far) {
+				far = true;
+#pragma unroll
+				for (int t = 0; t < 4; ++t) {
+#pragma unroll
+					for (int e = 0; e < 4; ++e) {
+						sc[t][e] = kv_far_score(sc[t][e], kscale[t], ref.m);
+					}
+					kscale[t] = 1.f;
+				}
+			}
+		} else {
+			ref.tv = fmaxf(ref.tv, tv);
 		}
-		m = ref.m, mv = ref.mv;
+		const float rm = far ? 0.f : ref.m, gap = ref.g - KV_LIFT;
 		kv_f16x8 pf[2], pl[HL ? 2 : 1];
 		const auto weigh = [&](auto rounded) {
 #pragma unroll
 			for (int t = 0; t < 4; ++t) {
-				const float k = __builtin_amdgcn_fmed3f(ref.gap - lv[t], -126.f, KV_REACH), from = -(ref.rm + k);
+				const float k = fminf(gap - lv[t], KV_REACH), from = -(rm + k);
 				float sum = 0.f;
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
@@ -812,7 +853,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 				l = __builtin_fmaf(sum, kv_exp2(k), l);
 			}
 		};
-		if (DT == KV_F16 && !__ballot(ref.gap > least + KV_NEAR)) {
+		if (DT == KV_F16 && !__ballot(gap > least + KV_NEAR)) {
 			weigh(std::integral_constant<bool, DT == KV_F16>());
 		} else {
 			weigh(std::false_type());
@@ -843,7 +884,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		*(kv_f32x4*)(p + 16 * d + 4 * g) = o[d];
 	}
 	if (g == 0) {
-		p[D] = m, p[D + 1] = l, p[D + 2] = mv;
+		p[D] = ref.m, p[D + 1] = l, p[D + 2] = ref.g;
 	}
 	__syncthreads();
 	// a thread per (row, quad of dims)
@@ -854,17 +895,21 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 		}
 		const float* const p = kv_lds + rr * (D + 4);
 		constexpr int W = 16 * (D + 4);
-		float M = -__builtin_inff(), MV = M;
+		float M = KV_LOW, G = KV_NO_GAP, gw[NW];
 #pragma unroll
 		for (int w = 0; w < NW; ++w) {
-			M = fmaxf(M, p[w * W + D]), MV = fmaxf(MV, p[w * W + D + 2]);
+			M = fmaxf(M, p[w * W + D]);
 		}
-		const float rm = M == -__builtin_inff() ? 0.f : M, rv = MV == -__builtin_inff() ? 0.f : MV;
+#pragma unroll
+		for (int w = 0; w < NW; ++w) { // the waves' second references, from M
+			gw[w] = (p[w * W + D] - M) + p[w * W + D + 2];
+			G = fmaxf(G, gw[w]);
+		}
 		float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 		for (int w = 0; w < NW; ++w) {
-			const float fo = kv_exp2(p[w * W + D + 2] - rv);
-			L += kv_exp2(p[w * W + D] - rm) * p[w * W + D + 1];
+			const float fo = kv_exp2(gw[w] - G);
+			L += kv_exp2(p[w * W + D] - M) * p[w * W + D + 1];
 			const kv_f32x4 x = *(const kv_f32x4*)(p + w * W + d);
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
@@ -879,13 +924,13 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void k_kv_decode(KvAttnA
 			const float f = L == 0.f ? (blind ? 0.f : __builtin_nanf("")) : 1.f / L;
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
-				y[e] = kv_result(y[e] * f, rm, rv);
+				y[e] = kv_result(y[e] * f, G);
 			}
 		}
 		kv_put<D, DT>(a, direct, at, split, d, y);
 		if (d == 0 && a.n_splits > 1) {
 			float* const pm = a.part + (at * a.n_splits + split) * (D + 4) + D;
-			pm[0] = M, pm[1] = direct ? -1.f : L == 0.f && !blind ? -0.f : L, pm[2] = MV; // (no sum of weights is negative: the row is written already)
+			pm[0] = M, pm[1] = direct ? -1.f : L == 0.f && !blind ? -0.f : L, pm[2] = G; // (no sum of weights is negative: the row is written already)
 		}
 	}
 }
@@ -901,18 +946,19 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 		return; // rows behind the last sequence stay as they are
 	}
 	const float* const p = a.part + row * a.n_splits * (D + 4);
-	float m = -__builtin_inff(), mv = m, l = 0.f;
+	float m = KV_LOW, g = KV_NO_GAP, l = 0.f;
 	if (lane < a.n_splits) {
-		m = p[(size_t)lane * (D + 4) + D], l = p[(size_t)lane * (D + 4) + D + 1], mv = p[(size_t)lane * (D + 4) + D + 2];
+		m = p[(size_t)lane * (D + 4) + D], l = p[(size_t)lane * (D + 4) + D + 1], g = p[(size_t)lane * (D + 4) + D + 2];
 	}
 	const int l0 = __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), 0); // (the first range's)
 	if (__builtin_bit_cast(float, l0) < 0.f) {
 		return; // one range: written by its workgroup
 	}
-	const bool empty = m == -__builtin_inff() && l == 0.f;
-	const float M = wave_max_dpp(m), MV = wave_max_dpp(mv);
-	const float rm = M == -__builtin_inff() ? 0.f : M, rv = MV == -__builtin_inff() ? 0.f : MV;
-	const float L = wave_sum(empty ? 0.f : kv_exp2(m - rm) * l), w = kv_exp2(mv - rv);
+	const bool empty = m == KV_LOW && l == 0.f;
+	const float M = wave_max_dpp(m);
+	g += m - M; // (from M)
+	const float G = wave_max_dpp(g);
+	const float L = wave_sum(empty ? 0.f : kv_exp2(m - M) * l), w = kv_exp2(g - G);
 	const unsigned long long some = __ballot(!empty);
 	constexpr int N = (D + 255) / 256;
 	const int d = lane * 4;
@@ -934,7 +980,7 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 		const float f = L == 0.f ? (l0 < 0 ? __builtin_nanf("") : 0.f) : 1.f / L; // (-0: tokens seen, no score in range)
 #pragma unroll
 		for (int e = 0; e < 4; ++e) {
-			y[e] = kv_result(y[e] * f, rm, rv);
+			y[e] = kv_result(y[e] * f, G);
 		}
 		kv_store4<DT>(a.out, row * D + d, y);
 	}
@@ -1021,7 +1067,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	if (i0 >= i1 && split > 0) {
 		if (!direct && live && hh == 0) {
 			float* const p = a.part + (row_of(rr) * a.n_splits + split) * (D + 4) + D;
-			p[0] = -__builtin_inff(), p[1] = 0.f, p[2] = -__builtin_inff();
+			p[0] = KV_LOW, p[1] = 0.f, p[2] = KV_NO_GAP;
 		}
 		return;
 	}
@@ -1064,7 +1110,8 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			}
 		}
 	}
-	float m = -__builtin_inff(), mv = m, top = m, topv = m, l = 0.f; // (top, topv: the largest met, which the references trail)
+	KvRefs ref;
+	float l = 0.f;
 	kv_f32x16 o[ND], zero;
 #pragma unroll
 	for (int e = 0; e < 16; ++e) {
@@ -1212,6 +1259,7 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 				}
 			}
 			int least = 255; // (as in k_kv_decode)
+			float xb[4], top = -__builtin_inff();
 #pragma unroll
 			for (int b = 0; b < 4; ++b) {
 				float t = -__builtin_inff();
@@ -1219,21 +1267,43 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 				for (int e = 0; e < 8; ++e) {
 					t = fmaxf(t, sc[b >> 1][8 * (b & 1) + e]);
 				}
-				t *= f[b];
-				top = fmaxf(top, t), topv = fmaxf(topv, t + (float)lv[b]);
-				least = min(least, t > -__builtin_inff() ? lv[b] : 255);
+				xb[b] = t * f[b];
+				top = fmaxf(top, xb[b]);
+				least = min(least, xb[b] > -__builtin_inff() ? lv[b] : 255);
 			}
-			top = kv_max32(top), topv = kv_max32(topv);
-			const KvRefs ref(m, mv, top, topv);
-			m = ref.m, mv = ref.mv;
-			l *= ref.of_l();
-			const float by = ref.of_o();
-			const int gap = (int)ref.gap;
+			const auto join = [](float x) { return kv_max32(x); };
+			const auto largest = [&](float m) {
+				return fmaxf(fmaxf((xb[0] - m) + (float)lv[0], (xb[1] - m) + (float)lv[1]), fmaxf((xb[2] - m) + (float)lv[2], (xb[3] - m) + (float)lv[3]));
+			};
+			const float tv = largest(ref.m);
+			bool far = false;
+			if (__ballot(ref.asks(top, tv)) || ref.far) {
+				const float by = ref.follow(l, join, largest);
+#pragma unroll
+				for (int d = 0; d < ND; ++d) {
+					o[d] *= by;
+				}
+				if (ref.far) {
+					far = true;
+#pragma unroll
+					for (int b = 0; b < 4; ++b) {
+#pragma unroll
+						for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; ++e) {
+							sc[b >> 1][e] = kv_far_score(sc[b >> 1][e], f[b], ref.m);
+						}
+						f[b] = 1.f;
+					}
+				}
+			} else {
+				ref.tv = fmaxf(ref.tv, tv);
+			}
+			const float rm = far ? 0.f : ref.m;
+			const int gap = (int)(ref.g - KV_LIFT);
 			const auto weigh = [&](auto rounded) {
 #pragma unroll
 				for (int b = 0; b < 4; ++b) {
-					const int k = min(max(gap - lv[b], -126), (int)KV_REACH);
-					const float from = -(ref.rm + (float)k);
+					const int k = min(gap - lv[b], (int)KV_REACH);
+					const float from = -(rm + (float)k);
 					float sum = 0.f;
 #pragma unroll
 					for (int e = 0; e < 8; ++e) {
@@ -1248,19 +1318,13 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 						const u32x4 w = __builtin_bit_cast(u32x4, pf[b]);
 						sum = kv_add2(kv_add2(kv_add2(kv_add2(0.f, w[0]), w[1]), w[2]), w[3]);
 					}
-					l = __builtin_fmaf(sum, kv_exp2i(k), l);
+					l = __builtin_fmaf(sum, kv_exp2i(max(k, -126)), l);
 				}
 			};
 			if (DT == KV_F16 && !__ballot(gap > least + (int)KV_NEAR)) {
 				weigh(std::integral_constant<bool, DT == KV_F16>());
 			} else {
 				weigh(std::false_type());
-			}
-			if (__ballot(ref.moved)) {
-#pragma unroll
-				for (int d = 0; d < ND; ++d) {
-					o[d] *= by;
-				}
 			}
 			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1291,7 +1355,6 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 	}
 	const size_t row = row_of(again);
 	const bool blind = l == 0.f && len - n + again / a.group < 0;
-	const float rm = m == -__builtin_inff() ? 0.f : m, rv = mv == -__builtin_inff() ? 0.f : mv;
 	const float f = l == 0.f ? (blind ? 0.f : __builtin_nanf("")) : 1.f / l;
 #pragma unroll
 	for (int d = 0; d < ND; ++d) {
@@ -1300,14 +1363,14 @@ __global__ __launch_bounds__(256, D > 128 || (DT == KV_F32 && D > 64) ? 1 : 2) v
 			float y[4];
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
-				y[e] = direct ? kv_result(o[d][4 * q + e] * f, rm, rv) : o[d][4 * q + e];
+				y[e] = direct ? kv_result(o[d][4 * q + e] * f, ref.g) : o[d][4 * q + e];
 			}
 			kv_put<D, DT>(a, direct, row, split, 32 * d + 8 * q + 4 * hh, y);
 		}
 	}
 	if (hh == 0 && a.n_splits > 1) {
 		float* const p = a.part + (row * a.n_splits + split) * (D + 4) + D;
-		p[0] = m, p[1] = direct ? -1.f : l == 0.f && !blind ? -0.f : l, p[2] = mv; // (as above)
+		p[0] = ref.m, p[1] = direct ? -1.f : l == 0.f && !blind ? -0.f : l, p[2] = ref.g; // (as above)
 	}
 }
 

@@ -122,6 +122,32 @@ def test_a_row_that_weighs_one_token_returns_its_value(hiplib, dtype, rows, toke
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,tokens", [(1, 300), (45, 300), (1, 4100), (45, 4100)])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 22, 2.0 ** 26, 2.0 ** 60, 2.0 ** 110])
+def test_huge_scores_pick_their_token_whatever_the_scales(hiplib, dtype, rows, tokens, size):
+    """one token's score `size` above the others', among V's of very different scales, up to where fp32 ends: the output is that token's V (as above); where K is turned
+    round, at -size, the output is that of the sequence without it"""
+    if dtype == "float16" and size > 2.0 ** 22:
+        pytest.skip("queries of fp16 and keys of int8 do not reach that far")
+    r = Rig(1, tokens, 1, 64, np.random.default_rng(39))
+    at = tokens // 3
+    k = np.zeros((tokens, 1, 64))
+    k[at, 0] = np.where(r.rng.random(64) < 0.5, 1.0, -1.0) * size ** 0.5
+    v = r.rng.standard_normal((tokens, 1, 64)) * np.repeat(2.0 ** r.rng.integers(-9, 10, -(-tokens // 16)), 16)[:tokens, None, None]
+    r.add([tokens], "float32", k=to_type(k, "float32"), v=to_type(v, "float32"))
+    q = to_type(np.sign(k[at, 0]) * np.ones((rows, 4, 1)) * size ** 0.5 / 8, dtype)
+    vv = r.v.values(0)[:, 0]
+    got = from_type(paged.attend(r.pool, r.batch([rows]), dev(q, dtype)).numpy(), dtype)
+    np.testing.assert_allclose(got, np.broadcast_to(vv[at], got.shape), rtol=2.0 ** -21 if dtype == "float32" else 0, atol=1e-9 * np.abs(vv[at]).max())
+    got = from_type(paged.attend(r.pool, r.batch([rows]), dev(to_type(-from_type(q, dtype), dtype), dtype)).numpy(), dtype)
+    left = np.arange(tokens) != at
+    for t in range(rows):
+        want = vv[left & (np.arange(tokens) <= tokens - rows + t)].mean(axis=0)
+        assert np.abs(got[t] - want).max() <= (2.0 ** -9 + U[dtype]) * np.abs(vv).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 40])
 def test_what_lies_behind_the_tokens_does_not_matter(hiplib, dtype, rows):
     """the same bits whatever the pages hold behind a sequence's tokens, in rows and blocks of one tile that some rows do not see, and in pages of nobody"""
@@ -234,6 +260,26 @@ def test_zeros_and_the_smallest_and_largest_scales(hiplib, rows):
         want = attention(q.astype(np.float64), one.k.values(0), one.v.values(0), 0.125, 0, 0)
         err = np.abs(got - want) / max(np.abs(v[lo:hi]).max(), 1e-37)
         assert err.max() <= 2.0 ** -9 and (err ** 2).mean() ** 0.5 <= 2e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 50])
+def test_values_beyond_any_weight(hiplib, rows):
+    """V's 2^122 apart, the large ones under a weight of 2^-115: the output is made of both"""
+    dim, rng = 64, np.random.default_rng(42)
+    r = Rig(1, 300, 1, dim, rng)
+    u = np.where(rng.random(dim) < 0.5, 1.0, -1.0)
+    k, v = np.zeros((300, 1, dim)), rng.standard_normal((300, 1, dim)) * 2.0 ** -20
+    k[64:80] = u * -(115 * np.log(2) / 8)  # q . K * dim ** -0.5 = -115 ln 2 for q = u
+    v[64:80] *= 2.0 ** 122
+    r.add([300], "float32", k=to_type(k, "float32"), v=to_type(v, "float32"))
+    q = to_type(np.broadcast_to(u, (rows, 2, dim)), "float32")
+    got = paged.attend(r.pool, r.batch([rows]), dev(q)).numpy().astype(np.float64)
+    x, kv, vv = q.astype(np.float64), r.k.values(0), r.v.values(0)
+    want, size = attention(x, kv, vv, dim ** -0.5, 0, 0), weighted_size(x, kv, vv, dim ** -0.5, 0, 0)
+    err = np.abs(got - want) / size[..., None]
+    # (a score of 80 is off by 80 * 2^-24 times a few: 1e-5 of its weight)
+    assert err.max() <= 2.0 ** -9 + U["float32"] and (err ** 2).mean() ** 0.5 <= 2e-5, err.max()
 
 
 # ---- batches that do not add up -------------------------------------------------------------------------------------------------------
