@@ -989,11 +989,11 @@ __global__ __launch_bounds__(256) void k_kv_merge(KvAttnArgs a) {
 // Many rows (a prompt chunk).  A workgroup takes 128 rows (32 per wave) of one sequence and kv head and walks
 // the pages they see; a page's codes become binary16 ONCE per workgroup on their way into LDS (two buffers: the next page's loads are in
 // flight while a page is computed), laid out so that every operand is one 16-byte read of consecutive lanes.
-// Measured: 2049 rows of 32 heads (8 kv heads of 128) on 4099 tokens 162 - 172 us = 620 TFLOP/s; five ragged chunks of up to 1021 rows of 32 heads
-// (4 kv heads of 64) behind a window of 2048 75 us.  What bounds it is the chain of pages of the heaviest tiles (65, 49 on average; 2.5 us each): of the first
-// shape's 387k cycles the matrix unit is busy 100k and vector instructions issue 161k, with 1.32 of two possible waves on a SIMD on average -- light
+// Measured: 2049 rows of 32 heads (8 kv heads of 128) on 4099 tokens 169 - 174 us = 600 TFLOP/s; five ragged chunks of up to 1021 rows of 32 heads
+// (4 kv heads of 64) behind a window of 2048 77 us.  What bounds it is the chain of pages of the heaviest tiles (65, 49 on average; 2.6 us each): of the first
+// shape's 395k cycles the matrix unit is busy 100k and vector instructions issue 158k, with 1.31 of two possible waves on a SIMD on average -- light
 // tiles end early, nothing follows them -- and a wave issues 46 % of its time, waits to issue 30 and for memory, LDS and barriers 24.  (Under the
-// window: 200k cycles, 25k and 73k, 1.05 waves.)  Tried and slower: PV of a page with QK of
+// window: 203k cycles, 25k and 73k, 1.07 waves.)  Tried and slower: PV of a page with QK of
 // the next in one phase, the other phase's waves beside it behind barriers (eight waves of 256 rows: 199 us; four waves: 181), products of
 // neighbouring pages interleaved within a wave (257 us), light tiles behind heavy ones on a CU (187).
 // grid = row tiles x seqs x splits x kv heads

@@ -66,4 +66,20 @@ with fwd.dual_level():
 assert torch.equal(paged.attend(pool, batch, q), want)
 refused(lambda: paged.KvPool.over(pool.k, pool.v, pool.k_scale.clone().requires_grad_(), pool.v_scale), "no backward")
 print("forward mode", flush=True)
+
+# from a selection to a fork: the beams of a group as rows of the table
+groups, width = 2, 3
+table6 = torch.arange(12, dtype=torch.int32, device="cuda").view(6, 2)
+pool6 = paged.KvPool(1, 12, 1, 64, device="cuda")
+refs6, lens6 = torch.ones(12, dtype=torch.int32, device="cuda"), ints([128] * 6)
+logits = torch.full((6, 10), -5.0, device="cuda")
+for row, tok in ((2, 4), (2, 5), (0, 6), (4, 1), (4, 2), (4, 3)):
+    logits[row, tok] = 9.0 - tok
+best, beams, tokens, done = paged.beam_select(logits, torch.zeros((groups, width), device="cuda"))
+parents = (beams + torch.arange(0, groups * width, width, dtype=torch.int32, device="cuda")[:, None]).view(-1)
+t2, r2 = paged.fork(pool6, table6, lens6, refs6, parents)
+assert torch.equal(t2, table6[parents.long()]) and parents.tolist()[3:] == [4, 4, 4] and set(parents.tolist()[:3]) <= {0, 1, 2}
+assert torch.equal(r2, torch.bincount(t2.flatten().long(), minlength=12).to(torch.int32))
+pool6.check()
+print("selection to fork", flush=True)
 print("ALL OK")
