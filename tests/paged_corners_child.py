@@ -78,7 +78,9 @@ for row, tok in ((2, 4), (2, 5), (0, 6), (4, 1), (4, 2), (4, 3)):
 best, beams, tokens, done = paged.beam_select(logits, torch.zeros((groups, width), device="cuda"))
 parents = (beams + torch.arange(0, groups * width, width, dtype=torch.int32, device="cuda")[:, None]).view(-1)
 t2, r2 = paged.fork(pool6, table6, lens6, refs6, parents)
-assert torch.equal(t2, table6[parents.long()]) and parents.tolist()[3:] == [4, 4, 4] and set(parents.tolist()[:3]) <= {0, 1, 2}
+# (row 0: one token at 3, -0.0; row 2: 5 and 4, -0.3 and -1.3; row 4: 8, 7 and 6, -0.4, -1.4 and -2.4; the even rows: -log 10 = -2.3 each)
+assert parents.tolist() == [0, 2, 2, 4, 4, 3]
+assert torch.equal(t2, table6[parents.long()])
 assert torch.equal(r2, torch.bincount(t2.flatten().long(), minlength=12).to(torch.int32))
 pool6.check()
 print("selection to fork", flush=True)
