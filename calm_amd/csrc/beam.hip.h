@@ -11,7 +11,7 @@
 // The sum decides the order of continuations of DIFFERENT beams, where 32 bits lose what matters: sums and totals are 64 bits wide from a
 // lane's 32 values on.  The exponentials are 32 bits (2^-23 each; their errors are not alike and average over the row): all totals of a beam are off by
 // one amount, below 2^-22 and 1e-8 as a rule, and candidates of two beams that are nearer to each other than that may come in either order.
-// Equal rows get equal sums (a value's place in them follows from its index alone), so equal totals stay equal.
+// Rows that are equal, or differ by a constant, get equal sums (a value's place in them follows from its index alone), so equal totals stay equal.
 #pragma once
 
 namespace calm {
@@ -450,8 +450,8 @@ __global__ __launch_bounds__(1024) void k_beam_pick(BeamArgs a) {
 			s += m == (double)BEAM_NONE ? x : x * (double)beam_exp((float)(m - M)); // (a difference of fp32 numbers)
 		}
 		s = beam_wave_sum(s);
-		const double lse = M + log(s), base = (double)a.score[row];
-		const bool dead = !(lse - lse == 0.) || !(base > (double)BEAM_NONE); // not finite (NaN included)
+		const double ls = log(s), base = (double)a.score[row];
+		const bool dead = !(M + ls - (M + ls) == 0.) || !(base > (double)BEAM_NONE); // not finite (NaN included)
 		if (dead) {
 			if (lane < W) {
 				sm_t[w * W + lane] = (double)BEAM_NONE, sm_i[w * W + lane] = lane < a.vocab ? lane : -1;
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(1024) void k_beam_pick(BeamArgs a) {
 			__builtin_amdgcn_wave_barrier();
 		}
 		if (lane < W) {
-			sm_t[w * W + lane] = bi < 0 ? (double)BEAM_NONE : base + ((double)bv - lse);
+			sm_t[w * W + lane] = bi < 0 ? (double)BEAM_NONE : base + (((double)bv - M) - ls); // (a constant on all of a row's logits leaves no trace)
 			sm_i[w * W + lane] = bi;
 		}
 	}

@@ -518,6 +518,22 @@ def test_select_refuses_vocabularies_beyond_its_indexes(hiplib):
     assert hiplib.beam_workspace_hip(1, 1, (1 << 30) + 1) == -1 and b"2^30 tokens" in hiplib.calm_hip_error()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("beams,vocab", [(8, 500), (5, 9001)])
+def test_select_beams_whose_logits_differ_by_a_constant(hiplib, dtype, beams, vocab):
+    """a constant on all of a row's logits changes no log softmax: the totals are equal still, and the lowest beam comes first"""
+    rng = np.random.default_rng(beams)
+    x = np.repeat(rng.integers(-8, 9, (6, 1, vocab)).astype(np.float64), beams, axis=1).reshape(6 * beams, vocab)
+    scores = np.repeat(-3 * rng.random((6, 1)), beams, axis=1)
+    shifted = to_type(x + np.tile(rng.permutation(np.arange(beams)), 6)[:, None] * 16, dtype)  # (whole numbers below 256: exact in every type)
+    want = paged.beam_select(dev(to_type(x, dtype), dtype), dev(scores.astype(np.float32)))
+    got = paged.beam_select(dev(shifted, dtype), dev(scores.astype(np.float32)))
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a.numpy(), b.numpy())
+    check_select(x, scores, None, -1, dtype)
+
+
 # ---- handles and streams --------------------------------------------------------------------------------------------------------------
 
 
